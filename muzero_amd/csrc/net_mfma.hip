@@ -433,9 +433,9 @@ __device__ __forceinline__ void ln_apply(const f32x16& v, float mean, float rstd
 }
 
 // Packed variant: o[j] = 16-bit pair of relu(LN(v)) rows (2j, 2j+1).
-// bf16 operands: per element half a v_pk_fma_f32 (normalise), one v_fma_mix_f32 (fp16 gamma/beta), half a v_cvt_pk_bf16_f32
-// and half a v_pk_max_i16 (ReLU on the packed pair: a negative bf16 is a negative int16) = 2.5 instructions.
-// fp16 operands: half a v_pk_fma_f32 and one v_fma_mixlo/mixhi_f16 with the clamp modifier = 1.5 instructions: the mix-FMA
+// bf16 operands: per element one v_fma_f32 (normalise; packed fp32 forms are off), one v_fma_mix_f32 (fp16 gamma/beta), half a v_cvt_pk_bf16_f32
+// and half a v_pk_max_i16 (ReLU on the packed pair: a negative bf16 is a negative int16) = 3 instructions.
+// fp16 operands: one v_fma_f32 and one v_fma_mixlo/mixhi_f16 with the clamp modifier = 2 instructions: the mix-FMA
 // rounds straight to the fp16 half of the result register, and its clamp to [0, 1] IS the ReLU because the table holds
 // gamma / S and beta / S (S a power of two >= the largest value the LayerNorm can put out, ln_scale() on the host) and the conv
 // that reads these activations has its weights multiplied by S: the same products bit for bit (power-of-two scaling), except

@@ -1,7 +1,7 @@
 // The chunk loop of the exact-fp32 conv (net_fp32.hip:conv_mfma, MT = 1, NTW = 3) in isolation: 48 x v_mfma_f32_16x16x4_f32 per
 // chunk, A operands by 4 global_load_dwordx4 a chunk ahead, B operands by 3 ds_read_b128 a group ahead.  Variants switch the
 // operand traffic off / make the operands constant to find what keeps a lone wave from 32 cycles per MFMA.
-// Build: hipcc --offload-arch=gfx950 -O3 -o f32_chunk f32_chunk.hip
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o f32_chunk f32_chunk.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -1,5 +1,5 @@
 // Issue rate of the fp32 MFMA shapes on gfx950: cycles (s_memtime) per instruction for 1, 2 and 4 waves per SIMD, each wave
-// running NACC independent accumulators.  Build: hipcc --offload-arch=gfx950 -O3 -o mfma_f32_rate mfma_f32_rate.hip
+// running NACC independent accumulators.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o mfma_f32_rate mfma_f32_rate.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -1,7 +1,7 @@
 #!/bin/bash
 # Register / spill summary of the MFMA kernels (hipcc resource-usage remarks, compacted).
 cd "$(dirname "$0")/../muzero_amd/csrc"
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC "$@" -c net_mfma.hip -o /tmp/nm_regs.o -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c '
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC "$@" -c net_mfma.hip -o /tmp/nm_regs.o -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c '
 import re,sys
 name=None
 for l in sys.stdin:
