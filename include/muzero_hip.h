@@ -252,6 +252,55 @@ int mz_search_moves_injected_noalloc(mz_ctx* ctx, int B, const uint8_t* legal, c
                                      const double* dirichlet, const uint8_t* exploration_time, const double* u,
                                      const mz_move_outputs* out);
 
+/* ---- operators on device tensors -----------------------------------------------------------------------------
+ * No counterpart in the reference (its PlanAction.playAfterJustWithInitialInference, P/agent/c_planning/PlanAction.java:174-193,
+ * draws from the renormalised policy of one network).  Operators a program applies to its own tensors beside the search: no
+ * context is needed, all state is in the arguments.  For each of them
+ *  - every data pointer is memory of ONE device (hipMalloc / managed); the call runs there, whatever device is current, and
+ *    leaves the current device as it was.  Host pointers and pointers of two devices are refused;
+ *  - `stream` is a hipStream_t of that device (NULL: its default stream).  The call queues its kernels there and returns: no
+ *    allocation, no synchronisation, no host copy, so it can be captured into a graph;
+ *  - `workspace` is device memory of at least mz_*_workspace_bytes(args) bytes, 256-byte aligned, that nothing else uses until
+ *    the call's work is done (NULL when that is 0): calls in flight at the same time, and graphs that may run at the same time,
+ *    need one each.  Its contents before and after do not matter;
+ *  - arguments are checked on the host before anything is queued: -1 and mz_last_error(NULL) (per thread) otherwise.  Calls
+ *    from several threads are independent.  Strides are in elements; rows are contiguous; outputs must not overlap inputs;
+ *  - rows == 0 is a successful call that does nothing. */
+enum { MZ_DTYPE_FP32 = 0, MZ_DTYPE_BF16 = 1, MZ_DTYPE_F16 = 2 }; /* the numbers of MZ_PRECISION_* */
+
+/* One action per row of logits, drawn from given random numbers after temperature, top-k, top-p and min-p.
+ * Row z[0..actions), over its legal entries that are not NaN or -inf (masked places may hold anything):
+ *   w_i = exp((z_i - max z) / temperature); ranking: larger z first, lower index first among equals;
+ *   top_k  > 0: the first k of the ranking (0 = off);
+ *   top_p  < 1: of those, the entries whose predecessors hold less than top_p of those k's weight (1 = off);
+ *   min_p  > 0: of those, the entries with w_i >= min_p (0 = off); the first of the ranking always stays;
+ *   action = the first kept entry in INDEX order at which the running sum of w exceeds u * (sum of the kept), u in [0, 1].
+ *   temperature == 0: the first of the ranking, whatever u.  +inf entries share all the weight.
+ * A row with no such entry, and a row whose u or per-row parameter is out of range or NaN, gets action -1, kept 0, logprob 0
+ * and probs 0.  Weights and sums are 64-bit; a row's result does not depend on the other rows. */
+typedef struct mz_sample_args {
+    int32_t rows, actions;          /* actions: 1 .. 262144 */
+    int32_t dtype;                  /* MZ_DTYPE_* of logits */
+    int32_t top_k;
+    double temperature, top_p, min_p;
+    const void* logits;             /* [rows][actions], row_stride */
+    int64_t row_stride;             /* >= 0 (0: all rows share one) */
+    const uint8_t* legal;           /* [rows][actions], legal_stride; 0 = masked; NULL = all legal */
+    int64_t legal_stride;
+    const double* u;                /* [rows] */
+    const double* row_temperature;  /* [rows] each, or NULL: the scalar above for every row */
+    const int32_t* row_top_k;
+    const double* row_top_p;
+    const double* row_min_p;
+    int32_t* action;                /* [rows] */
+    float* logprob;                 /* [rows] log of the drawn action's share of the kept weight, or NULL */
+    int32_t* kept;                  /* [rows] number of entries kept, or NULL */
+    float* probs;                   /* [rows][actions], probs_stride: shares of the kept weight, 0 elsewhere; or NULL */
+    int64_t probs_stride;           /* >= actions */
+} mz_sample_args;
+size_t mz_sample_workspace_bytes(const mz_sample_args* args); /* 0 for invalid arguments */
+int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -47,6 +47,15 @@ class MoveOutputs(C.Structure):
         "playout_policy", "playout_appended", "sims_run", "status")]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("actions", C.c_int32), ("dtype", C.c_int32), ("top_k", C.c_int32),
+                ("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("logits", C.c_void_p),
+                ("row_stride", C.c_int64), ("legal", C.c_void_p), ("legal_stride", C.c_int64), ("u", C.c_void_p),
+                ("row_temperature", C.c_void_p), ("row_top_k", C.c_void_p), ("row_top_p", C.c_void_p),
+                ("row_min_p", C.c_void_p), ("action", C.c_void_p), ("logprob", C.c_void_p), ("kept", C.c_void_p),
+                ("probs", C.c_void_p), ("probs_stride", C.c_int64)]
+
+
 EXPORTS = (
     "mz_create", "mz_destroy", "mz_last_error", "mz_set_action_cells", "mz_load_weights", "mz_num_params",
     "mz_weights_device_ptr", "mz_commit_weights", "mz_initial_inference", "mz_recurrent_inference",
@@ -54,7 +63,8 @@ EXPORTS = (
     "mz_tree_num_nodes", "mz_tree_node", "mz_tree_minmax", "mz_set_timing", "mz_get_timing", "mz_get_last_stats",
     "mz_synchronize", "mz_version", "mz_comm_unique_id", "mz_comm_init", "mz_comm_destroy", "mz_broadcast_weights",
     "mz_gather_stats", "mz_comm_barrier", "mz_get_recording_games", "mz_get_gumbel", "mz_seed_gumbel",
-    "mz_child_order", "mz_noalloc_scratch_bytes", "mz_search_moves_injected_noalloc", "mz_set_stream_split")
+    "mz_child_order", "mz_noalloc_scratch_bytes", "mz_search_moves_injected_noalloc", "mz_set_stream_split",
+    "mz_sample_workspace_bytes", "mz_sample_actions")
 NOALLOC_SCRATCH_BYTES = 16 << 20
 COMM_ID_BYTES = 128
 
@@ -109,6 +119,9 @@ def lib():
         L.mz_noalloc_scratch_bytes.argtypes = [vp, C.c_int]
         L.mz_noalloc_scratch_bytes.restype = C.c_size_t
         L.mz_search_moves_injected_noalloc.argtypes = L.mz_search_moves_injected.argtypes
+        L.mz_sample_workspace_bytes.argtypes = [C.POINTER(SampleArgs)]
+        L.mz_sample_workspace_bytes.restype = C.c_size_t
+        L.mz_sample_actions.argtypes = [C.POINTER(SampleArgs), vp, C.c_size_t, vp]
         _lib = L
     return _lib
 

@@ -17,6 +17,7 @@
 
 #include "net.h"
 #include "net_mfma.h"
+#include "ops.h"
 #include "tree.h"
 
 using namespace mz;
@@ -67,6 +68,13 @@ struct EventPair {
 };
 
 }  // namespace
+
+namespace mz {
+int op_fail(const std::string& msg) {   // ops.h: errors of calls without a context
+    g_create_error = msg;
+    return -1;
+}
+}  // namespace mz
 
 struct mz_ctx {
     mz_config cfg{};

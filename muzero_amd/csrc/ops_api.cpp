@@ -1,0 +1,160 @@
+// C entries of the operators on device tensors (include/muzero_hip.h): every check of the arguments, then the launchers of ops.h.
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "../../include/muzero_hip.h"
+#include "ops.h"
+
+using namespace mz;
+
+namespace {
+
+constexpr int kMaxSampleActions = 262144;   // 2^18: sample.hip's histogram masses are sums of 2^46 in 64 bits
+
+// The device all operands live on: the first pointer names it, every other one must agree.
+struct Operands {
+    int device = -1;
+    const char* bad = nullptr;
+    std::string why;
+    void add(const void* p, const char* name, size_t align) {
+        if (bad || !p) return;
+        hipPointerAttribute_t at;
+        if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+            (void)hipGetLastError();
+            fail(name, "is not device memory");
+        } else if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged) {
+            fail(name, "is not device memory");
+        } else if (reinterpret_cast<uintptr_t>(p) % align) {
+            fail(name, "is not aligned to its type");
+        } else if (at.type == hipMemoryTypeDevice) {
+            if (device < 0) device = at.device;
+            else if (device != at.device) fail(name, "is memory of another device");
+        }
+    }
+    void fail(const char* name, const char* what) {
+        bad = name;
+        why = std::string(name) + " " + what;
+    }
+};
+
+struct DeviceGuard {   // runs on `device`, leaves the caller's device as it was
+    int before = -1;
+    hipError_t err;
+    explicit DeviceGuard(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else if (err == hipSuccess) before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+size_t type_bytes(int t) { return t == MZ_DTYPE_FP32 ? 4 : 2; }
+bool known_type(int t) { return t == MZ_DTYPE_FP32 || t == MZ_DTYPE_BF16 || t == MZ_DTYPE_F16; }
+
+// Common end of a call: device and stream, workspace, launch.
+template <typename F>
+int run_op(Operands& o, void* workspace, size_t have, size_t need, void* stream, F launch) {
+    if (need) {
+        if (!workspace || have < need)
+            return op_fail("workspace has " + std::to_string(workspace ? have : 0) + " bytes, needs " + std::to_string(need));
+        o.add(workspace, "workspace", 256);
+    }
+    if (o.bad) return op_fail(o.why);
+    int dev = o.device;
+    if (dev < 0 && hipGetDevice(&dev) != hipSuccess) return op_fail("no HIP device");   // all operands are managed memory
+    DeviceGuard g(dev);
+    if (g.err != hipSuccess) return op_fail(std::string("hipSetDevice: ") + hipGetErrorString(g.err));
+    if (stream) {
+        int sd = -1;
+        if (hipStreamGetDevice(static_cast<hipStream_t>(stream), &sd) != hipSuccess) {
+            (void)hipGetLastError();
+            return op_fail("stream is not a stream");
+        }
+        if (sd != dev) return op_fail("stream is a stream of another device");
+    }
+    const hipError_t e = launch(static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return op_fail(std::string("launch: ") + hipGetErrorString(e));
+    return 0;
+}
+
+const char* check_sample(const mz_sample_args* a) {
+    if (!a) return "args is NULL";
+    if (a->rows < 0) return "rows < 0";
+    if (a->actions < 1 || a->actions > kMaxSampleActions) return "actions must be 1 .. 262144";
+    if (!known_type(a->dtype)) return "unknown dtype";
+    if (!a->row_temperature && !(a->temperature >= 0 && std::isfinite(a->temperature))) return "temperature must be finite and >= 0";
+    if (!a->row_top_k && a->top_k < 0) return "top_k must be >= 0";
+    if (!a->row_top_p && !(a->top_p > 0 && a->top_p <= 1)) return "top_p must be in (0, 1]";
+    if (!a->row_min_p && !(a->min_p >= 0 && a->min_p <= 1)) return "min_p must be in [0, 1]";
+    if (a->row_stride < 0 || (a->legal && a->legal_stride < 0)) return "strides must be >= 0";
+    if (a->probs && a->rows > 1 && a->probs_stride < a->actions) return "probs_stride < actions";
+    if (a->rows > 0 && (!a->logits || !a->u || !a->action)) return "logits, u and action must not be NULL";
+    return nullptr;
+}
+SampleOp sample_op(const mz_sample_args& a) {
+    SampleOp o{};
+    o.rows = a.rows;
+    o.actions = a.actions;
+    o.type = a.dtype;
+    o.logits = a.logits;
+    o.row_stride = a.row_stride;
+    o.legal = a.legal;
+    o.legal_stride = a.legal_stride;
+    o.u = a.u;
+    o.temperature = a.temperature;
+    o.top_p = a.top_p;
+    o.min_p = a.min_p;
+    o.top_k = a.top_k;
+    o.row_temperature = a.row_temperature;
+    o.row_top_k = a.row_top_k;
+    o.row_top_p = a.row_top_p;
+    o.row_min_p = a.row_min_p;
+    o.action = a.action;
+    o.logprob = a.logprob;
+    o.kept = a.kept;
+    o.probs = a.probs;
+    o.probs_stride = a.probs_stride;
+    return o;
+}
+
+// no exception (std::string may throw) crosses the C boundary
+template <typename F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (...) {
+        return -1;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mz_sample_workspace_bytes(const mz_sample_args* args) { return check_sample(args) ? 0 : sample_workspace_bytes(sample_op(*args)); }
+
+int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        if (const char* e = check_sample(args)) return op_fail(std::string("mz_sample_actions: ") + e);
+        const SampleOp op = sample_op(*args);
+        if (op.rows == 0) return 0;
+        Operands o;
+        o.add(op.logits, "logits", type_bytes(op.type));
+        o.add(op.legal, "legal", 1);
+        o.add(op.u, "u", 8);
+        o.add(op.row_temperature, "row_temperature", 8);
+        o.add(op.row_top_k, "row_top_k", 4);
+        o.add(op.row_top_p, "row_top_p", 8);
+        o.add(op.row_min_p, "row_min_p", 8);
+        o.add(op.action, "action", 4);
+        o.add(op.logprob, "logprob", 4);
+        o.add(op.kept, "kept", 4);
+        o.add(op.probs, "probs", 4);
+        return run_op(o, workspace, workspace_bytes, sample_workspace_bytes(op), stream, [&](hipStream_t st) { return launch_sample(st, op, workspace); });
+    });
+}
+
+}  // extern "C"
