@@ -301,6 +301,32 @@ typedef struct mz_sample_args {
 size_t mz_sample_workspace_bytes(const mz_sample_args* args); /* 0 for invalid arguments */
 int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* A projection that all rows share, with a low-rank adapter of each row's own beside it:
+ *   y[m] = x[m] W^T + bias + scale[i] * (x[m] A[i]^T) B[i]^T,   i = index[m]
+ * index -1: the shared projection alone; any other index outside [0, adapters) makes the row NaN.  Sums are fp32 (inputs of
+ * 16 bits on 16-bit matrix instructions, fp32 on fp32 ones), rounded once to y's type.  Rows do not influence one another:
+ * a row's inf or NaN, or an adapter's, stay with the rows that use them. */
+typedef struct mz_adapter_args {
+    int32_t rows, in_features, out_features;
+    int32_t rank, adapters;         /* rank: 1 .. 128; shorter adapters are padded with zeros */
+    int32_t dtype;                  /* MZ_DTYPE_* of x, weight, bias, a, b */
+    int32_t out_dtype;              /* of y: dtype, or MZ_DTYPE_FP32 */
+    int32_t reserved0;
+    const void* x;                  /* [rows][in_features], x_stride */
+    int64_t x_stride;               /* >= 0 */
+    const void* weight;             /* [out_features][in_features], weight_stride */
+    int64_t weight_stride;          /* >= in_features */
+    const void* bias;               /* [out_features] or NULL */
+    const void* a;                  /* [adapters][rank][in_features], dense */
+    const void* b;                  /* [adapters][out_features][rank], dense */
+    const float* scale;             /* [adapters] or NULL: 1 */
+    const int32_t* index;           /* [rows] */
+    void* y;                        /* [rows][out_features], y_stride */
+    int64_t y_stride;               /* >= out_features */
+} mz_adapter_args;
+size_t mz_adapter_workspace_bytes(const mz_adapter_args* args); /* 0 for invalid arguments */
+int mz_adapter_linear(const mz_adapter_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,6 +56,14 @@ class SampleArgs(C.Structure):
                 ("probs", C.c_void_p), ("probs_stride", C.c_int64)]
 
 
+class AdapterArgs(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("in_features", C.c_int32), ("out_features", C.c_int32), ("rank", C.c_int32),
+                ("adapters", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("reserved0", C.c_int32),
+                ("x", C.c_void_p), ("x_stride", C.c_int64), ("weight", C.c_void_p), ("weight_stride", C.c_int64),
+                ("bias", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("index", C.c_void_p),
+                ("y", C.c_void_p), ("y_stride", C.c_int64)]
+
+
 EXPORTS = (
     "mz_create", "mz_destroy", "mz_last_error", "mz_set_action_cells", "mz_load_weights", "mz_num_params",
     "mz_weights_device_ptr", "mz_commit_weights", "mz_initial_inference", "mz_recurrent_inference",
@@ -64,7 +72,7 @@ EXPORTS = (
     "mz_synchronize", "mz_version", "mz_comm_unique_id", "mz_comm_init", "mz_comm_destroy", "mz_broadcast_weights",
     "mz_gather_stats", "mz_comm_barrier", "mz_get_recording_games", "mz_get_gumbel", "mz_seed_gumbel",
     "mz_child_order", "mz_noalloc_scratch_bytes", "mz_search_moves_injected_noalloc", "mz_set_stream_split",
-    "mz_sample_workspace_bytes", "mz_sample_actions")
+    "mz_sample_workspace_bytes", "mz_sample_actions", "mz_adapter_workspace_bytes", "mz_adapter_linear")
 NOALLOC_SCRATCH_BYTES = 16 << 20
 COMM_ID_BYTES = 128
 
@@ -122,6 +130,9 @@ def lib():
         L.mz_sample_workspace_bytes.argtypes = [C.POINTER(SampleArgs)]
         L.mz_sample_workspace_bytes.restype = C.c_size_t
         L.mz_sample_actions.argtypes = [C.POINTER(SampleArgs), vp, C.c_size_t, vp]
+        L.mz_adapter_workspace_bytes.argtypes = [C.POINTER(AdapterArgs)]
+        L.mz_adapter_workspace_bytes.restype = C.c_size_t
+        L.mz_adapter_linear.argtypes = [C.POINTER(AdapterArgs), vp, C.c_size_t, vp]
         _lib = L
     return _lib
 

@@ -35,4 +35,21 @@ struct SampleOp {
 size_t sample_workspace_bytes(const SampleOp& op);
 hipError_t launch_sample(hipStream_t st, const SampleOp& op, void* workspace);
 
+struct AdapterOp {
+    int rows, K, N, rank, adapters, type, out_type;
+    const void* x;
+    long long x_stride;
+    const void* w;
+    long long w_stride;
+    const void* bias;
+    const void* a;       // [adapters][rank][K]
+    const void* b;       // [adapters][N][rank]
+    const float* scale;
+    const int* index;
+    void* y;
+    long long y_stride;
+};
+size_t adapter_workspace_bytes(const AdapterOp& op);
+hipError_t launch_adapter(hipStream_t st, const AdapterOp& op, void* workspace);
+
 }  // namespace mz

@@ -10,6 +10,7 @@ using namespace mz;
 
 namespace {
 
+constexpr int kMaxRank = 128;
 constexpr int kMaxSampleActions = 262144;   // 2^18: sample.hip's histogram masses are sums of 2^46 in 64 bits
 
 // The device all operands live on: the first pointer names it, every other one must agree.
@@ -120,6 +121,43 @@ SampleOp sample_op(const mz_sample_args& a) {
     return o;
 }
 
+const char* check_adapter(const mz_adapter_args* a) {
+    if (!a) return "args is NULL";
+    if (a->rows < 0) return "rows < 0";
+    if (a->in_features < 1 || a->out_features < 1) return "in_features and out_features must be >= 1";
+    if (a->rank < 1 || a->rank > kMaxRank) return "rank must be 1 .. 128";
+    if (a->adapters < 1) return "adapters must be >= 1";
+    if (!known_type(a->dtype)) return "unknown dtype";
+    if (a->out_dtype != a->dtype && a->out_dtype != MZ_DTYPE_FP32) return "out_dtype must be dtype or fp32";
+    if (a->x_stride < 0) return "x_stride must be >= 0";
+    if (a->weight_stride < a->in_features) return "weight_stride < in_features";
+    if (a->rows > 1 && a->y_stride < a->out_features) return "y_stride < out_features";
+    if (a->rows > 0 && (!a->x || !a->weight || !a->a || !a->b || !a->index || !a->y)) return "x, weight, a, b, index and y must not be NULL";
+    return nullptr;
+}
+AdapterOp adapter_op(const mz_adapter_args& a) {
+    AdapterOp o{};
+    o.rows = a.rows;
+    o.K = a.in_features;
+    o.N = a.out_features;
+    o.rank = a.rank;
+    o.adapters = a.adapters;
+    o.type = a.dtype;
+    o.out_type = a.out_dtype;
+    o.x = a.x;
+    o.x_stride = a.x_stride;
+    o.w = a.weight;
+    o.w_stride = a.weight_stride;
+    o.bias = a.bias;
+    o.a = a.a;
+    o.b = a.b;
+    o.scale = a.scale;
+    o.index = a.index;
+    o.y = a.y;
+    o.y_stride = a.y_stride;
+    return o;
+}
+
 // no exception (std::string may throw) crosses the C boundary
 template <typename F>
 int guarded(F f) {
@@ -154,6 +192,27 @@ int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t worksp
         o.add(op.kept, "kept", 4);
         o.add(op.probs, "probs", 4);
         return run_op(o, workspace, workspace_bytes, sample_workspace_bytes(op), stream, [&](hipStream_t st) { return launch_sample(st, op, workspace); });
+    });
+}
+
+size_t mz_adapter_workspace_bytes(const mz_adapter_args* args) { return check_adapter(args) ? 0 : adapter_workspace_bytes(adapter_op(*args)); }
+
+int mz_adapter_linear(const mz_adapter_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        if (const char* e = check_adapter(args)) return op_fail(std::string("mz_adapter_linear: ") + e);
+        const AdapterOp op = adapter_op(*args);
+        if (op.rows == 0) return 0;
+        const size_t es = type_bytes(op.type);
+        Operands o;
+        o.add(op.x, "x", es);
+        o.add(op.w, "weight", es);
+        o.add(op.bias, "bias", es);
+        o.add(op.a, "a", es);
+        o.add(op.b, "b", es);
+        o.add(op.scale, "scale", 4);
+        o.add(op.index, "index", 4);
+        o.add(op.y, "y", type_bytes(op.out_type));
+        return run_op(o, workspace, workspace_bytes, adapter_workspace_bytes(op), stream, [&](hipStream_t st) { return launch_adapter(st, op, workspace); });
     });
 }
 

@@ -1,4 +1,4 @@
-"""The library's operators on torch tensors (mz_sample_actions of include/muzero_hip.h): checks of types, shapes and
+"""The library's operators on torch tensors (mz_sample_actions, mz_adapter_linear of include/muzero_hip.h): checks of types, shapes and
 devices, then one call of the C ABI on torch's current stream of the tensors' device.  Nothing is copied, converted or
 synchronised; a call can be captured into a torch.cuda.graph.  Errors are capi.MuZeroError."""
 import torch
@@ -104,4 +104,44 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     ref = capi.C.byref(a)
     keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(ref), workspace, dev)
     _finish(L.mz_sample_actions(ref, ws, nbytes, torch.cuda.current_stream(dev).cuda_stream))
+    return out
+
+
+def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None, out=None, workspace=None):
+    """x [M, K] @ weight [N, K]^T + bias [N], plus each row's own adapter i = index[m] (int32 [M], -1 = none):
+    scale[i] * (x[m] @ a[i]^T) @ b[i]^T with a [n, r, K], b [n, N, r] and scale float32 [n] (None: 1).  All of one type (float32,
+    bfloat16, float16); the result [M, N] has it too, or float32 with out_dtype=torch.float32 (mz_adapter_linear)."""
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x: a 2-d torch tensor is needed")
+    _need(x.is_cuda, "x: must be on a GPU")
+    t, dev = x.dtype, x.device
+    _need(t in DTYPES, f"x: {t} is not supported")
+    M, K = x.shape
+    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight: a 2-d torch tensor is needed")
+    _need(isinstance(a, torch.Tensor) and a.dim() == 3, "a: a 3-d torch tensor is needed")
+    N, (n, r, _) = weight.shape[0], a.shape
+    if out_dtype is None:
+        out_dtype = t if out is None else out.dtype
+    _need(out_dtype in DTYPES, f"out_dtype: {out_dtype} is not supported")
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    g = capi.AdapterArgs()
+    g.rows, g.in_features, g.out_features, g.rank, g.adapters = M, K, N, r, n
+    g.dtype, g.out_dtype = DTYPES[t], DTYPES[out_dtype]
+    g.x = _tensor(x, "x", t, (M, K), dev, dense=False)
+    g.x_stride = _row_stride(x)
+    g.weight = _tensor(weight, "weight", t, (N, K), dev, dense=False)
+    g.weight_stride = _row_stride(weight)
+    if bias is not None:
+        g.bias = _tensor(bias, "bias", t, (N,), dev)
+    g.a = _tensor(a, "a", t, (n, r, K), dev)
+    g.b = _tensor(b, "b", t, (n, N, r), dev)
+    if scale is not None:
+        g.scale = _tensor(scale, "scale", torch.float32, (n,), dev)
+    g.index = _tensor(index, "index", torch.int32, (M,), dev)
+    g.y = _tensor(out, "out", out_dtype, (M, N), dev, dense=False)
+    g.y_stride = _row_stride(out)
+    L = capi.lib()
+    ref = capi.C.byref(g)
+    keep, ws, nbytes = _workspace(L.mz_adapter_workspace_bytes(ref), workspace, dev)
+    _finish(L.mz_adapter_linear(ref, ws, nbytes, torch.cuda.current_stream(dev).cuda_stream))
     return out

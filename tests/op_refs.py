@@ -52,3 +52,24 @@ def sample(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     rows = [sample_row(z[i], ok[i], *(q[i] for q in par), u[i]) for i in range(len(z))]
     return dict(action=np.array([r[0] for r in rows], np.int32), logprob=np.array([r[1] for r in rows]),
                 kept=np.array([r[2] for r in rows], np.int32), probs=np.array([r[3] for r in rows]))
+
+
+def adapter(x, weight, a, b, index, bias=None, scale=None):
+    """(y, size) in 64 bits on the host: y of mz_adapter_linear, and the sum of the absolute values of all terms of each y,
+    which is what rounding errors of the sums go by."""
+    f = lambda v: v.detach().cpu().double().numpy()  # noqa: E731
+    x, w, a, b, index = f(x), f(weight), f(a), f(b), index.cpu().numpy()
+    with np.errstate(invalid="ignore", over="ignore"):
+        y, size = x @ w.T, np.abs(x) @ np.abs(w).T
+        if bias is not None:
+            y = y + f(bias)
+            size = size + np.abs(f(bias))
+        for i in np.unique(index):
+            rows = np.flatnonzero(index == i)
+            if i < -1 or i >= len(a):
+                y[rows] = np.nan
+            elif i >= 0:
+                s = 1.0 if scale is None else float(scale[i])
+                y[rows] += s * (x[rows] @ a[i].T) @ b[i].T
+                size[rows] += abs(s) * (np.abs(x[rows]) @ np.abs(a[i]).T) @ np.abs(b[i]).T
+    return y, size

@@ -63,3 +63,25 @@ def test_the_restatement_on_a_row_done_by_hand():
     assert op_refs.sample_row(z, ok, T, 0, 0.49, 0.0, 0.3)[:1] == (2,)
     assert op_refs.sample_row(z, ok, T, 0, 1.0, 0.26, 0.9)[2] == 2
     assert op_refs.sample_row(z, np.zeros(4, bool), T, 0, 1.0, 0.0, 0.9)[0] == -1
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(rows=-1), "rows"), (dict(in_features=0), "in_features"), (dict(out_features=0), "out_features"), (dict(rank=0), "rank"),
+    (dict(rank=129), "rank"), (dict(adapters=0), "adapters"), (dict(dtype=3), "dtype"), (dict(out_dtype=2), "out_dtype"),
+    (dict(x_stride=-1), "x_stride"), (dict(weight_stride=63), "weight_stride"), (dict(y_stride=31), "y_stride"), (dict(x=None), "NULL"),
+    (dict(weight=None), "NULL"), (dict(a=None), "NULL"), (dict(b=None), "NULL"), (dict(index=None), "NULL"), (dict(y=None), "NULL")])
+def test_adapter_refuses(change, text):
+    a = capi.AdapterArgs(rows=2, in_features=64, out_features=32, rank=4, adapters=2, dtype=1, out_dtype=1, x=64, x_stride=64,
+                         weight=64, weight_stride=64, a=64, b=64, index=64, y=64, y_stride=32)
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert capi.lib().mz_adapter_linear(C.byref(a), None, 0, None) == -1
+    assert text in last_error()
+    assert capi.lib().mz_adapter_workspace_bytes(C.byref(a)) == 0
+
+
+def test_adapter_needs_device_tensors():
+    z = torch.zeros
+    assert C.sizeof(capi.AdapterArgs) == 8 * 4 + 12 * 8 - 8
+    with pytest.raises(capi.MuZeroError, match="GPU"):
+        ops.adapter_linear(z(2, 8), z(4, 8), z(1, 2, 8), z(1, 4, 2), z(2, dtype=torch.int32))
