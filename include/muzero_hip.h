@@ -279,7 +279,7 @@ enum { MZ_DTYPE_FP32 = 0, MZ_DTYPE_BF16 = 1, MZ_DTYPE_F16 = 2 }; /* the numbers 
  * A row with no such entry, and a row whose u or per-row parameter is out of range or NaN, gets action -1, kept 0, logprob 0
  * and probs 0.  Weights and sums are 64-bit; a row's result does not depend on the other rows. */
 typedef struct mz_sample_args {
-    int32_t rows, actions;          /* actions: 1 .. 262144 */
+    int32_t rows, actions;          /* rows: 0 .. 2097152, actions: 1 .. 262144 */
     int32_t dtype;                  /* MZ_DTYPE_* of logits */
     int32_t top_k;
     double temperature, top_p, min_p;
@@ -307,7 +307,7 @@ int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t worksp
  * 16 bits on 16-bit matrix instructions, fp32 on fp32 ones), rounded once to y's type.  Rows do not influence one another:
  * a row's inf or NaN, or an adapter's, stay with the rows that use them. */
 typedef struct mz_adapter_args {
-    int32_t rows, in_features, out_features;
+    int32_t rows, in_features, out_features; /* out_features <= 2^26, ceil(rows / 256) * ceil(out_features / 256) <= 2^22 */
     int32_t rank, adapters;         /* rank: 1 .. 128; shorter adapters are padded with zeros */
     int32_t dtype;                  /* MZ_DTYPE_* of x, weight, bias, a, b */
     int32_t out_dtype;              /* of y: dtype, or MZ_DTYPE_FP32 */

@@ -1,14 +1,20 @@
 // mz_adapter_linear: y[m] = x[m] W^T + bias + s_i (x[m] A_i^T) B_i^T with i = index[m], the row's own adapter.
-//   k_shrink   t[m] = s_i x[m] A_i^T, fp32, [rows][rank] in the workspace
-//   k_project  the product with W on the matrix cores, then t[m] B_i^T and the bias on its accumulators
+//   k_shrink  t[m] = x[m] A_i^T in fp32, in parts over K, into the workspace.  The rows of a workgroup are ordered by adapter, so
+//             that up to 16 rows of one adapter share its A on the matrix cores.
+//   k_skinny  up to 64 rows (single tokens): bound by the bytes of W, which go straight from memory into the matrix
+//             instructions' registers, once; the waves of a workgroup split K.  With one or two rows of small rank t is computed
+//             by every workgroup for itself (A is read from L2), which saves the launch of k_shrink.
+//   k_tile    more rows: a tiled product, operands staged through LDS; the rows of a tile are ordered by adapter, so that
+//             t B_i^T is one more step of the same matrix instructions on the accumulators, per adapter in 16 rows.
+// Both end with bias, the adapter's term and one rounding.  The adapter's term is computed apart from the accumulators and added
+// where the row uses that adapter: no row sees another row's adapter, whatever values it holds.
+#include "net.h"
 #include "ops.h"
 
 #include <math.h>
 
 namespace mz {
 namespace {
-
-constexpr int W = 64;
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -67,111 +73,631 @@ __device__ __forceinline__ u32x4 load_chunk(const T* row, int k, int K) {
     return v;
 }
 
-// ---- t = s x A^T: a wave per (row, rank) -----------------------------------------------------------------------------------
+// ---- shapes shared by the kernels ------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void k_shrink(AdapterOp op, float* t) {
-    const int lane = threadIdx.x & 63;
-    const long long job = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int m = (int)(job / op.rank), j = (int)(job % op.rank);
-    if (m >= op.rows) return;
+constexpr int kChunk = 16 / sizeof(T);        // elements of a 16-byte chunk
+constexpr int kRankTile = 16;
+__host__ __device__ inline int padded_rank(int r) { return (r + kRankTile - 1) / kRankTile * kRankTile; }
+
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p) {   // any alignment
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+constexpr int kNone = -3, kForeign = -2, kNoRow = -1;   // as unsigned numbers: behind every adapter, in this order
+__device__ __forceinline__ int adapter_of(const AdapterOp& op, int m) {
     const int i = op.index[m];
-    if (i < 0 || i >= op.adapters) return;
-    const T* x = static_cast<const T*>(op.x) + m * op.x_stride;
-    const T* a = static_cast<const T*>(op.a) + ((long long)i * op.rank + j) * op.K;
-    float s = 0;
-    for (int k = lane; k < op.K; k += W) s = fmaf(to_float(x[k]), to_float(a[k]), s);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-    if (lane == 0) t[(long long)m * op.rank + j] = op.scale ? op.scale[i] * s : s;
+    return i >= 0 && i < op.adapters ? i : i == -1 ? kNone : kForeign;
 }
 
-// ---- the projection --------------------------------------------------------------------------------------------------------
-template <typename T, typename O>
-__global__ __launch_bounds__(256) void k_project(AdapterOp op, const float* t) {
-    constexpr int BM = 64, BN = 64, CH = 8, N16 = 16 / sizeof(T);   // tile rows of x / of W; 16-byte chunks of k per step
-    __shared__ u32x4 sx[BM * CH], sw[BN * CH];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int ntn = (op.N + BN - 1) / BN;
-    const int m0 = (int)(blockIdx.x / ntn) * BM, n0 = (int)(blockIdx.x % ntn) * BN;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    f32x4 acc[2][2] = {};   // [n tile][m tile]
-    for (int k0 = 0; k0 < op.K; k0 += CH * N16) {
-        __syncthreads();
-        for (int c = tid; c < BM * CH; c += 256) {
-            const int r = c / CH, s = c % CH;
-            const int m = min(m0 + r, op.rows - 1);
-            sx[r * CH + (s ^ (r & 7))] = load_chunk(static_cast<const T*>(op.x) + m * op.x_stride, k0 + s * N16, op.K);
+// Orders the rows [m0, m0 + count) of a workgroup by adapter (rows of none last): order[p] = row, key[p] = its adapter, kNone or
+// kForeign (p >= count: kNoRow), nth[p] = how many rows of that key are in front of it.  count <= BR <= threads; ends with a barrier.
+template <int BR>
+__device__ __forceinline__ void order_rows(const AdapterOp& op, int m0, int count, int* raw, int* order, int* key, int* nth) {
+    const int tid = threadIdx.x;
+    if (tid < BR) raw[tid] = tid < count ? adapter_of(op, m0 + tid) : kNoRow;
+    __syncthreads();
+    if (tid < BR) {
+        const unsigned mine = (unsigned)raw[tid];   // negative values are the largest
+        int pos = 0, eq = 0;
+#pragma unroll 8
+        for (int j = 0; j < BR; j++) {
+            const unsigned o = (unsigned)raw[j];
+            pos += o < mine || (o == mine && j < tid);
+            eq += o == mine && j < tid;
         }
-        for (int c = tid; c < BN * CH; c += 256) {
-            const int r = c / CH, s = c % CH;
-            const int n = min(n0 + r, op.N - 1);
-            sw[r * CH + (s ^ (r & 7))] = load_chunk(static_cast<const T*>(op.w) + n * op.w_stride, k0 + s * N16, op.K);
-        }
-        __syncthreads();
+        order[pos] = tid;
+        key[pos] = (int)mine;
+        nth[pos] = eq;
+    }
+    __syncthreads();
+}
+
+// 16-bit chunk with inf and NaN entries, which are rare, set to zero
+template <typename T>
+__device__ __forceinline__ u32x4 finite_only(u32x4 v) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    constexpr unsigned kExp = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+    u16x2 m = {0, 0};
 #pragma unroll
-        for (int ks = 0; ks < CH / 4; ks++) {
-            const int c = ks * 4 + (lane >> 4);
-            u32x4 fw[2], fx[2];
+    for (int i = 0; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+    if (__builtin_expect(m.x >= kExp || m.y >= kExp, 0)) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int rw = wn + i * 16 + (lane & 15), rx = wm + i * 16 + (lane & 15);
-                fw[i] = sw[rw * CH + (c ^ (rw & 7))];
-                fx[i] = sx[rx * CH + (c ^ (rx & 7))];
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] = mma<T>(fw[i], fx[j], acc[i][j]);
+        for (int i = 0; i < 4; i++) {
+            if ((v[i] & kExp) == kExp) v[i] &= 0xffff0000u;
+            if ((v[i] >> 16 & kExp) == kExp) v[i] &= 0x0000ffffu;
         }
     }
+    return v;
+}
+
+// ---- t = x A^T -------------------------------------------------------------------------------------------------------------
+// Workgroup (block of BR rows, part of K): jobs of up to 16 rows of one adapter, a wave each.  part[s][row][padded rank].
+template <typename T, int RT, int BR>
+__global__ __launch_bounds__(256) void k_shrink(AdapterOp op, float* part, int splits) {
+    constexpr int CE = kChunk<T>;
+    __shared__ int raw[BR], order[BR], key[BR], nth[BR], job[BR], jobs;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, kq = lane >> 4;
+    const int m0 = blockIdx.x * BR, count = min(BR, op.rows - m0), split = blockIdx.y;
+    order_rows<BR>(op, m0, count, raw, order, key, nth);
+    if (tid < BR) {
+        const bool start = key[tid] >= 0 && nth[tid] % 16 == 0;
+        int id = 0;
+        for (int j = 0; j < tid; j++) id += key[j] >= 0 && nth[j] % 16 == 0;
+        if (start) job[id] = tid;
+        if (tid == BR - 1) jobs = id + start;
+    }
+    __syncthreads();
+    const int rp = padded_rank(op.rank);
+    const int pairs = (op.K + 8 * CE - 1) / (8 * CE);           // 128-byte steps of k
+    const int p0 = (int)((long long)pairs * split / splits), p1 = (int)((long long)pairs * (split + 1) / splits);
+    const int pf = min(p1, op.K / (8 * CE));                    // whole ones
+    for (int j = wave; j < jobs; j += 4) {
+        const int at = job[j], i = key[at], p = at + lr;
+        const bool mine = p < count && key[p] == i;
+        const int m = m0 + order[mine ? p : at];
+        const T* x = static_cast<const T*>(op.x) + m * op.x_stride + kq * 2 * CE;
+        const T* a[RT];
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int m = m0 + wm + j * 16 + (lane & 15);
-        if (m >= op.rows) continue;
-        const int idx = op.index[m];
-        const bool some = idx >= 0 && idx < op.adapters;
-        const float* tm = t + (long long)m * op.rank;
+        for (int q = 0; q < RT; q++)   // ranks beyond the last: a row that is there, its results are dropped
+            a[q] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min(q * 16 + lr, op.rank - 1)) * op.K + kq * 2 * CE;
+        f32x4 acc[RT] = {};
+        int k = p0;
+        constexpr int U = RT <= 2 ? 4 : 2;
+        for (; k + U <= pf; k += U) {
+            u32x4 fx[U][2], fa[U][RT][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    fx[u][h] = load16(x + (k + u) * 8 * CE + h * CE);
+#pragma unroll
+                    for (int q = 0; q < RT; q++) fa[u][q][h] = load16(a[q] + (k + u) * 8 * CE + h * CE);
+                }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int q = 0; q < RT; q++) acc[q] = mma<T>(fa[u][q][h], fx[u][h], acc[q]);
+        }
+        for (; k < p1; k++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int left = op.K - kq * 2 * CE;             // x and a already stand at this lane's first chunk
+                const u32x4 fx = load_chunk(x, k * 8 * CE + h * CE, left);
+#pragma unroll
+                for (int q = 0; q < RT; q++) acc[q] = mma<T>(load_chunk(a[q], k * 8 * CE + h * CE, left), fx, acc[q]);
+            }
+        if (mine) {
+            float* dst = part + ((long long)split * op.rows + m) * rp + kq * 4;
+#pragma unroll
+            for (int q = 0; q < RT; q++) {
+                f32x4 v = acc[q];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (q * 16 + kq * 4 + e >= op.rank) v[e] = 0.f;
+                if (q * 16 < rp) *reinterpret_cast<f32x4*>(dst + q * 16) = v;
+            }
+        }
+    }
+}
+// the parts of four ranks of a row, added in order
+__device__ __forceinline__ f32x4 sum_parts(const float* part, int splits, long long rows, long long m, int rp, int r) {
+    f32x4 v = {};
+    for (int s = 0; s < splits; s++) v += *reinterpret_cast<const f32x4*>(part + (s * rows + m) * rp + r);
+    return v;
+}
+
+// four neighbouring results of a row
+template <typename T>
+__device__ __forceinline__ void store4(const AdapterOp& op, int m, int n, f32x4 v) {
+    const long long at = m * op.y_stride + n;
+    const bool whole = n + 4 <= op.N;
+    if (op.bias) {
+        const T* b = static_cast<const T*>(op.bias) + n;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < op.N) v[e] += to_float(b[e]);
+    }
+    if (sizeof(T) == 4 || op.out_type == kFp32) {
+        float* y = static_cast<float*>(op.y) + at;
+        if (whole) __builtin_memcpy(y, &v, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < op.N) y[e] = v[e];
+    } else {
+        T* y = static_cast<T*>(op.y) + at;
+        T h[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = from_float<T>(v[e]);
+        if (whole) __builtin_memcpy(y, h, 4 * sizeof(T));
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < op.N) y[e] = h[e];
+    }
+}
+
+// ---- up to 64 rows -----------------------------------------------------------------------------------------------------------
+// Workgroup: 16 NT rows of W, all 16 MT rows of x; 8 waves split K by 128-byte steps; partial sums meet in LDS.
+// FJ > 0: t is computed here, FJ >= rows * rank tiles more tiles of 16 rows (of A).
+constexpr int kSkinnyWaves = 8;
+template <int MT, int NT, int FJ>
+constexpr size_t skinny_lds() {
+    return (size_t)kSkinnyWaves * (MT * NT + FJ) * 64 * 16;
+}
+template <typename T, int MT, int NT, int FJ>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, const float* part, int splits) {
+    constexpr int CE = kChunk<T>, NW = kSkinnyWaves, TILES = MT * NT;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    f32x4* red = reinterpret_cast<f32x4*>(smem);                              // [NW][TILES + FJ][64]
+    float* tl = reinterpret_cast<float*>(smem + skinny_lds<MT, NT, FJ>());    // [rows][padded rank]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, kq = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NT, rp = padded_rank(op.rank), rt = rp / 16;
+    const T *w[NT], *x[MT], *a[FJ ? FJ : 1];
+#pragma unroll
+    for (int i = 0; i < NT; i++) w[i] = static_cast<const T*>(op.w) + min(n0 + i * 16 + lr, op.N - 1) * op.w_stride + kq * 2 * CE;
+#pragma unroll
+    for (int i = 0; i < MT; i++) x[i] = static_cast<const T*>(op.x) + min(i * 16 + lr, op.rows - 1) * op.x_stride + kq * 2 * CE;
+#pragma unroll
+    for (int j = 0; j < FJ; j++) {
+        const int m = min(j / rt, op.rows - 1), i = max(adapter_of(op, m), 0);   // of none: some A, its t is not used
+        a[j] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min((j % rt) * 16 + lr, op.rank - 1)) * op.K + kq * 2 * CE;
+    }
+    f32x4 acc[NT][MT] = {}, ta[FJ ? FJ : 1] = {};
+    const int pairs = (op.K + 8 * CE - 1) / (8 * CE), pf = op.K / (8 * CE);
+    constexpr int U = TILES + FJ <= 3 ? 4 : MT + NT <= 4 ? 2 : 1;
+    int p = wave;
+    for (; p + (U - 1) * NW < pf; p += U * NW) {
+        u32x4 fw[U][NT][2], fx[U][MT][2], fa[U][FJ ? FJ : 1][2];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = (p + u * NW) * 8 * CE + h * CE;
+#pragma unroll
+                for (int i = 0; i < NT; i++) fw[u][i][h] = load16(w[i] + k);
+#pragma unroll
+                for (int j = 0; j < FJ; j++) fa[u][j][h] = load16(a[j] + k);
+#pragma unroll
+                for (int i = 0; i < MT; i++) fx[u][i][h] = load16(x[i] + k);
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int i = 0; i < NT; i++)
+#pragma unroll
+                    for (int j = 0; j < MT; j++) acc[i][j] = mma<T>(fw[u][i][h], fx[u][j][h], acc[i][j]);
+#pragma unroll
+                for (int j = 0; j < FJ; j++) ta[j] = mma<T>(fa[u][j][h], fx[u][0][h], ta[j]);
+            }
+    }
+    for (; p < pairs; p += NW)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int k = p * 8 * CE + h * CE, left = op.K - kq * 2 * CE;
+            u32x4 fx[MT];
+#pragma unroll
+            for (int j = 0; j < MT; j++) fx[j] = load_chunk(x[j], k, left);
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const u32x4 fw = load_chunk(w[i], k, left);
+#pragma unroll
+                for (int j = 0; j < MT; j++) acc[i][j] = mma<T>(fw, fx[j], acc[i][j]);
+            }
+#pragma unroll
+            for (int j = 0; j < FJ; j++) ta[j] = mma<T>(load_chunk(a[j], k, left), fx[0], ta[j]);
+        }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) red[(wave * (TILES + FJ) + i * MT + j) * 64 + lane] = acc[i][j];
+#pragma unroll
+    for (int j = 0; j < FJ; j++) red[(wave * (TILES + FJ) + TILES + j) * 64 + lane] = ta[j];
+    if (!FJ) {
+        for (int q = tid; q < op.rows * (rp / 4); q += 64 * NW) {
+            const int m = q / (rp / 4), r = q % (rp / 4) * 4;
+            *reinterpret_cast<f32x4*>(tl + m * rp + r) = sum_parts(part, splits, op.rows, m, rp, r);
+        }
+    }
+    __syncthreads();
+    if (FJ) {   // column m of job (m, rank tile) holds t[m]
+        for (int q = tid; q < op.rows * rp; q += 64 * NW) {
+            const int m = q / rp, r = q % rp, j = m * rt + r / 16;
+            float v = 0;
+            for (int s = 0; s < NW; s++) v += red[(s * (TILES + FJ) + TILES + j) * 64 + (r % 16 / 4) * 16 + m][r & 3];
+            tl[m * rp + r] = r < op.rank ? v : 0.f;
+        }
+        __syncthreads();
+    }
+    for (int q = tid; q < TILES * 64; q += 64 * NW) {
+        const int tile = q / 64, l = q % 64, m = (tile % MT) * 16 + (l & 15), n = n0 + (tile / MT) * 16 + (l >> 4) * 4;
+        if (m >= op.rows || n >= op.N) continue;
+        f32x4 v = {};
+#pragma unroll
+        for (int s = 0; s < NW; s++) v += red[(s * (TILES + FJ) + tile) * 64 + l];
+        const int i = adapter_of(op, m);
+        if (i >= 0) {
+            const float sc = op.scale ? op.scale[i] : 1.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int n = n0 + wn + i * 16 + (lane >> 4) * 4 + e;
-                if (n >= op.N) continue;
-                float v = acc[i][j][e];
-                if (some) {
-                    const T* b = static_cast<const T*>(op.b) + ((long long)idx * op.N + n) * op.rank;
-                    float s = 0;
-                    for (int q = 0; q < op.rank; q++) s = fmaf(tm[q], to_float(b[q]), s);
-                    v += s;
-                } else if (idx != -1) {
-                    v = NAN;
+                const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + min(n + e, op.N - 1)) * op.rank;
+                float d = 0;
+                for (int r = 0; r < op.rank; r += CE) {
+                    const u32x4 c = load_chunk(b, r, op.rank);
+                    T h[CE];
+                    __builtin_memcpy(h, &c, 16);
+#pragma unroll
+                    for (int k = 0; k < CE; k++) d = fmaf(tl[m * rp + r + k], to_float(h[k]), d);
                 }
-                if (op.bias) v += to_float(static_cast<const T*>(op.bias)[n]);
-                static_cast<O*>(op.y)[m * op.y_stride + n] = from_float<O>(v);
+                v[e] = fmaf(sc, d, v[e]);
             }
+        } else if (i == kForeign) {
+            v = f32x4{NAN, NAN, NAN, NAN};
+        }
+        store4<T>(op, m, n, v);
     }
 }
 
-template <typename T, typename O>
+// ---- tiles -------------------------------------------------------------------------------------------------------------------
+// LDS: a ring of stages, each 64 bytes of k (4 chunks) of BM rows of x and BN rows of W.  Chunk c of row r stands at slot
+// c ^ (r >> 1 & 3): the 8 lanes that an LDS read serves at a time then hit 8 different 16-byte columns.
+// DMA: rows of both operands are 16-byte aligned: global -> LDS without registers, three stages ahead.  Otherwise through
+// registers, one stage ahead.
+template <int BM, int BN>
+constexpr size_t tile_stage_bytes() {
+    return (size_t)(BM + BN) * 64;
+}
+constexpr int kRing = 4;
+template <int BM>
+constexpr int kOrderBytes = 4 * BM * (int)sizeof(int);
+
+template <typename T, int BM, int BN, int WM, int WN, bool DMA>
+__global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float* part, int splits) {
+    constexpr int CE = kChunk<T>, NW = WM * WN, NTH = 64 * NW, MI = BM / WM / 16, NI = BN / WN / 16;
+    constexpr int STAGE = (int)tile_stage_bytes<BM, BN>();
+    extern __shared__ __attribute__((aligned(16))) char lds[];   // (all of it dynamic: the opt-in covers 160 KiB of that)
+    int *raw = reinterpret_cast<int*>(lds), *order = raw + BM, *key = order + BM, *nth = key + BM;
+    char* smem = lds + kOrderBytes<BM>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, kq = lane >> 4;
+    // tiles of 8 row blocks x all column blocks in turn, so that what runs at one time shares operands in L2; consecutive
+    // workgroups go to the 8 XCDs in turn: each takes a contiguous share
+    const int ntm = (op.rows + BM - 1) / BM, ntn = (op.N + BN - 1) / BN, nt = ntm * ntn;
+    int tile = blockIdx.x;
+    {
+        const int per = nt / 8, rem = nt % 8, xcd = tile % 8, at = tile / 8;
+        tile = xcd * per + min(xcd, rem) + at;
+    }
+    constexpr int G = 8;
+    const int group = tile / (G * ntn), gm = min(G, ntm - group * G), in = tile - group * G * ntn;
+    const int m0 = (group * G + in % gm) * BM, n0 = in / gm * BN;
+    const int count = min(BM, op.rows - m0);
+    order_rows<BM>(op, m0, count, raw, order, key, nth);
+
+    const T* xb = static_cast<const T*>(op.x) + m0 * op.x_stride;
+    const T* wb = static_cast<const T*>(op.w) + n0 * op.w_stride;
+    f32x4 acc[NI][MI] = {};
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    auto compute = [&](const char* st) {
+        u32x4 fx[MI], fw[NI];
+#pragma unroll
+        for (int j = 0; j < MI; j++) {
+            const int r = wm + j * 16 + lr;
+            fx[j] = *reinterpret_cast<const u32x4*>(st + r * 64 + ((kq ^ (r >> 1 & 3)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int r = wn + i * 16 + lr;
+            fw[i] = *reinterpret_cast<const u32x4*>(st + (BM + r) * 64 + ((kq ^ (r >> 1 & 3)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int j = 0; j < MI; j++) acc[i][j] = mma<T>(fw[i], fx[j], acc[i][j]);
+    };
+    constexpr int LX = BM / 16 / NW, LW = BN / 16 / NW;   // 16-row pieces of each operand that a wave brings
+    static_assert(LX * NW * 16 == BM && LW * NW * 16 == BN, "pieces");
+    // piece i of this wave: lane -> (row of the tile, slot); its source row and k chunk
+    const int slot = lane & 3;
+    if constexpr (DMA) {
+        unsigned ox[LX], ow[LW];
+        const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
+#pragma unroll
+        for (int i = 0; i < LX; i++) {
+            const int r = (wave * LX + i) * 16 + (lane >> 2);
+            ox[i] = (unsigned)(min(order[r], count - 1) * op.x_stride * sizeof(T)) + ((slot ^ (r >> 1 & 3)) << 4);
+        }
+#pragma unroll
+        for (int i = 0; i < LW; i++) {
+            const int r = (wave * LW + i) * 16 + (lane >> 2);
+            ow[i] = (unsigned)(min(r, op.N - 1 - n0) * op.w_stride * sizeof(T)) + ((slot ^ (r >> 1 & 3)) << 4);
+        }
+        const char* gx = reinterpret_cast<const char*>(xb);
+        const char* gw = reinterpret_cast<const char*>(wb);
+        // written as one statement each, M0 with it: the compiler's own waits for such loads in flight would drain them at
+        // every LDS read
+        auto issue = [&](int stage) {
+            const unsigned dst = lds0 + (stage % kRing) * STAGE;
+#pragma unroll
+            for (int i = 0; i < LX; i++)
+                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(ox[i]), "s"(dst + (wave * LX + i) * 1024), "s"(gx) : "memory");
+#pragma unroll
+            for (int i = 0; i < LW; i++)
+                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(ow[i]), "s"(dst + BM * 64 + (wave * LW + i) * 1024), "s"(gw) : "memory");
+            gx += 64;
+            gw += 64;
+        };
+        constexpr int PER = LX + LW;
+        const int full = op.K / (4 * CE);
+#pragma unroll
+        for (int s = 0; s < kRing - 1; s++)
+            if (s < full) issue(s);
+        for (int s = 0; s < full; s++) {
+            // this wave's loads of stage s have arrived (those of the next two may be in flight), then everyone's
+            if (s + 2 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER) : "memory");
+            else if (s + 1 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (s + kRing - 1 < full) issue(s + kRing - 1);   // into the slot of stage s - 1, which everyone has left
+            compute(smem + (s % kRing) * STAGE);
+        }
+    }
+    {
+        // through registers: all of K without DMA, what is left of a stage with it
+        const int first = DMA ? op.K / (4 * CE) : 0, last = (op.K + 4 * CE - 1) / (4 * CE);
+        const T *px[LX], *pw[LW];
+#pragma unroll
+        for (int i = 0; i < LX; i++) px[i] = xb + min(order[(wave * LX + i) * 16 + (lane >> 2)], count - 1) * op.x_stride;
+#pragma unroll
+        for (int i = 0; i < LW; i++) pw[i] = wb + min((wave * LW + i) * 16 + (lane >> 2), op.N - 1 - n0) * op.w_stride;
+        u32x4 vx[LX], vw[LW];
+        auto fetch = [&](int s) {
+            const int k = s * 4 * CE + slot * CE;
+#pragma unroll
+            for (int i = 0; i < LX; i++) vx[i] = load_chunk(px[i], k, op.K);
+#pragma unroll
+            for (int i = 0; i < LW; i++) vw[i] = load_chunk(pw[i], k, op.K);
+        };
+        auto put = [&](char* st) {
+#pragma unroll
+            for (int i = 0; i < LX; i++) {
+                const int r = (wave * LX + i) * 16 + (lane >> 2);
+                *reinterpret_cast<u32x4*>(st + r * 64 + ((slot ^ (r >> 1 & 3)) << 4)) = vx[i];
+            }
+#pragma unroll
+            for (int i = 0; i < LW; i++) {
+                const int r = (wave * LW + i) * 16 + (lane >> 2);
+                *reinterpret_cast<u32x4*>(st + (BM + r) * 64 + ((slot ^ (r >> 1 & 3)) << 4)) = vw[i];
+            }
+        };
+        if (first < last) {
+            fetch(first);
+            if (DMA) __syncthreads();   // the ring has been read
+            put(smem);
+        }
+        for (int s = first; s < last; s++) {
+            if (s + 1 < last) fetch(s + 1);
+            __syncthreads();            // stage s is there, and stage s - 1 has been read
+            compute(smem + ((s - first) & 1) * STAGE);
+            if (s + 1 < last) put(smem + ((s + 1 - first) & 1) * STAGE);
+        }
+    }
+
+    // ---- the adapters' term: t of this tile's rows, in its order -> LDS
+    const int rp = padded_rank(op.rank), ts = rp + 4;
+    float* tl = reinterpret_cast<float*>(smem);          // [BM][ts]
+    __syncthreads();
+    for (int q = tid; q < BM * (rp / 4); q += NTH) {
+        const int p = q / (rp / 4), r = q % (rp / 4) * 4;
+        f32x4 v = {};
+        if (key[p] >= 0) v = sum_parts(part, splits, op.rows, m0 + order[p], rp, r);
+        *reinterpret_cast<f32x4*>(tl + p * ts + r) = v;
+    }
+    __syncthreads();
+    int em = 0;   // fp16: t scaled into [0.5, 1) by a power of two per row
+#pragma unroll
+    for (int j = 0; j < MI; j++) {
+        const int p = wm + j * 16 + lr, mine = key[p];
+        float back = 1.f, to = 1.f;
+        if constexpr (__is_same(T, _Float16)) {
+            float mx = 0;
+            for (int r = kq * 4; r < rp; r += 16)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(tl[p * ts + r + e]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            em = mx > 0 && mx < INFINITY ? max(-100, min(100, ilogbf(mx) + 1)) : 0;
+            back = ldexpf(1.f, em);
+            to = ldexpf(1.f, -em);
+        }
+        // per adapter among the 16 rows
+        unsigned long long todo = __ballot(mine >= 0);
+        while (todo) {
+            const int i = __shfl(mine, __ffsll(todo) - 1);
+            const bool use = mine == i;
+            todo &= ~__ballot(use);
+            const float sc = (op.scale ? op.scale[i] : 1.f) * back;
+            f32x4 d[NI] = {};
+            for (int r0 = 0; r0 < rp; r0 += 16) {
+                u32x4 ft;   // 16 bits: k = 16 ranks of the leading part of t, then the same 16 of what it leaves; fp32: the 16 ranks
+                int rb;
+                if constexpr (sizeof(T) == 4) {
+                    rb = r0 + kq * 4;
+                    ft = *reinterpret_cast<const u32x4*>(tl + p * ts + rb);
+                } else {
+                    rb = r0 + (kq & 1) * 8;
+                    T h[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float v = tl[p * ts + rb + e] * to;
+                        h[e] = from_float<T>(v);
+                        if (kq >= 2) {
+                            const float rest = v - to_float(h[e]);
+                            h[e] = from_float<T>(rest == rest ? rest : 0.f);   // inf - inf: the leading part says it
+                        }
+                    }
+                    __builtin_memcpy(&ft, h, 16);
+                }
+#pragma unroll
+                for (int ni = 0; ni < NI; ni++) {
+                    const int n = min(n0 + wn + ni * 16 + lr, op.N - 1);
+                    const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + n) * op.rank;
+                    u32x4 fb = load_chunk(b, rb, op.rank);
+                    if constexpr (sizeof(T) == 2) {
+                        // an inf of B times the rest of t, which may have the other sign, is not wanted beside inf times its leading part
+                        if (kq >= 2) fb = finite_only<T>(fb);
+                    }
+                    d[ni] = mma<T>(fb, ft, d[ni]);
+                }
+            }
+            if (use) {
+#pragma unroll
+                for (int ni = 0; ni < NI; ni++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[ni][j][e] = fmaf(sc, d[ni][e], acc[ni][j][e]);
+            }
+        }
+        if (p < count) {
+            const int m = m0 + order[p];
+#pragma unroll
+            for (int ni = 0; ni < NI; ni++) {
+                const int n = n0 + wn + ni * 16 + kq * 4;
+                if (n < op.N) store4<T>(op, m, n, mine == kForeign ? f32x4{NAN, NAN, NAN, NAN} : acc[ni][j]);
+            }
+        }
+    }
+}
+
+// ---- launch ------------------------------------------------------------------------------------------------------------------
+struct Plan {
+    bool skinny, fused;
+    int mt, nt;          // skinny: tiles of 16 rows of x / of W
+    int tile;            // 256, 128, 64
+    int splits, block;   // k_shrink: parts of K, rows per workgroup
+};
+constexpr int kCus = 256;
+
+Plan make_plan(const AdapterOp& op) {
+    Plan p{};
+    const int rt = padded_rank(op.rank) / 16;
+    const int pairs = (op.K * (op.type == kFp32 ? 4 : 2) + 127) / 128;
+    p.skinny = op.rows <= 64;
+    if (p.skinny) {
+        p.mt = (op.rows + 15) / 16;
+        // more rows of W per workgroup once there are enough workgroups: x is read once per workgroup
+        p.nt = p.mt == 1 ? (op.N > 16 * 2 * kCus ? 2 : 1) : p.mt == 2 ? 2 : 4;
+        // every workgroup reads the A of all rows: only while that is little
+        p.fused = p.mt == 1 && op.rows * rt <= 2;
+        p.block = 16;
+    } else {
+        p.block = op.rows <= 1024 ? 16 : 128;
+        auto tiles = [&](int b) { return (long long)((op.rows + b - 1) / b) * ((op.N + b - 1) / b); };
+        p.tile = tiles(256) >= kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
+    }
+    const int blocks = (op.rows + p.block - 1) / p.block;
+    int s = (2 * kCus + blocks - 1) / blocks;
+    p.splits = s < 1 ? 1 : s > 16 ? 16 : s;
+    if (p.splits > (pairs + 1) / 2) p.splits = (pairs + 1) / 2;
+    if (p.fused) p.splits = 0;
+    return p;
+}
+
+template <typename T, int MT, int NT, int FJ>
+void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
+    const size_t lds = skinny_lds<MT, NT, FJ>() + (size_t)op.rows * padded_rank(op.rank) * 4;
+    lds_optin((const void*)k_skinny<T, MT, NT, FJ>);
+    k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT)), dim3(64 * kSkinnyWaves), lds, st>>>(op, part, splits);
+}
+template <typename T, int B, int WM, int WN>
+void launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
+    const int nt = ((op.rows + B - 1) / B) * ((op.N + B - 1) / B);
+    const size_t es = sizeof(T), ring = kRing * tile_stage_bytes<B, B>(), tl = (size_t)B * (padded_rank(op.rank) + 4) * 4;
+    const bool dma = ((uintptr_t)op.x | (uintptr_t)op.w) % 16 == 0 && op.x_stride * es % 16 == 0 && op.w_stride * es % 16 == 0 &&
+                     (long long)B * op.x_stride * (long long)es < (1ll << 31) && (long long)B * op.w_stride * (long long)es < (1ll << 31);
+    const size_t lds = kOrderBytes<B> + (ring > tl ? ring : tl);
+    if (dma) {
+        lds_optin((const void*)k_tile<T, B, B, WM, WN, true>);
+        k_tile<T, B, B, WM, WN, true><<<dim3(nt), dim3(64 * WM * WN), lds, st>>>(op, part, splits);
+    } else {
+        lds_optin((const void*)k_tile<T, B, B, WM, WN, false>);
+        k_tile<T, B, B, WM, WN, false><<<dim3(nt), dim3(64 * WM * WN), lds, st>>>(op, part, splits);
+    }
+}
+template <typename T, int BR>
+void launch_shrink(hipStream_t st, const AdapterOp& op, float* part, int splits) {
+    const dim3 grid((op.rows + BR - 1) / BR, splits);
+    const int rt = padded_rank(op.rank) / 16;
+    if (rt == 1) k_shrink<T, 1, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
+    else if (rt == 2) k_shrink<T, 2, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
+    else if (rt <= 4) k_shrink<T, 4, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
+    else k_shrink<T, 8, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
+}
+
+template <typename T>
 hipError_t launch_typed(hipStream_t st, const AdapterOp& op, void* workspace) {
-    float* t = static_cast<float*>(workspace);
-    k_shrink<T><<<dim3((unsigned)(((long long)op.rows * op.rank + 3) / 4)), dim3(256), 0, st>>>(op, t);
-    if (hipError_t e = hipGetLastError()) return e;
-    const unsigned nt = (unsigned)((op.rows + 63) / 64) * ((op.N + 63) / 64);
-    k_project<T, O><<<dim3(nt), dim3(256), 0, st>>>(op, t);
+    const Plan p = make_plan(op);
+    float* part = static_cast<float*>(workspace);
+    if (!p.fused) {
+        if (p.block == 16) launch_shrink<T, 16>(st, op, part, p.splits);
+        else launch_shrink<T, 128>(st, op, part, p.splits);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    if (p.skinny) {
+        if (p.fused && p.nt == 1) launch_skinny<T, 1, 1, 2>(st, op, part, p.splits);
+        else if (p.fused) launch_skinny<T, 1, 2, 2>(st, op, part, p.splits);
+        else if (p.mt == 1 && p.nt == 1) launch_skinny<T, 1, 1, 0>(st, op, part, p.splits);
+        else if (p.mt == 1) launch_skinny<T, 1, 2, 0>(st, op, part, p.splits);
+        else if (p.mt == 2) launch_skinny<T, 2, 2, 0>(st, op, part, p.splits);
+        else if (p.mt == 3) launch_skinny<T, 3, 4, 0>(st, op, part, p.splits);
+        else launch_skinny<T, 4, 4, 0>(st, op, part, p.splits);
+    } else if (p.tile == 256) {
+        launch_tile<T, 256, 4, 2>(st, op, part, p.splits);
+    } else if (p.tile == 128) {
+        launch_tile<T, 128, 2, 2>(st, op, part, p.splits);
+    } else {
+        launch_tile<T, 64, 2, 2>(st, op, part, p.splits);
+    }
+    if (hipError_t e = take_optin_error()) return e;
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t adapter_workspace_bytes(const AdapterOp& op) { return (size_t)op.rows * op.rank * sizeof(float); }
+size_t adapter_workspace_bytes(const AdapterOp& op) {
+    if (op.rows == 0) return 0;
+    const Plan p = make_plan(op);
+    return p.fused ? 0 : (size_t)p.splits * op.rows * padded_rank(op.rank) * sizeof(float);
+}
 
 hipError_t launch_adapter(hipStream_t st, const AdapterOp& op, void* workspace) {
-    const bool f = op.out_type == kFp32;
     switch (op.type) {
-        case kFp32: return launch_typed<float, float>(st, op, workspace);
-        case kBf16: return f ? launch_typed<bf16_t, float>(st, op, workspace) : launch_typed<bf16_t, bf16_t>(st, op, workspace);
-        default: return f ? launch_typed<_Float16, float>(st, op, workspace) : launch_typed<_Float16, _Float16>(st, op, workspace);
+        case kFp32: return launch_typed<float>(st, op, workspace);
+        case kBf16: return launch_typed<bf16_t>(st, op, workspace);
+        default: return launch_typed<_Float16>(st, op, workspace);
     }
 }
 

@@ -11,6 +11,7 @@ using namespace mz;
 namespace {
 
 constexpr int kMaxRank = 128;
+constexpr int kMaxSampleRows = 1 << 21;     // a workgroup of up to 1024 threads each: below 2^32 threads
 constexpr int kMaxSampleActions = 262144;   // 2^18: sample.hip's histogram masses are sums of 2^46 in 64 bits
 
 // The device all operands live on: the first pointer names it, every other one must agree.
@@ -83,7 +84,7 @@ int run_op(Operands& o, void* workspace, size_t have, size_t need, void* stream,
 
 const char* check_sample(const mz_sample_args* a) {
     if (!a) return "args is NULL";
-    if (a->rows < 0) return "rows < 0";
+    if (a->rows < 0 || a->rows > kMaxSampleRows) return "rows must be 0 .. 2097152";
     if (a->actions < 1 || a->actions > kMaxSampleActions) return "actions must be 1 .. 262144";
     if (!known_type(a->dtype)) return "unknown dtype";
     if (!a->row_temperature && !(a->temperature >= 0 && std::isfinite(a->temperature))) return "temperature must be finite and >= 0";
@@ -124,6 +125,7 @@ SampleOp sample_op(const mz_sample_args& a) {
 const char* check_adapter(const mz_adapter_args* a) {
     if (!a) return "args is NULL";
     if (a->rows < 0) return "rows < 0";
+    if (((long long)a->rows + 255) / 256 * (((long long)a->out_features + 255) / 256) > (1 << 22) || a->out_features > (1 << 26)) return "too many outputs for one call";
     if (a->in_features < 1 || a->out_features < 1) return "in_features and out_features must be >= 1";
     if (a->rank < 1 || a->rank > kMaxRank) return "rank must be 1 .. 128";
     if (a->adapters < 1) return "adapters must be >= 1";

@@ -85,3 +85,10 @@ def test_adapter_needs_device_tensors():
     assert C.sizeof(capi.AdapterArgs) == 8 * 4 + 12 * 8 - 8
     with pytest.raises(capi.MuZeroError, match="GPU"):
         ops.adapter_linear(z(2, 8), z(4, 8), z(1, 2, 8), z(1, 4, 2), z(2, dtype=torch.int32))
+
+
+def test_adapter_of_no_rows():
+    a = capi.AdapterArgs(rows=0, in_features=64, out_features=32, rank=4, adapters=2, dtype=1, out_dtype=1, x_stride=64,
+                         weight_stride=64, y_stride=32)
+    assert capi.lib().mz_adapter_workspace_bytes(C.byref(a)) == 0
+    assert capi.lib().mz_adapter_linear(C.byref(a), None, 0, None) == 0
