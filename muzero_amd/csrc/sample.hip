@@ -324,56 +324,66 @@ __global__ __launch_bounds__(W * kWaveRows) void k_sample_wave(SampleOp op) {
 
 // ---- a workgroup per row ---------------------------------------------------------------------------------------------------
 template <typename T>
-struct RowView {
-    const T* src;           // entry 0
-    const uint8_t* legal;
-    int A, shift, nvec;     // vector v = the 16 aligned bytes with the entries [v * VEC - shift, + VEC)
-};
-template <typename T>
 struct Vec {
     static constexpr int N = 16 / sizeof(T);
     float z[N];
+    int i0;                 // index of z[0]
 };
 template <typename T>
-__device__ __forceinline__ void unpack(const u32x4 d, float* z) {
+struct RowView {
+    const T* src;
+    const uint8_t* legal;
+    int A, nvec;            // A >= Vec<T>::N; vector v = the entries [v N, v N + N), the last one moved back to end with the row
+};
+// Vector v: 16 bytes wherever they start.  Entries without a part in the draw - masked, NaN, -inf, and in the last vector those
+// that the vector before has - are -inf; a vector behind the last (v >= end) is all that.  CLEAN = false leaves NaN and -0 in.
+template <bool CLEAN, typename T>
+__device__ __forceinline__ Vec<T> load_vec(const RowView<T>& r, int v, int end) {
+    constexpr int N = Vec<T>::N;
+    Vec<T> o;
+    const int want = v * N;
+    o.i0 = min(want, r.A - N);
+    u32x4 d;
+    __builtin_memcpy(&d, r.src + o.i0, 16);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) z[i] = __uint_as_float(d[i]);
+        for (int i = 0; i < 4; i++) o.z[i] = __uint_as_float(d[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const uint16_t h = (uint16_t)(d[i >> 1] >> (16 * (i & 1)));
             T t;
             __builtin_memcpy(&t, &h, 2);
-            z[i] = to_float(t);
+            o.z[i] = to_float(t);
         }
     }
-}
-// one vector of the row; entries outside the row, masked or without a value are -inf
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const RowView<T>& r, int v) {
-    constexpr int N = Vec<T>::N;
-    Vec<T> o;
-    const int i0 = v * N - r.shift;
-    if (i0 >= 0 && i0 + N <= r.A) {
-        unpack<T>(*reinterpret_cast<const u32x4*>(r.src + i0), o.z);
-        if (r.legal) {
-            uint8_t l[N];
-            __builtin_memcpy(l, r.legal + i0, N);
+    if (r.legal) {
+        uint32_t l[N / 4];
+        __builtin_memcpy(l, r.legal + o.i0, N);
 #pragma unroll
-            for (int i = 0; i < N; i++) o.z[i] = clean(o.z[i], l[i] != 0);
-        } else {
+        for (int i = 0; i < N; i++) o.z[i] = (l[i >> 2] >> (8 * (i & 3)) & 255u) ? o.z[i] : -INFINITY;
+    }
+    if (v >= end || want != o.i0) {
+        const int skip = v >= end ? N : want - o.i0;
 #pragma unroll
-            for (int i = 0; i < N; i++) o.z[i] = clean(o.z[i], true);
-        }
-    } else {
+        for (int i = 0; i < N; i++)
+            if (i < skip) o.z[i] = -INFINITY;
+    }
+    if constexpr (CLEAN) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int j = i0 + i;
-            o.z[i] = j >= 0 && j < r.A ? clean(to_float(r.src[j]), !r.legal || r.legal[j]) : -INFINITY;
-        }
+        for (int i = 0; i < N; i++) o.z[i] = fmaxf(o.z[i], -INFINITY) + 0.0f;   // NaN -> -inf, -0 -> +0
     }
     return o;
+}
+// f(vector) over this wave's vectors [v0, v1): lanes take consecutive vectors, all lanes take part in every call
+template <bool CLEAN = true, typename T, typename F>
+__device__ __forceinline__ void wave_pass(const RowView<T>& r, int v0, int v1, int lane, F f) {
+#pragma unroll 1
+    for (int v = v0; v < v1; v += 2 * W) {
+        const Vec<T> a = load_vec<CLEAN>(r, v + lane, v1), b = load_vec<CLEAN>(r, v + W + lane, v1);
+        f(a);
+        f(b);
+    }
 }
 
 template <int NT>
@@ -384,38 +394,23 @@ struct Shared {
     u64 list[kList];
     uint32_t group[256];
     double wd[NW];
-    double wd2[NW];
     int wi[NW];
-    float wf[NW], wf2[NW];
+    float wf[NW];
     int list_n, bin;
     uint32_t bound;
     double above_mass;
     int above_cnt, bin_cnt;
-    double out_d[2];
-    int out_i[4];
+    double out_d;
+    int out_i;
+    float out_f;
     u64 out_r;
 };
 
-// f(vector, first index) over this wave's vectors [v0, v1): lanes take consecutive vectors
-template <typename T, typename F>
-__device__ __forceinline__ void wave_pass(const RowView<T>& r, int v0, int v1, int lane, F f) {
-    constexpr int N = Vec<T>::N;
-    int v = v0 + lane;
-    for (; v + 3 * W < v1; v += 4 * W) {
-        const Vec<T> a = load_vec(r, v), b = load_vec(r, v + W), c = load_vec(r, v + 2 * W), d = load_vec(r, v + 3 * W);
-        f(a, v * N - r.shift);
-        f(b, (v + W) * N - r.shift);
-        f(c, (v + 2 * W) * N - r.shift);
-        f(d, (v + 3 * W) * N - r.shift);
-    }
-    for (; v < v1; v += W) f(load_vec(r, v), v * N - r.shift);
-}
-
 // First entry in index order at which the running sum of wf(z, index) exceeds target(total); the last entry with a weight if
 // none does.  Sums in a fixed order: vector, lane, wave segments, then the segment of the border again in 1/NW pieces.
-// Every thread returns the index; *total and the entry's z likewise.
-template <typename T, int NT, typename WF, typename TF>
-__device__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, double* total, float* z_out) {
+// Every thread returns the index; *total and the entry's z likewise.  `seen` is called once for every entry.
+template <int NT, typename T, typename WF, typename TF, typename SF>
+__device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, SF seen, double* total, float* z_out) {
     constexpr int NW = NT / W, N = Vec<T>::N;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo = 0, hi = r.nvec;
@@ -425,9 +420,13 @@ __device__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, 
         const int per = ((hi - lo + NW - 1) / NW + W - 1) / W * W;
         const int v0 = min(hi, lo + wave * per), v1 = min(hi, v0 + per);
         double s = 0;
-        wave_pass(r, v0, v1, lane, [&](const Vec<T>& x, int i0) {
+        wave_pass(r, v0, v1, lane, [&](const Vec<T>& x) {
 #pragma unroll
-            for (int i = 0; i < N; i++) s += wf(x.z[i], i0 + i);
+            for (int i = 0; i < N; i++) s += wf(x.z[i], x.i0 + i);
+            if (level == 0) {
+#pragma unroll
+                for (int i = 0; i < N; i++) seen(x.z[i], x.i0 + i);
+            }
         });
         s = wave_sum(s);
         __syncthreads();
@@ -466,15 +465,12 @@ __device__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, 
     if (wave == 0) {
         int found = -1, last = -1;
         float fz = 0, lz = 0;
+#pragma unroll 1
         for (int v = lo; v < hi && found < 0; v += W) {
-            Vec<T> x;
-            const bool on = v + lane < hi;
-            if (on) x = load_vec(r, v + lane);
-            const int i0 = (v + lane) * N - r.shift;
+            const Vec<T> x = load_vec<true>(r, v + lane, hi);
             double s = 0;
-            if (on)
 #pragma unroll
-                for (int i = 0; i < N; i++) s += wf(x.z[i], i0 + i);
+            for (int i = 0; i < N; i++) s += wf(x.z[i], x.i0 + i);
             const double inc = wave_scan(s, lane);
             const double prev = __shfl_up(inc, 1);
             const u64 some = __ballot(s > 0), over = __ballot(s > 0 && base + inc > target);
@@ -486,14 +482,14 @@ __device__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, 
                     double c = base + (lane ? prev : 0.0);
 #pragma unroll
                     for (int i = 0; i < N; i++) {
-                        const double w = wf(x.z[i], i0 + i);
+                        const double w = wf(x.z[i], x.i0 + i);
                         c += w;
                         if (w > 0) {
-                            ml = i0 + i;
+                            ml = x.i0 + i;
                             mlz = x.z[i];
                             if (mi < 0 && c > target) {
-                                mi = i0 + i;
-                                mz = x.z[i];
+                                mi = ml;
+                                mz = mlz;
                             }
                         }
                     }
@@ -512,20 +508,20 @@ __device__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, 
             base += __shfl(inc, 63);
         }
         if (lane == 0) {
-            sh.out_i[0] = found < 0 ? last : found;
-            sh.wf[0] = found < 0 ? lz : fz;
+            sh.out_i = found < 0 ? last : found;
+            sh.out_f = found < 0 ? lz : fz;
         }
     }
     __syncthreads();
-    const int res = sh.out_i[0];
-    *z_out = sh.wf[0];
+    const int res = sh.out_i;
+    *z_out = sh.out_f;
     __syncthreads();
     return res;
 }
 
-// Entry `list` (unordered, n <= 256) finished by one wave: prefix, draw, output.  All z of the row that can be kept are in it.
+// The list (unordered, n <= 64 E) finished by one wave: prefix, draw, output.  All entries of the row that can be kept are in it.
 template <int NT, int E>
-__device__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, const RowParams& rp, const Scale& sc, double mass, int lane) {
+__device__ __forceinline__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, const RowParams& rp, const Scale& sc, double mass, int lane) {
     u64 r[E];
 #pragma unroll
     for (int e = 0; e < E; e++) r[e] = e * W + lane < n ? sh.list[e * W + lane] : 0ull;
@@ -538,13 +534,8 @@ __device__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, 
     for (int e = 0; e < E; e++) o[e] = e * W + lane < keep ? (r[e] << 32) | (r[e] >> 32) : 0ull;   // ~index first: descending = index ascending
     wave_sort<E>(o, lane);
     double w[E];
-    float z[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const u64 t = (o[e] << 32) | (o[e] >> 32);
-        z[e] = o[e] ? of_key((uint32_t)(t >> 32)) : -INFINITY;
-        w[e] = o[e] ? weight(z[e], sc) : 0.0;
-    }
+    for (int e = 0; e < E; e++) w[e] = o[e] ? weight(of_key((uint32_t)o[e]), sc) : 0.0;
     double total;
     const int pos = wave_draw<E>(w, rp.u, lane, &total);
     const u64 d = at_position<E>(o, pos);
@@ -554,12 +545,12 @@ __device__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, 
         const double x = (double)zp == sc.zmax ? 0.0 : (double)zp - sc.zmax;
         write_row(op, row, pick, x / rp.T - log(total), keep);
         sh.out_r = border;
-        sh.out_d[0] = total;
+        sh.out_d = total;
     }
 }
-// The border inside a crossing bin whose entries are listed: *border = its rank value, returns how many of the list are kept.
+// The border inside a crossing bin whose entries are listed: its rank value.
 template <int NT, int E>
-__device__ int border_of_list(Shared<NT>& sh, int n, int want, double before, double target, const Scale& sc, int lane, u64* border) {
+__device__ __forceinline__ u64 border_of_list(Shared<NT>& sh, int n, int want, double before, double target, const Scale& sc, int lane) {
     u64 r[E];
 #pragma unroll
     for (int e = 0; e < E; e++) r[e] = e * W + lane < n ? sh.list[e * W + lane] : 0ull;
@@ -578,24 +569,48 @@ __device__ int border_of_list(Shared<NT>& sh, int n, int want, double before, do
         }
         keep = max(keep, 1);
     }
-    *border = at_position<E>(r, keep - 1);
-    return keep;
+    return at_position<E>(r, keep - 1);
 }
 
 // log2-spaced bin of an entry, 32 to a factor of two below the maximum, the last one open; its weight is 2^(-(bin >> 5)) times
-// the value 2^f, f in [-0.5, 0.5], returned beside it
+// 2^f, f in [-0.5, 0.5], returned beside it
+constexpr double kDeep = -63.4375;                     // bin 2046
 __device__ __forceinline__ int bin_of(float z, const Scale& s, double* f) {
-    const double y = fmax(log2_weight(z, s), -63.4375);   // bin 2046 at the deepest
-    const int b = z > -INFINITY && log2_weight(z, s) < -63.4375 ? kBins - 1 : (int)((0.5 - y) * 32.0);
+    const double y = log2_weight(z, s);
+    const int b = (int)((0.5 - fmax(y, kDeep)) * 32.0);
     *f = y + (double)(b >> 5);
-    return b;
+    return y < kDeep ? kBins - 1 : b;
+}
+// Smallest key in [lo, hi] that `is` holds for; it holds for hi and, monotone, for every key above one it holds for.  64 keys a
+// step, the first ones around `guess`.
+template <typename P>
+__device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, float guess, int lane, P is) {
+    uint32_t at = key_of(guess);
+    at = max(lo, at < lo + 32 ? lo : at - 32);
+    uint32_t step = 1;
+#pragma unroll 1
+    while (lo < hi) {
+        const uint32_t k = at + step * lane;                      // keys above hi count as true
+        const bool t = k < at || k >= hi || is(of_key(k));
+        const u64 b = __ballot(t);
+        if (b & 1) hi = min(hi, at);
+        else if (b) {
+            const int l = __ffsll(b) - 1;
+            lo = at + step * (l - 1) + 1;
+            const uint32_t h = at + step * l;
+            hi = h < at ? hi : min(hi, h);
+        } else lo = at + step * 63 + 1;
+        step = (hi - lo) / 64 + 1;
+        at = lo;
+    }
+    return lo;
 }
 
-struct Border {       // kept: z > z0 or (z == z0 and index <= i0)
+struct Border {       // kept: z > z0 or (z == z0 and index <= i0); z0 > -inf
     float z0;
     int i0;
 };
-__device__ __forceinline__ bool inside(float z, int i, const Border& b) { return z > b.z0 || (z == b.z0 && i <= b.i0 && z > -INFINITY); }
+__device__ __forceinline__ bool inside(float z, int i, const Border& b) { return z > b.z0 || (z == b.z0 && i <= b.i0); }
 
 // p in [0.7, 1.42] as an integer of kFix fraction bits on top of the bits of 128.0 (2^(52 - 45) = 128)
 __device__ __forceinline__ u64 fixed_bits(double p) { return (u64)__double_as_longlong(p + 128.0); }
@@ -620,16 +635,12 @@ struct LowBits<_Float16> {
 template <typename T, int NT>
 struct Row {
     static constexpr int NW = NT / W, N = Vec<T>::N;
-    const SampleOp& op;
     Shared<NT>& sh;
     RowView<T> view;
     Scale sc;
-    int row, lane, wave, v0, v1;
+    int lane, wave, v0, v1;
 
-    template <typename F>
-    __device__ void pass(F f) { wave_pass(view, v0, v1, lane, f); }
-
-    __device__ void clear_hist(bool with_mass) {
+    __device__ __forceinline__ void clear_hist(bool with_mass) {
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += NT) {
             sh.cnt[i] = 0;
@@ -638,28 +649,27 @@ struct Row {
         if (threadIdx.x == 0) sh.bin = -1;
         __syncthreads();
     }
-    // entries with z >= zlo, z <= zhi inside `b` -> sh.list; returns how many there are (the list holds at most kList)
-    __device__ int gather(float zlo, float zhi, const Border& b) {
+    // entries with zlo <= z <= zhi inside `b` -> sh.list; returns how many there are (the list holds at most kList)
+    __device__ __forceinline__ int gather(float zlo, float zhi, const Border& b) {
         __syncthreads();
         if (threadIdx.x == 0) sh.list_n = 0;
         __syncthreads();
-        pass([&](const Vec<T>& x, int i0) {
+        wave_pass(view, v0, v1, lane, [&](const Vec<T>& x) {
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (x.z[i] >= zlo && x.z[i] <= zhi && inside(x.z[i], i0 + i, b)) {
+                if (x.z[i] >= zlo && x.z[i] <= zhi && inside(x.z[i], x.i0 + i, b)) {
                     const int p = atomicAdd(&sh.list_n, 1);
-                    if (p < kList) sh.list[p] = rank_of(x.z[i], i0 + i);
+                    if (p < kList) sh.list[p] = rank_of(x.z[i], x.i0 + i);
                 }
         });
         __syncthreads();
         return sh.list_n;
     }
     // Scans the histogram: picks the last non-empty bin whose predecessors count < want (want >= 0) or hold mass < frac * total
-    // (want < 0; *total_mass receives the total when `fresh`, is the given total otherwise); counts and masses start at the
-    // given offsets.  exponent_of(bin) gives the power of two of a bin's masses.
-    template <typename EX>
-    __device__ int pick_bin(int want, double frac, bool fresh, double* total_mass, int cnt0, double mass0, EX exponent_of, int* above_cnt, double* above_mass,
-                            int* bin_cnt) {
+    // (want < 0; *total receives the whole mass when `fresh`); counts and masses start at the given offsets.  A bin's masses
+    // are in units of 2^(e0 - (bin >> shift)), and zero from bin `open` on.
+    __device__ __forceinline__ int pick_bin(int want, double frac, bool fresh, double* total, int cnt0, double mass0, int e0, int shift, int open, int* above_cnt,
+                                            double* above_mass, int* bin_cnt) {
         constexpr int PER = kBins / NT;
         uint32_t c[PER];
         double m[PER];
@@ -669,7 +679,7 @@ struct Row {
         for (int i = 0; i < PER; i++) {
             const int b = threadIdx.x * PER + i;
             c[i] = sh.cnt[b];
-            m[i] = want < 0 && c[i] ? of_fixed(sh.mass[b], c[i], exponent_of(b)) : 0.0;
+            m[i] = want < 0 && c[i] && b < open ? of_fixed(sh.mass[b], c[i], e0 - (b >> shift)) : 0.0;
             ct += (int)c[i];
             mt += m[i];
         }
@@ -689,8 +699,8 @@ struct Row {
             }
             all += sh.wd[i];
         }
-        if (fresh) *total_mass = all;
-        const double target = want < 0 ? frac * *total_mass : 0.0;
+        if (fresh) *total = all;
+        const double target = want < 0 ? frac * *total : 0.0;
         const double mprev = __shfl_up(mi, 1);
         cb += ci - ct;
         mb += lane ? mprev : 0.0;
@@ -719,96 +729,70 @@ struct Row {
         *bin_cnt = sh.bin_cnt;
         return sh.bin;
     }
-    __device__ void add(int b, bool with_mass, double f) {
-        atomicAdd(&sh.cnt[b], 1u);
-        if (with_mass) atomicAdd(&sh.mass[b], fixed_bits(exp2_frac(f)));
-    }
 
-    // The border of the prefix of entries inside `b0` with `want` entries (want >= 0), or (want < 0) with the entries whose
+    // The border of the prefix of the entries inside `b0` with `want` entries (want >= 0), or (want < 0) with the entries whose
     // predecessors hold less than frac of the whole mass.  A histogram over log2-spaced bins, then - inside the border's bin -
     // over its range of float keys, until 256 entries or a single value are left.
     // *small: set when everything down to the border's bin is a list of <= 256 entries: sh.list holds it, *mass the whole mass.
-    __device__ Border select(int want, double frac, const Border& b0, bool* small, int* list_n, double* mass) {
+    __device__ __forceinline__ Border select(int want, double frac, const Border b0, bool* small, int* list_n, double* mass) {
         const bool wm = want < 0;
-        clear_hist(wm);
-        pass([&](const Vec<T>& x, int i0) {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (inside(x.z[i], i0 + i, b0)) {
-                    double f;
-                    const int b = bin_of(x.z[i], sc, &f);
-                    add(b, wm && b < kBins - 1, f);
-                }
-        });
-        // the open bin: count without mass (each entry < 2^-63 of the maximum)
-        __syncthreads();
-        if (wm && threadIdx.x == 0) sh.mass[kBins - 1] = (u64)sh.cnt[kBins - 1] * (u64)__double_as_longlong(128.0);
-        __syncthreads();
-        int above, cnt;
-        double above_mass;
-        int bin = pick_bin(want, frac, true, mass, 0, 0.0, [](int b) { return -(b >> 5); }, &above, &above_mass, &cnt);
-        const double target = frac * *mass;
-        const int shift_n = bin >> 5;
-        const bool open = bin == kBins - 1;
-        // the bin's range of keys, by bisection on the (monotone) bin number
-        uint32_t klo, khi;
-        {
-            uint32_t lo = kNoKey + 1, hi = key_of((float)sc.zmax);   // smallest key with bin <= `bin`
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                double f;
-                if (bin_of(of_key(mid), sc, &f) <= bin) hi = mid;
-                else lo = mid + 1;
-            }
-            klo = lo;
-            lo = klo;
-            hi = key_of((float)sc.zmax);                             // largest key with bin >= `bin`
-            while (lo < hi) {
-                const uint32_t mid = hi - (hi - lo) / 2;
-                double f;
-                if (bin_of(of_key(mid), sc, &f) >= bin) lo = mid;
-                else hi = mid - 1;
-            }
-            khi = lo;
-        }
+        int above = 0, cnt = 0, shift = 0, n_bin = 0;
+        double above_mass = 0;
+        uint32_t klo = kNoKey + 1, khi = key_of((float)sc.zmax);
+        bool open = false;
         *small = false;
-        if (above + cnt <= kList) {
-            *list_n = gather(of_key(klo), INFINITY, b0);
-            *small = true;
-            return b0;
-        }
-        while (cnt > kList && (khi >> LowBits<T>::N) != (klo >> LowBits<T>::N)) {
-            const uint32_t range = khi - klo;
-            const int sh_bits = max(0, 32 - __clz((int)range) - 11);
+#pragma unroll 1
+        for (int level = 0;; level++) {
             clear_hist(wm);
             const float zl = of_key(klo), zh = of_key(khi);
-            pass([&](const Vec<T>& x, int i0) {
+            const uint32_t kh = khi;
+            wave_pass(view, v0, v1, lane, [&](const Vec<T>& x) {
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (x.z[i] >= zl && x.z[i] <= zh && inside(x.z[i], i0 + i, b0)) {
+                for (int i = 0; i < N; i++) {
+                    const float z = x.z[i];
+                    if (z >= zl && z <= zh && inside(z, x.i0 + i, b0)) {
                         double f;
-                        bin_of(x.z[i], sc, &f);
-                        add((int)((khi - key_of(x.z[i])) >> sh_bits), wm && !open, f);
+                        int b = bin_of(z, sc, &f);
+                        const bool heavy = wm && b < kBins - 1;      // the open bin: below 2^-63 of the maximum each, no mass
+                        if (level) b = (int)((kh - key_of(z)) >> shift);
+                        atomicAdd(&sh.cnt[b], 1u);
+                        if (heavy) atomicAdd(&sh.mass[b], fixed_bits(exp2_frac(f)));
                     }
+                }
             });
             __syncthreads();
-            if (wm && open) {
-                for (int i = threadIdx.x; i < kBins; i += NT) sh.mass[i] = (u64)sh.cnt[i] * (u64)__double_as_longlong(128.0);
-                __syncthreads();
+            if (level == 0) {
+                const int bin = pick_bin(want, frac, true, mass, 0, 0.0, 0, 5, kBins - 1, &above, &above_mass, &cnt);
+                n_bin = bin >> 5;
+                open = bin == kBins - 1;
+                // the bin's range of keys
+                const double zb = sc.zmax + (0.5 - bin / 32.0) / sc.c, za = sc.zmax + (0.5 - (bin + 1) / 32.0) / sc.c;
+                const Scale s = sc;
+                const uint32_t top = khi;
+                if (!open) klo = first_key(klo, top, (float)za, lane, [=](float z) { double f; return bin_of(z, s, &f) <= bin; });
+                khi = first_key(klo, top + 1, (float)zb, lane, [=](float z) { double f; return bin_of(z, s, &f) < bin; }) - 1;
+                if (above + cnt <= kList) {
+                    *list_n = gather(of_key(klo), INFINITY, b0);
+                    *small = true;
+                    return b0;
+                }
+            } else {
+                const int a0 = above;
+                const double m0 = above_mass;
+                const int rb = pick_bin(want, frac, false, mass, a0, m0, -n_bin, 30, open ? 0 : kBins, &above, &above_mass, &cnt);
+                khi = khi - ((uint32_t)rb << shift);
+                const uint32_t width = (1u << shift) - 1;
+                klo = khi - klo > width ? khi - width : klo;
             }
-            const int a0 = above;
-            const double m0 = above_mass;
-            const int rb = pick_bin(want, frac, false, mass, a0, m0, [=](int) { return -shift_n; }, &above, &above_mass, &cnt);
-            khi = khi - ((uint32_t)rb << sh_bits);
-            const uint32_t width = (1u << sh_bits) - 1;
-            klo = khi - klo > width ? khi - width : klo;
+            if (cnt <= kList || (khi >> LowBits<T>::N) == (klo >> LowBits<T>::N)) break;
+            shift = max(0, 32 - __clz((int)(khi - klo)) - 11);
         }
+        const double target = frac * *mass;
         Border b;
         if (cnt <= kList) {
             const int n = gather(of_key(klo), of_key(khi), b0);
             if (wave == 0) {
-                u64 border;
-                border_of_list<NT, kList / W>(sh, n, wm ? -1 : want - above, above_mass, target, sc, lane, &border);
+                const u64 border = border_of_list<NT, kList / W>(sh, n, wm ? -1 : want - above, above_mass, target, sc, lane);
                 if (lane == 0) sh.out_r = border;
             }
             __syncthreads();
@@ -837,22 +821,19 @@ struct Row {
             double tot;
             float zz;
             const Border bb = b0;
-            b.i0 = locate<T, NT>(view, sh, [=](float z, int i) { return z == zv && inside(z, i, bb) ? 1.0 : 0.0; }, [=](double) { return (double)ties - 1.0; }, &tot, &zz);
+            b.i0 = locate<NT>(view, sh, [=](float z, int i) { return z == zv && inside(z, i, bb) ? 1.0 : 0.0; }, [=](double) { return (double)ties - 1.0; },
+                              [](float, int) {}, &tot, &zz);
         }
         return b;
     }
 };
 
 // Smallest float whose weight is at least m: min-p as a border (the weights are monotone in z)
-__device__ __forceinline__ float min_p_border(double m, double T, const Scale& sc) {
-    if (!(m > 0) || sc.zmax == INFINITY) return sc.zmax == INFINITY && m > 0 ? INFINITY : -FLT_MAX;
-    uint32_t lo = kNoKey + 1, hi = key_of((float)sc.zmax);
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (weight(of_key(mid), sc) >= m) hi = mid;
-        else lo = mid + 1;
-    }
-    return of_key(lo);
+__device__ __forceinline__ float min_p_border(double m, double T, const Scale& sc, int lane) {
+    if (!(m > 0)) return -FLT_MAX;
+    if (sc.zmax == (double)INFINITY) return INFINITY;
+    const float guess = (float)fmax(sc.zmax + T * log(m), -(double)FLT_MAX);
+    return of_key(first_key(kNoKey + 1, key_of((float)sc.zmax), guess, lane, [=](float z) { return weight(z, sc) >= m; }));
 }
 
 template <typename T, int NT>
@@ -860,14 +841,13 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
     constexpr int NW = NT / W, N = Vec<T>::N;
     __shared__ Shared<NT> sh;
     const int row = blockIdx.x, tid = threadIdx.x;
-    const int lane = tid & 63, wave = tid >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int A = op.actions;
     RowView<T> view;
     view.src = static_cast<const T*>(op.logits) + row * op.row_stride;
     view.legal = op.legal ? op.legal + row * op.legal_stride : nullptr;
     view.A = A;
-    view.shift = (int)((reinterpret_cast<uintptr_t>(view.src) & 15) / sizeof(T));
-    view.nvec = (A + view.shift + N - 1) / N;
+    view.nvec = (A + N - 1) / N;
     const int per = ((view.nvec + NW - 1) / NW + W - 1) / W * W;
     const int v0 = min(view.nvec, wave * per), v1 = min(view.nvec, v0 + per);
     const RowParams rp = row_params(op, row);
@@ -875,7 +855,7 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
 
     float tmax = -INFINITY;
     int tcnt = 0;
-    wave_pass(view, v0, v1, lane, [&](const Vec<T>& x, int) {
+    wave_pass<false>(view, v0, v1, lane, [&](const Vec<T>& x) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             tmax = fmaxf(tmax, x.z[i]);
@@ -883,6 +863,7 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         }
     });
     {
+        tmax += 0.0f;
         const float m = wave_max(tmax);
         const int c = wave_sum(tcnt);
         if (lane == 0) {
@@ -891,7 +872,10 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         }
         // 256 partial maxima
         float g = tmax;
-        if (NT == 1024) g = fmaxf(fmaxf(g, __shfl_xor(g, 1)), fmaxf(__shfl_xor(g, 2), __shfl_xor(g, 3)));
+        if (NT == 1024) {
+            g = fmaxf(g, __shfl_xor(g, 1));
+            g = fmaxf(g, __shfl_xor(g, 2));
+        }
         if (tid % (NT / 256) == 0) sh.group[tid / (NT / 256)] = key_of(g);
     }
     __syncthreads();
@@ -902,34 +886,33 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         count += sh.wi[i];
     }
     __syncthreads();
-    if (!rp.valid || count == 0) {
-        if (tid == 0) write_row(op, row, -1, 0.0, 0);
-        if (probs)
-            for (int i = tid; i < A; i += NT) probs[i] = 0.f;
-        return;
-    }
-    double total;
-    float zp;
-    if (rp.T == 0) {
-        const int pick = locate<T, NT>(view, sh, [=](float z, int) { return z == zmax ? 1.0 : 0.0; }, [](double) { return 0.0; }, &total, &zp);
-        if (tid == 0) write_row(op, row, pick, 0.0, 1);
+    const bool none = !rp.valid || count == 0;
+    double total = 1.0;
+    if (none || rp.T == 0) {
+        int pick = -1;
+        if (!none) {
+            float zp;
+            pick = locate<NT>(view, sh, [=](float z, int) { return z == zmax ? 1.0 : 0.0; }, [](double) { return 0.0; }, [](float, int) {}, &total, &zp);
+        }
+        if (tid == 0) write_row(op, row, pick, 0.0, none ? 0 : 1);
         if (probs)
             for (int i = tid; i < A; i += NT) probs[i] = i == pick ? 1.f : 0.f;
         return;
     }
     const Scale sc = make_scale(zmax, rp.T);
-    Row<T, NT> R{op, sh, view, sc, row, lane, wave, v0, v1};
+    Row<T, NT> R{sh, view, sc, lane, wave, v0, v1};
     const int k = rp.k > 0 && rp.k < count ? rp.k : 0;
-    const float zcut = min_p_border(rp.m, rp.T, sc);
-    Border b{-INFINITY, 0x7fffffff};
-    bool done = false, small = false;
+    const float zcut = min_p_border(rp.m, rp.T, sc, lane);
+    Border b{-FLT_MAX, 0x7fffffff};
+    bool small = false;
     int ln = 0;
     double mass = -1.0;
     // short cuts: a lower bound of all that can be kept, from top-k or min-p, that leaves few candidates
-    if ((k && k <= kFastK) || (rp.m > 0 && rp.p >= 1)) {
+    const bool by_k = k && k <= kFastK;
+    if (by_k || (rp.m > 0 && rp.p >= 1)) {
         if (wave == 0) {
             uint32_t t = 0;
-            if (k && k <= kFastK) {   // the k-th largest partial maximum: at least k entries are not below it
+            if (by_k) {   // the k-th largest partial maximum: at least k entries are not below it
                 uint32_t g[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) g[e] = sh.group[e * W + lane];
@@ -949,23 +932,19 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         ln = R.gather(zl, INFINITY, b);
         small = ln <= kList;
     }
-    if (!small && k) {
+#pragma unroll 1
+    for (int step = 0; step < 2; step++) {   // top-k, then top-p within it
+        if (small || (step == 0 ? !k : rp.p >= 1)) continue;
         bool s2 = false;
         double mm;
-        b = R.select(k, 0.0, b, &s2, &ln, &mm);
+        const Border nb = R.select(step == 0 ? k : -1, rp.p, b, &s2, &ln, &mm);
         small = s2;
-    }
-    if (!small && rp.p < 1) {
-        bool s2 = false;
-        const Border nb = R.select(-1, rp.p, b, &s2, &ln, &mass);
-        if (s2) small = true;
-        else b = nb;
+        b = nb;
+        if (step) mass = mm;
     }
     if (small) {
         RowParams q = rp;
-        q.k = k;
-        // a list from top-p's histogram was cut by top-k before: its border is in it, its mass is `mass`
-        if (mass >= 0) q.k = 0;
+        q.k = mass >= 0 ? 0 : k;   // a list from top-p's histogram has been cut by top-k before; its whole mass is `mass`
         if (wave == 0) {
             if (ln <= W) finish_list<NT, 1>(op, row, sh, ln, q, sc, mass, lane);
             else finish_list<NT, kList / W>(op, row, sh, ln, q, sc, mass, lane);
@@ -974,20 +953,15 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         if (probs) {
             b.z0 = z_of_rank(sh.out_r);
             b.i0 = index_of_rank(sh.out_r);
-            total = sh.out_d[0];
+            total = sh.out_d;
         }
-        done = true;
-    }
-    if (!done) {
+    } else {
         int kn = 0;
         const Border bb = b;
-        const int pick = locate<T, NT>(
-            view, sh, [=](float z, int i) { return z >= zcut && inside(z, i, bb) ? weight(z, sc) : 0.0; }, [&](double t) { return rp.u * t; }, &total, &zp);
-        // how many are kept
-        R.pass([&](const Vec<T>& x, int i0) {
-#pragma unroll
-            for (int i = 0; i < N; i++) kn += x.z[i] >= zcut && inside(x.z[i], i0 + i, bb);
-        });
+        float zp;
+        const int pick = locate<NT>(
+            view, sh, [=](float z, int i) { return z >= zcut && inside(z, i, bb) ? weight(z, sc) : 0.0; }, [&](double t) { return rp.u * t; },
+            [&](float z, int i) { kn += z >= zcut && inside(z, i, bb); }, &total, &zp);
         kn = wave_sum(kn);
         if (lane == 0) sh.wi[wave] = kn;
         __syncthreads();
@@ -998,14 +972,11 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
             write_row(op, row, pick, x / rp.T - log(total), n);
         }
     }
-    if (probs) {
-        const Border bb = b;
-        R.pass([&](const Vec<T>& x, int i0) {
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (i0 + i >= 0 && i0 + i < A) probs[i0 + i] = x.z[i] >= zcut && inside(x.z[i], i0 + i, bb) ? (float)(weight(x.z[i], sc) / total) : 0.f;
-        });
-    }
+    if (probs)
+        for (int i = tid; i < A; i += NT) {
+            const float z = clean(to_float(view.src[i]), !view.legal || view.legal[i]);
+            probs[i] = z >= zcut && inside(z, i, b) ? (float)(weight(z, sc) / total) : 0.f;
+        }
 }
 
 template <typename T>

@@ -1,10 +1,13 @@
 """The library's operators on torch tensors (mz_sample_actions, mz_adapter_linear of include/muzero_hip.h): checks of types, shapes and
 devices, then one call of the C ABI on torch's current stream of the tensors' device.  Nothing is copied, converted or
 synchronised; a call can be captured into a torch.cuda.graph.  Errors are capi.MuZeroError."""
+from ctypes import byref
+
 import torch
 
 from . import capi
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the same number without a Stream object around it
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MZ_DTYPE_*
 
 
@@ -14,15 +17,18 @@ def _need(ok, text):
 
 
 def _tensor(t, name, dtype, shape, device, dense=True):
-    """t as a tensor of that dtype, shape and device whose rows are contiguous (dense: entirely)."""
+    """Address of t, a tensor of that dtype, shape and device whose rows are contiguous (dense: all of it)."""
+    try:   # one test for the usual case; which one failed is found out below
+        if t.dtype is dtype and t.shape == shape and t.device == device and (t.is_contiguous() or not dense and t.stride(-1) == 1):
+            return t.data_ptr()
+    except AttributeError:
+        pass
     _need(isinstance(t, torch.Tensor), f"{name}: a torch tensor is needed")
     _need(t.dtype == dtype, f"{name}: {t.dtype}, needs {dtype}")
     _need(tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, needs {tuple(shape)}")
     _need(t.device == device, f"{name}: on {t.device}, the other operands on {device}")
-    if dense:
-        _need(t.is_contiguous(), f"{name}: must be contiguous")
-    else:
-        _need(t.dim() < 1 or t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must be contiguous")
+    _need(not dense, f"{name}: must be contiguous")
+    _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must be contiguous")
     return t.data_ptr()
 
 
@@ -30,9 +36,20 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _finish(rc):
-    if rc != 0:
-        raise capi.MuZeroError(capi.lib().mz_last_error(None).decode())
+def _stream(device):
+    """torch's current stream of the device, as a hipStream_t."""
+    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+
+
+def _fail():
+    raise capi.MuZeroError(capi.lib().mz_last_error(None).decode())
+
+
+def _setting(v, name, dtype, shape, device):
+    """A number, or a tensor with one per row: (scalar, address)."""
+    if isinstance(v, torch.Tensor):
+        return 0, _tensor(v, name, dtype, shape, device)
+    return v, None
 
 
 def _workspace(need, given, device):
@@ -55,55 +72,47 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
 
     Returns dict(action int32 [B], logprob float32 [B], kept int32 [B], and with probs=True probs float32 [B, A]).  `out`: such
     a dict of tensors to write into instead (action required, the others as wanted)."""
-    _need(isinstance(logits, torch.Tensor) and logits.dim() == 2, "logits: a 2-d torch tensor is needed")
-    _need(logits.is_cuda, "logits: must be on a GPU")
-    _need(logits.dtype in DTYPES, f"logits: {logits.dtype} is not supported")
-    B, A = logits.shape
-    dev = logits.device
-    a = capi.SampleArgs()
-    a.rows, a.actions, a.dtype = B, A, DTYPES[logits.dtype]
-    a.logits = _tensor(logits, "logits", logits.dtype, (B, A), dev, dense=False)
-    a.row_stride = _row_stride(logits)
+    if not (isinstance(logits, torch.Tensor) and logits.dim() == 2):
+        raise capi.MuZeroError("logits: a 2-d torch tensor is needed")
+    t, dev = logits.dtype, logits.device
+    if not logits.is_cuda or t not in DTYPES:
+        raise capi.MuZeroError(f"logits: must be on a GPU and float32, bfloat16 or float16, not {t} on {dev}")
+    shape = logits.shape
+    B, A = shape
+    rows = (B,)
+    p_legal, s_legal = None, 0
     if legal is not None:
-        _need(isinstance(legal, torch.Tensor) and legal.dtype in (torch.uint8, torch.bool), "legal: uint8 or bool is needed")
-        a.legal = _tensor(legal, "legal", legal.dtype, (B, A), dev, dense=False)
-        a.legal_stride = _row_stride(legal)
-    a.u = _tensor(u, "u", torch.float64, (B,), dev)
-    if isinstance(temperature, torch.Tensor):
-        a.row_temperature = _tensor(temperature, "temperature", torch.float64, (B,), dev)
-    else:
-        a.temperature = temperature
-    if isinstance(top_k, torch.Tensor):
-        a.row_top_k = _tensor(top_k, "top_k", torch.int32, (B,), dev)
-    else:
-        _need(0 <= top_k, "top_k must be >= 0")
-        a.top_k = min(int(top_k), 2**31 - 1)
-    if isinstance(top_p, torch.Tensor):
-        a.row_top_p = _tensor(top_p, "top_p", torch.float64, (B,), dev)
-    else:
-        a.top_p = top_p
-    if isinstance(min_p, torch.Tensor):
-        a.row_min_p = _tensor(min_p, "min_p", torch.float64, (B,), dev)
-    else:
-        a.min_p = min_p
+        lt = getattr(legal, "dtype", None)
+        if lt is not torch.uint8 and lt is not torch.bool:
+            raise capi.MuZeroError("legal: a uint8 or bool tensor is needed")
+        p_legal, s_legal = _tensor(legal, "legal", lt, shape, dev, dense=False), _row_stride(legal)
+    temperature, p_t = _setting(temperature, "temperature", torch.float64, rows, dev)
+    top_k, p_k = _setting(top_k, "top_k", torch.int32, rows, dev)
+    top_p, p_p = _setting(top_p, "top_p", torch.float64, rows, dev)
+    min_p, p_m = _setting(min_p, "min_p", torch.float64, rows, dev)
+    if top_k >= 2**31:
+        top_k = 2**31 - 1
     if out is None:
         out = dict(action=torch.empty(B, dtype=torch.int32, device=dev), logprob=torch.empty(B, device=dev),
                    kept=torch.empty(B, dtype=torch.int32, device=dev))
         if probs:
             out["probs"] = torch.empty(B, A, device=dev)
-    _need("action" in out, "out: 'action' is needed")
-    a.action = _tensor(out["action"], "out['action']", torch.int32, (B,), dev)
-    if out.get("logprob") is not None:
-        a.logprob = _tensor(out["logprob"], "out['logprob']", torch.float32, (B,), dev)
-    if out.get("kept") is not None:
-        a.kept = _tensor(out["kept"], "out['kept']", torch.int32, (B,), dev)
-    if out.get("probs") is not None:
-        a.probs = _tensor(out["probs"], "out['probs']", torch.float32, (B, A), dev, dense=False)
-        a.probs_stride = _row_stride(out["probs"])
+    get = out.get
+    action, logprob, kept, pr = get("action"), get("logprob"), get("kept"), get("probs")
+    args = capi.SampleArgs(
+        B, A, DTYPES[t], top_k, temperature, top_p, min_p,
+        _tensor(logits, "logits", t, shape, dev, dense=False), _row_stride(logits), p_legal, s_legal,
+        _tensor(u, "u", torch.float64, rows, dev), p_t, p_k, p_p, p_m,
+        _tensor(action, "out['action']", torch.int32, rows, dev),
+        None if logprob is None else _tensor(logprob, "out['logprob']", torch.float32, rows, dev),
+        None if kept is None else _tensor(kept, "out['kept']", torch.int32, rows, dev),
+        None if pr is None else _tensor(pr, "out['probs']", torch.float32, shape, dev, dense=False),
+        0 if pr is None else _row_stride(pr))
     L = capi.lib()
-    ref = capi.C.byref(a)
+    ref = byref(args)
     keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(ref), workspace, dev)
-    _finish(L.mz_sample_actions(ref, ws, nbytes, torch.cuda.current_stream(dev).cuda_stream))
+    if L.mz_sample_actions(ref, ws, nbytes, _stream(dev)) != 0:
+        _fail()
     return out
 
 
@@ -111,37 +120,35 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
     """x [M, K] @ weight [N, K]^T + bias [N], plus each row's own adapter i = index[m] (int32 [M], -1 = none):
     scale[i] * (x[m] @ a[i]^T) @ b[i]^T with a [n, r, K], b [n, N, r] and scale float32 [n] (None: 1).  All of one type (float32,
     bfloat16, float16); the result [M, N] has it too, or float32 with out_dtype=torch.float32 (mz_adapter_linear)."""
-    _need(isinstance(x, torch.Tensor) and x.dim() == 2, "x: a 2-d torch tensor is needed")
-    _need(x.is_cuda, "x: must be on a GPU")
+    for v, name, dims in ((x, "x", 2), (weight, "weight", 2), (a, "a", 3)):
+        if not (isinstance(v, torch.Tensor) and v.dim() == dims):
+            raise capi.MuZeroError(f"{name}: a {dims}-d torch tensor is needed")
     t, dev = x.dtype, x.device
-    _need(t in DTYPES, f"x: {t} is not supported")
+    if not x.is_cuda or t not in DTYPES:
+        raise capi.MuZeroError(f"x: must be on a GPU and float32, bfloat16 or float16, not {t} on {dev}")
     M, K = x.shape
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight: a 2-d torch tensor is needed")
-    _need(isinstance(a, torch.Tensor) and a.dim() == 3, "a: a 3-d torch tensor is needed")
-    N, (n, r, _) = weight.shape[0], a.shape
-    if out_dtype is None:
-        out_dtype = t if out is None else out.dtype
-    _need(out_dtype in DTYPES, f"out_dtype: {out_dtype} is not supported")
+    n, r, _ = a.shape
+    N = weight.shape[0]
     if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=dev)
-    g = capi.AdapterArgs()
-    g.rows, g.in_features, g.out_features, g.rank, g.adapters = M, K, N, r, n
-    g.dtype, g.out_dtype = DTYPES[t], DTYPES[out_dtype]
-    g.x = _tensor(x, "x", t, (M, K), dev, dense=False)
-    g.x_stride = _row_stride(x)
-    g.weight = _tensor(weight, "weight", t, (N, K), dev, dense=False)
-    g.weight_stride = _row_stride(weight)
-    if bias is not None:
-        g.bias = _tensor(bias, "bias", t, (N,), dev)
-    g.a = _tensor(a, "a", t, (n, r, K), dev)
-    g.b = _tensor(b, "b", t, (n, N, r), dev)
-    if scale is not None:
-        g.scale = _tensor(scale, "scale", torch.float32, (n,), dev)
-    g.index = _tensor(index, "index", torch.int32, (M,), dev)
-    g.y = _tensor(out, "out", out_dtype, (M, N), dev, dense=False)
-    g.y_stride = _row_stride(out)
+        out = torch.empty(M, N, dtype=t if out_dtype is None else out_dtype, device=dev)
+    elif out_dtype is None:
+        out_dtype = getattr(out, "dtype", None)
+    if out_dtype is None:
+        out_dtype = t
+    if out_dtype not in DTYPES:
+        raise capi.MuZeroError(f"out: {out_dtype} is not supported")
+    args = capi.AdapterArgs(
+        M, K, N, r, n, DTYPES[t], DTYPES[out_dtype], 0,
+        _tensor(x, "x", t, (M, K), dev, dense=False), _row_stride(x),
+        _tensor(weight, "weight", t, (N, K), dev, dense=False), _row_stride(weight),
+        None if bias is None else _tensor(bias, "bias", t, (N,), dev),
+        _tensor(a, "a", t, (n, r, K), dev), _tensor(b, "b", t, (n, N, r), dev),
+        None if scale is None else _tensor(scale, "scale", torch.float32, (n,), dev),
+        _tensor(index, "index", torch.int32, (M,), dev), _tensor(out, "out", out_dtype, (M, N), dev, dense=False),
+        _row_stride(out))
     L = capi.lib()
-    ref = capi.C.byref(g)
+    ref = byref(args)
     keep, ws, nbytes = _workspace(L.mz_adapter_workspace_bytes(ref), workspace, dev)
-    _finish(L.mz_adapter_linear(ref, ws, nbytes, torch.cuda.current_stream(dev).cuda_stream))
+    if L.mz_adapter_linear(ref, ws, nbytes, _stream(dev)) != 0:
+        _fail()
     return out
