@@ -50,24 +50,72 @@ __device__ __forceinline__ double exp2_frac(double f) {
     q = fma(q, f, 0x1.62e42fefa39f7p-1);
     return fma(q, f, 1.0);
 }
-// The row's scale: x / ln 2 = (z - zmax) * c.
+// The row's scale: x / ln 2 = (z - zmax) * c.  A maximum of +inf stands as 2^128 with a c that leaves no weight to finite
+// entries; T = 5e-324 would make c infinite, and 0 * inf is not wanted.
 struct Scale {
     double zmax, c;
 };
 __device__ __forceinline__ Scale make_scale(float zmax, double T) {
+    const bool inf = zmax == INFINITY;
     Scale s;
-    s.zmax = (double)zmax;
-    s.c = fmin(1.4426950408889634 / T, 1e290);   // T = 5e-324: 0 * inf is not wanted
+    s.zmax = inf ? 0x1p128 : (double)zmax;
+    s.c = inf ? 1e290 : fmin(1.4426950408889634 / T, 1e290);
     return s;
 }
-// (z - zmax) / (T ln 2) in [-2000, 0]; z = zmax = +inf counts as 0
-__device__ __forceinline__ double log2_weight(float z, const Scale& s) {
-    const double d = (double)z == s.zmax ? 0.0 : (double)z - s.zmax;
-    return fmax(d * s.c, -2000.0);
+// y = (z - zmax) / (T ln 2) in [low, 0]
+__device__ __forceinline__ double log2_weight(float z, const Scale& s, double low) { return fmax(fmin(((double)z - s.zmax) * s.c, 0.0), low); }
+// log of the share of an entry: x - log(total)
+__device__ __forceinline__ double log_share(float z, float zmax, double T, double total) {
+    return (z == zmax ? 0.0 : ((double)z - (double)zmax) / T) - log(total);
 }
-__device__ __forceinline__ double weight(float z, const Scale& s) {   // 0 for z = -inf
-    const double y = log2_weight(z, s), n = rint(y);
-    return ldexp(exp2_frac(y - n), (int)n);
+// Integers and 64-bit floats meet in the low word of 1.5 * 2^52 + n: an addition rounds to the nearest integer and shows it
+// there; conversions, rounding and ldexp instructions run at a quarter of the rate of an addition.
+constexpr double kRound = 6755399441055744.0;
+__device__ __forceinline__ int low_word(double v) { return (int)(uint32_t)__double_as_longlong(v); }
+__device__ __forceinline__ double scaled(double p, int n) {   // p 2^n, p and the result normal numbers
+    const u64 b = (u64)__double_as_longlong(p);
+    return __longlong_as_double((long long)((u64)((uint32_t)(b >> 32) + ((uint32_t)n << 20)) << 32 | (uint32_t)b));
+}
+constexpr double kNoWeight = -1023.0;                          // and below: scaled(1.0, -1023) is 0, the weight of -inf too
+__device__ __forceinline__ double weight(float z, const Scale& s) {
+    const double y = log2_weight(z, s, kNoWeight), t = y + kRound;
+    return scaled(exp2_frac(y - (t - kRound)), low_word(t));
+}
+
+// The same for N entries side by side, for the passes over long rows: the constants of the polynomial stay in scalar registers
+// (compiled from exp2_frac each step is a move and a two-operand FMA).  The results must not go into DPP operations directly:
+// the compiler does not see that a vector instruction wrote them.
+__device__ __forceinline__ double fma_scalar(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+template <int N>
+__device__ __forceinline__ void exp2_fracs(const double (&f)[N], double (&p)[N]) {
+    constexpr double k[10] = {0x1.e5e9f548e5726p-28, 0x1.b6571de2f2351p-24, 0x1.62bfe46117445p-20, 0x1.ffcb76789860fp-17, 0x1.4309130378460p-13,
+                              0x1.5d87fe908f88ap-10, 0x1.3b2ab6fba385fp-7,  0x1.c6b08d7044119p-5,  0x1.ebfbdff82c590p-3,  0x1.62e42fefa39f7p-1};
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = k[0];
+#pragma unroll
+    for (int j = 1; j < 10; j++)
+#pragma unroll
+        for (int i = 0; i < N; i++) p[i] = fma_scalar(p[i], f[i], k[j]);
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = fma(p[i], f[i], 1.0);
+}
+template <int N>
+__device__ __forceinline__ void weights(const float (&z)[N], const Scale& s, double (&w)[N]) {
+    double f[N];
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const double y = log2_weight(z[i], s, kNoWeight), t = y + kRound;
+        n[i] = low_word(t);
+        f[i] = y - (t - kRound);
+    }
+    exp2_fracs(f, w);
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = scaled(w[i], n[i]);
 }
 
 // ---- order-preserving keys ---------------------------------------------------------------------------------------------
@@ -79,70 +127,110 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^
 constexpr uint32_t kNoKey = 0x007fffffu;   // key of -inf: an entry that takes no part
 // ranking as an unsigned 64-bit order: larger z first, then smaller index; 0 = no entry
 __device__ __forceinline__ u64 rank_of(float z, int i) { return z > -INFINITY ? ((u64)key_of(z) << 32) | (uint32_t)~i : 0ull; }
-__device__ __forceinline__ float z_of_rank(u64 r) { return r ? of_key((uint32_t)(r >> 32)) : -INFINITY; }
+__device__ __forceinline__ float z_of_rank(u64 r) { return of_key((uint32_t)(r >> 32)); }
 __device__ __forceinline__ int index_of_rank(u64 r) { return (int)~(uint32_t)r; }
 
 // ---- wave primitives -----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// Lanes exchange through DPP (inside rows of 16) and row / half swaps, which need neither LDS nor its latency.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_rows(uint32_t v) {   // 0 in the rows that are not written
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-template <typename V>
-__device__ __forceinline__ V wave_scan(V v, int lane) {   // inclusive
-#pragma unroll
-    for (int o = 1; o < W; o <<= 1) {
-        const V t = __shfl_up(v, o);
-        v += lane >= o ? t : V(0);
+template <int J>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t v, int lane) {
+    if constexpr (J == 1) return dpp<0xB1>(v);                 // quad_perm [1, 0, 3, 2]
+    else if constexpr (J == 2) return dpp<0x4E>(v);            // quad_perm [2, 3, 0, 1]
+    else if constexpr (J == 4) return dpp<0x141>(dpp<0x1B>(v));   // reversed quads, then reversed halves of 8
+    else if constexpr (J == 8) return dpp<0x128>(v);           // rotate a row by 8
+    else if constexpr (J == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);   // rows 0, 0, 2, 2 and 1, 1, 3, 3
+        return lane & 16 ? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);   // lower halves, upper halves
+        return lane & 32 ? r[0] : r[1];
     }
+}
+template <int J>
+__device__ __forceinline__ u64 xor_lane(u64 v, int lane) {
+    return (u64)xor_lane<J>((uint32_t)(v >> 32), lane) << 32 | xor_lane<J>((uint32_t)v, lane);
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ u64 lane_value(u64 v, int l) { return (u64)lane_value((uint32_t)(v >> 32), l) << 32 | lane_value((uint32_t)v, l); }
+__device__ __forceinline__ double lane_value(double v, int l) { return __longlong_as_double((long long)lane_value((u64)__double_as_longlong(v), l)); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(double& v) {
+    const u64 b = (u64)__double_as_longlong(v);
+    v += __longlong_as_double((long long)((u64)dpp_rows<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp_rows<CTRL, ROWS>((uint32_t)b)));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(int& v) { v += (int)dpp_rows<CTRL, ROWS>((uint32_t)v); }
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {   // inclusive
+    scan_step<0x111, 0xf>(v);                   // row_shr 1, 2, 4, 8
+    scan_step<0x112, 0xf>(v);
+    scan_step<0x114, 0xf>(v);
+    scan_step<0x118, 0xf>(v);
+    scan_step<0x142, 0xa>(v);                   // the end of rows 0 and 2 to rows 1 and 3
+    scan_step<0x143, 0xc>(v);                   // the end of row 1 to rows 2 and 3
     return v;
 }
-// descending bitonic sort of 64 E values, position e * 64 + lane
-template <int E>
-__device__ __forceinline__ void wave_sort(u64 (&r)[E], int lane) {
+__device__ __forceinline__ double one_lane_up(double v) {   // 0 into lane 0
+    const u64 b = (u64)__double_as_longlong(v);
+    return __longlong_as_double((long long)((u64)dpp_rows<0x138, 0xf>((uint32_t)(b >> 32)) << 32 | dpp_rows<0x138, 0xf>((uint32_t)b)));   // wave_shr 1
+}
+__device__ __forceinline__ double wave_sum(double v) { return lane_value(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_sum(int v) { return (int)lane_value((uint32_t)wave_scan(v), 63); }
+__device__ __forceinline__ float wave_max(float v, int lane) {
+    uint32_t k = key_of(v);
+    k = max(k, xor_lane<1>(k, lane));
+    k = max(k, xor_lane<2>(k, lane));
+    k = max(k, xor_lane<4>(k, lane));
+    k = max(k, xor_lane<8>(k, lane));
+    k = max(k, xor_lane<16>(k, lane));
+    k = max(k, xor_lane<32>(k, lane));
+    return of_key((uint32_t)uniform((int)k));
+}
+template <int E, int K, int J, typename V>
+__device__ __forceinline__ void sort_step(V (&r)[E], int lane) {
+    if constexpr (J >= W) {
+        constexpr int S = J / W;
 #pragma unroll
-    for (int k = 2; k <= W * E; k <<= 1) {
-#pragma unroll
-        for (int j = k >> 1; j; j >>= 1) {
-            if (j >= W) {
-                const int s = j / W;
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (!(e & s)) {
-                        const bool desc = ((e * W) & k) == 0;   // k > 64: the bit does not depend on the lane
-                        const u64 a = r[e], b = r[e | s];
-                        const bool sw = desc ? a < b : a > b;
-                        r[e] = sw ? b : a;
-                        r[e | s] = sw ? a : b;
-                    }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const u64 o = __shfl_xor(r[e], j);
-                    const bool desc = ((e * W + lane) & k) == 0, lower = (lane & j) == 0;
-                    const bool big = desc == lower;   // this position keeps the larger of the pair
-                    r[e] = (r[e] > o) == big ? r[e] : o;
-                }
+        for (int e = 0; e < E; e++)
+            if (!(e & S)) {
+                const bool desc = ((e * W) & K) == 0;   // K > 64: the bit does not depend on the lane
+                const V a = max(r[e], r[e | S]), b = min(r[e], r[e | S]);
+                r[e] = desc ? a : b;
+                r[e | S] = desc ? b : a;
             }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const V o = xor_lane<J>(r[e], lane);
+            const bool big = (((e * W + lane) & K) == 0) == ((lane & J) == 0);   // this position keeps the larger of the pair
+            r[e] = big ? max(r[e], o) : min(r[e], o);
         }
     }
+    if constexpr (J > 1) sort_step<E, K, J / 2>(r, lane);
 }
-template <int E>
-__device__ __forceinline__ u64 at_position(const u64 (&r)[E], int p) {
-    u64 v = 0;
+// descending bitonic sort of 64 E values, position e * 64 + lane
+template <int E, typename V, int K = 2>
+__device__ __forceinline__ void wave_sort(V (&r)[E], int lane) {
+    sort_step<E, K, K / 2>(r, lane);
+    if constexpr (K < W * E) wave_sort<E, V, K * 2>(r, lane);
+}
+template <int E, typename V>
+__device__ __forceinline__ V at_position(const V (&r)[E], int p) {   // p uniform
+    p = uniform(p);
+    V v = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const u64 t = __shfl(r[e], p & 63);
+        const V t = lane_value(r[e], p & 63);
         v = (p >> 6) == e ? t : v;
     }
     return v;
@@ -171,10 +259,12 @@ __device__ __forceinline__ void write_row(const SampleOp& op, int row, int actio
     if (op.kept) op.kept[row] = kept;
 }
 
-// Entries ranked[] (descending, position e * 64 + lane, `count` of them real): the length of the prefix that the filters keep.
-// `mass` < 0: top-p goes by the mass of the first k here; else by `mass`.
-template <int E>
-__device__ __forceinline__ int kept_prefix(const u64 (&ranked)[E], int count, const RowParams& rp, const Scale& sc, double mass, int lane) {
+__device__ __forceinline__ float z_of(uint32_t key) { return of_key(key); }
+__device__ __forceinline__ float z_of(u64 rank) { return of_key((uint32_t)(rank >> 32)); }
+// Entries ranked[] (keys or rank values, descending, position e * 64 + lane, `count` of them real): the length of the prefix
+// that the filters keep.  `mass` < 0: top-p goes by the mass of the first k here; else by `mass`.
+template <int E, typename V>
+__device__ __forceinline__ int kept_prefix(const V (&ranked)[E], int count, const RowParams& rp, const Scale& sc, double mass, int lane) {
     int n = rp.k > 0 ? min(rp.k, count) : count;
     if (rp.p < 1 || rp.m > 0) {
         double before[E], carry = 0;
@@ -182,11 +272,10 @@ __device__ __forceinline__ int kept_prefix(const u64 (&ranked)[E], int count, co
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const bool in = e * W + lane < n;
-            const double w = in ? weight(z_of_rank(ranked[e]), sc) : 0.0;
-            const double s = wave_scan(w, lane);
-            const double prev = __shfl_up(s, 1);
-            before[e] = carry + (lane ? prev : 0.0);
-            carry += __shfl(s, 63);
+            const double w = in ? weight(z_of(ranked[e]), sc) : 0.0;
+            const double s = wave_scan(w);
+            before[e] = carry + one_lane_up(s);
+            carry += lane_value(s, 63);
             nm += __popcll(__ballot(in && w >= rp.m));
         }
         if (rp.p < 1) {
@@ -203,13 +292,13 @@ __device__ __forceinline__ int kept_prefix(const u64 (&ranked)[E], int count, co
 
 // The draw over weights in index order, position e * 64 + lane: position of the drawn entry, and the sum of the weights.
 template <int E>
-__device__ __forceinline__ int wave_draw(const double (&w)[E], double u, int lane, double* total) {
+__device__ __forceinline__ int wave_draw(const double (&w)[E], double u, double* total) {
     double cum[E], carry = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const double s = wave_scan(w[e], lane);
+        const double s = wave_scan(w[e]);
         cum[e] = carry + s;
-        carry += __shfl(s, 63);
+        carry += lane_value(s, 63);
     }
     *total = carry;
     const double target = u * carry;
@@ -257,7 +346,7 @@ __global__ __launch_bounds__(W * kWaveRows) void k_sample_wave(SampleOp op) {
         count += __popcll(__ballot(z[e] > -INFINITY));
     }
     const RowParams rp = row_params(op, row);
-    zmax = wave_max(zmax);
+    zmax = wave_max(zmax, lane);
     float* probs = op.probs ? op.probs + row * op.probs_stride : nullptr;
     if (!rp.valid || count == 0) {
         if (lane == 0) write_row(op, row, -1, 0.0, 0);
@@ -279,46 +368,46 @@ __global__ __launch_bounds__(W * kWaveRows) void k_sample_wave(SampleOp op) {
     }
     const Scale sc = make_scale(zmax, rp.T);
     int n = count;
-    u64 border = 1;   // the last kept entry of the ranking
-    if ((rp.k > 0 && rp.k < count) || rp.p < 1) {
-        u64 r[E];
+    uint32_t border = 0;     // kept: keys above it, and the first `ties` equal to it
+    int ties = 64 * E;
+    uint32_t key[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) r[e] = rank_of(z[e], e * W + lane);
+    for (int e = 0; e < E; e++) key[e] = z[e] > -INFINITY ? key_of(z[e]) : 0u;
+    const bool cut = (rp.k > 0 && rp.k < count) || rp.p < 1;
+    if (cut) {
+        uint32_t r[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) r[e] = key[e];
         wave_sort<E>(r, lane);
         n = kept_prefix<E>(r, count, rp, sc, -1.0, lane);
         border = at_position<E>(r, n - 1);
-    } else if (rp.m > 0) {
-        n = 0;
+        ties = n;
+#pragma unroll
+        for (int e = 0; e < E; e++) ties -= __popcll(__ballot(r[e] > border));
     }
     double w[E];
+    int before = 0, kept = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
         w[e] = weight(z[e], sc);
-        bool keep = rank_of(z[e], e * W + lane) >= border;
-        if (border == 1 && rp.m > 0) {
-            keep = keep && w[e] >= rp.m;
-            n += __popcll(__ballot(keep));
-        }
-        if (!keep) w[e] = 0.0;
+        const u64 eq = __ballot(key[e] == border);
+        const int nth = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(eq >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)eq, 0));
+        before += __popcll(eq);
+        const bool keep = key[e] != 0 && (key[e] > border || (key[e] == border && nth < ties)) && (cut || w[e] >= rp.m);
+        kept += __popcll(__ballot(keep));
+        w[e] = keep ? w[e] : 0.0;
     }
     double total;
-    const int pick = wave_draw<E>(w, rp.u, lane, &total);
-    if (op.logprob || lane == 0) {
-        float zp = z[0];
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const float t = __shfl(z[e], pick & 63);
-            zp = (pick >> 6) == e ? t : zp;
-        }
-        if (lane == 0) {
-            const double d = (double)zp == sc.zmax ? 0.0 : (double)zp - sc.zmax;
-            write_row(op, row, pick, d / rp.T - log(total), n);
-        }
+    const int pick = wave_draw<E>(w, rp.u, &total);
+    const float zp = of_key(at_position<E>(key, pick));
+    if (lane == 0) {
+        write_row(op, row, pick, log_share(zp, zmax, rp.T, total), kept);
     }
     if (probs) {
+        const double share = 1.0 / total;
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (e * W + lane < A) probs[e * W + lane] = (float)(w[e] / total);
+            if (e * W + lane < A) probs[e * W + lane] = (float)(w[e] * share);
     }
 }
 
@@ -335,33 +424,44 @@ struct RowView {
     const uint8_t* legal;
     int A, nvec;            // A >= Vec<T>::N; vector v = the entries [v N, v N + N), the last one moved back to end with the row
 };
-// Vector v: 16 bytes wherever they start.  Entries without a part in the draw - masked, NaN, -inf, and in the last vector those
-// that the vector before has - are -inf; a vector behind the last (v >= end) is all that.  CLEAN = false leaves NaN and -0 in.
+template <typename T>
+struct Raw {
+    u32x4 d;
+    uint32_t legal[Vec<T>::N / 4];
+};
+// Vector v: 16 bytes wherever they start, and their legal flags
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const RowView<T>& r, int v) {
+    constexpr int N = Vec<T>::N;
+    const int i0 = min(v * N, r.A - N);
+    Raw<T> o;
+    __builtin_memcpy(&o.d, r.src + i0, 16);
+    if (r.legal) __builtin_memcpy(o.legal, r.legal + i0, N);
+    return o;
+}
+// Entries without a part in the draw - masked, NaN, -inf, and in the last vector those that the vector before has - become -inf;
+// a vector behind the last (v >= end) is all that.  CLEAN = false leaves NaN and -0 in.
 template <bool CLEAN, typename T>
-__device__ __forceinline__ Vec<T> load_vec(const RowView<T>& r, int v, int end) {
+__device__ __forceinline__ Vec<T> unpack(const RowView<T>& r, const Raw<T>& raw, int v, int end) {
     constexpr int N = Vec<T>::N;
     Vec<T> o;
     const int want = v * N;
     o.i0 = min(want, r.A - N);
-    u32x4 d;
-    __builtin_memcpy(&d, r.src + o.i0, 16);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) o.z[i] = __uint_as_float(d[i]);
+        for (int i = 0; i < 4; i++) o.z[i] = __uint_as_float(raw.d[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint16_t h = (uint16_t)(d[i >> 1] >> (16 * (i & 1)));
+            const uint16_t h = (uint16_t)(raw.d[i >> 1] >> (16 * (i & 1)));
             T t;
             __builtin_memcpy(&t, &h, 2);
             o.z[i] = to_float(t);
         }
     }
     if (r.legal) {
-        uint32_t l[N / 4];
-        __builtin_memcpy(l, r.legal + o.i0, N);
 #pragma unroll
-        for (int i = 0; i < N; i++) o.z[i] = (l[i >> 2] >> (8 * (i & 3)) & 255u) ? o.z[i] : -INFINITY;
+        for (int i = 0; i < N; i++) o.z[i] = (raw.legal[i >> 2] >> (8 * (i & 3)) & 255u) ? o.z[i] : -INFINITY;
     }
     if (v >= end || want != o.i0) {
         const int skip = v >= end ? N : want - o.i0;
@@ -378,11 +478,14 @@ __device__ __forceinline__ Vec<T> load_vec(const RowView<T>& r, int v, int end) 
 // f(vector) over this wave's vectors [v0, v1): lanes take consecutive vectors, all lanes take part in every call
 template <bool CLEAN = true, typename T, typename F>
 __device__ __forceinline__ void wave_pass(const RowView<T>& r, int v0, int v1, int lane, F f) {
+    if (v0 >= v1) return;
+    Raw<T> n0 = load_raw(r, v0 + lane), n1 = load_raw(r, v0 + W + lane);   // two loads ahead (behind the last vector: the last again)
 #pragma unroll 1
-    for (int v = v0; v < v1; v += 2 * W) {
-        const Vec<T> a = load_vec<CLEAN>(r, v + lane, v1), b = load_vec<CLEAN>(r, v + W + lane, v1);
-        f(a);
-        f(b);
+    for (int v = v0; v < v1; v += W) {
+        const Raw<T> c = n0;
+        n0 = n1;
+        n1 = load_raw(r, v + 2 * W + lane);
+        f(unpack<CLEAN>(r, c, v + lane, v1));
     }
 }
 
@@ -406,9 +509,9 @@ struct Shared {
     u64 out_r;
 };
 
-// First entry in index order at which the running sum of wf(z, index) exceeds target(total); the last entry with a weight if
-// none does.  Sums in a fixed order: vector, lane, wave segments, then the segment of the border again in 1/NW pieces.
-// Every thread returns the index; *total and the entry's z likewise.  `seen` is called once for every entry.
+// First entry in index order at which the running sum of the weights exceeds target(total); the last entry with a weight if
+// none does.  wf(vector, w) gives the weights of a vector's entries.  Sums in a fixed order: vector, lane, wave segments, then the segment of the border again in 1/NW pieces.
+// Every thread returns the index; *total and the entry's z likewise.  `seen` is called once for every vector.
 template <int NT, typename T, typename WF, typename TF, typename SF>
 __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf, TF target_of, SF seen, double* total, float* z_out) {
     constexpr int NW = NT / W, N = Vec<T>::N;
@@ -421,12 +524,11 @@ __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf
         const int v0 = min(hi, lo + wave * per), v1 = min(hi, v0 + per);
         double s = 0;
         wave_pass(r, v0, v1, lane, [&](const Vec<T>& x) {
+            double w[N];
+            wf(x, w);
 #pragma unroll
-            for (int i = 0; i < N; i++) s += wf(x.z[i], x.i0 + i);
-            if (level == 0) {
-#pragma unroll
-                for (int i = 0; i < N; i++) seen(x.z[i], x.i0 + i);
-            }
+            for (int i = 0; i < N; i++) s += w[i];
+            if (level == 0) seen(x);
         });
         s = wave_sum(s);
         __syncthreads();
@@ -467,24 +569,23 @@ __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf
         float fz = 0, lz = 0;
 #pragma unroll 1
         for (int v = lo; v < hi && found < 0; v += W) {
-            const Vec<T> x = load_vec<true>(r, v + lane, hi);
-            double s = 0;
+            const Vec<T> x = unpack<true>(r, load_raw(r, v + lane), v + lane, hi);
+            double w[N], s = 0;
+            wf(x, w);
 #pragma unroll
-            for (int i = 0; i < N; i++) s += wf(x.z[i], x.i0 + i);
-            const double inc = wave_scan(s, lane);
-            const double prev = __shfl_up(inc, 1);
+            for (int i = 0; i < N; i++) s += w[i];
+            const double inc = wave_scan(s), prev = one_lane_up(inc);
             const u64 some = __ballot(s > 0), over = __ballot(s > 0 && base + inc > target);
             if (some) {
                 const int who = over ? __ffsll(over) - 1 : 63 - __clzll(some);
                 int mi = -1, ml = -1;
                 float mz = 0, mlz = 0;
                 if (lane == who) {
-                    double c = base + (lane ? prev : 0.0);
+                    double c = base + prev;
 #pragma unroll
                     for (int i = 0; i < N; i++) {
-                        const double w = wf(x.z[i], x.i0 + i);
-                        c += w;
-                        if (w > 0) {
+                        c += w[i];
+                        if (w[i] > 0) {
                             ml = x.i0 + i;
                             mlz = x.z[i];
                             if (mi < 0 && c > target) {
@@ -505,7 +606,7 @@ __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf
                     fz = __shfl(mz, who);
                 }
             }
-            base += __shfl(inc, 63);
+            base += lane_value(inc, 63);
         }
         if (lane == 0) {
             sh.out_i = found < 0 ? last : found;
@@ -521,7 +622,7 @@ __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf
 
 // The list (unordered, n <= 64 E) finished by one wave: prefix, draw, output.  All entries of the row that can be kept are in it.
 template <int NT, int E>
-__device__ __forceinline__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, const RowParams& rp, const Scale& sc, double mass, int lane) {
+__device__ __forceinline__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, const RowParams& rp, const Scale& sc, float zmax, double mass, int lane) {
     u64 r[E];
 #pragma unroll
     for (int e = 0; e < E; e++) r[e] = e * W + lane < n ? sh.list[e * W + lane] : 0ull;
@@ -537,13 +638,12 @@ __device__ __forceinline__ void finish_list(const SampleOp& op, int row, Shared<
 #pragma unroll
     for (int e = 0; e < E; e++) w[e] = o[e] ? weight(of_key((uint32_t)o[e]), sc) : 0.0;
     double total;
-    const int pos = wave_draw<E>(w, rp.u, lane, &total);
+    const int pos = wave_draw<E>(w, rp.u, &total);
     const u64 d = at_position<E>(o, pos);
     const int pick = (int)~(uint32_t)(d >> 32);
     const float zp = of_key((uint32_t)d);
     if (lane == 0) {
-        const double x = (double)zp == sc.zmax ? 0.0 : (double)zp - sc.zmax;
-        write_row(op, row, pick, x / rp.T - log(total), keep);
+        write_row(op, row, pick, log_share(zp, zmax, rp.T, total), keep);
         sh.out_r = border;
         sh.out_d = total;
     }
@@ -562,24 +662,26 @@ __device__ __forceinline__ u64 border_of_list(Shared<NT>& sh, int n, int want, d
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const bool in = e * W + lane < n;
-            const double s = wave_scan(in ? weight(z_of_rank(r[e]), sc) : 0.0, lane);
-            const double prev = __shfl_up(s, 1);
-            keep += __popcll(__ballot(in && carry + (lane ? prev : 0.0) < target));
-            carry += __shfl(s, 63);
+            const double s = wave_scan(in ? weight(z_of(r[e]), sc) : 0.0);
+            keep += __popcll(__ballot(in && carry + one_lane_up(s) < target));
+            carry += lane_value(s, 63);
         }
         keep = max(keep, 1);
     }
     return at_position<E>(r, keep - 1);
 }
 
-// log2-spaced bin of an entry, 32 to a factor of two below the maximum, the last one open; its weight is 2^(-(bin >> 5)) times
-// 2^f, f in [-0.5, 0.5], returned beside it
-constexpr double kDeep = -63.4375;                     // bin 2046
+// log2-spaced bin of an entry, 32 to a factor of two below the maximum, the last one open (entries below 2^-63 of the maximum,
+// whose mass is left out); its weight is 2^-bin_power(bin) times
+// 2^f, |f| < 0.52, returned beside it
+constexpr int kOpen = kBins - 1;
+__device__ __forceinline__ int bin_power(int b) { return (b + 16) >> 5; }
 __device__ __forceinline__ int bin_of(float z, const Scale& s, double* f) {
-    const double y = log2_weight(z, s);
-    const int b = (int)((0.5 - fmax(y, kDeep)) * 32.0);
-    *f = y + (double)(b >> 5);
-    return y < kDeep ? kBins - 1 : b;
+    const double y = log2_weight(z, s, -(double)kOpen / 32.0);
+    const int b = -low_word(fma(y, 32.0, kRound));
+    // kRound + power, its low word being the power
+    *f = y + (__longlong_as_double(__double_as_longlong(kRound) + bin_power(b)) - kRound);
+    return b;
 }
 // Smallest key in [lo, hi] that `is` holds for; it holds for hi and, monotone, for every key above one it holds for.  64 keys a
 // step, the first ones around `guess`.
@@ -610,7 +712,7 @@ struct Border {       // kept: z > z0 or (z == z0 and index <= i0); z0 > -inf
     float z0;
     int i0;
 };
-__device__ __forceinline__ bool inside(float z, int i, const Border& b) { return z > b.z0 || (z == b.z0 && i <= b.i0); }
+__device__ __forceinline__ bool inside(float z, int i, const Border& b) { return (z > b.z0) | ((z == b.z0) & (i <= b.i0)); }
 
 // p in [0.7, 1.42] as an integer of kFix fraction bits on top of the bits of 128.0 (2^(52 - 45) = 128)
 __device__ __forceinline__ u64 fixed_bits(double p) { return (u64)__double_as_longlong(p + 128.0); }
@@ -667,8 +769,8 @@ struct Row {
     }
     // Scans the histogram: picks the last non-empty bin whose predecessors count < want (want >= 0) or hold mass < frac * total
     // (want < 0; *total receives the whole mass when `fresh`); counts and masses start at the given offsets.  A bin's masses
-    // are in units of 2^(e0 - (bin >> shift)), and zero from bin `open` on.
-    __device__ __forceinline__ int pick_bin(int want, double frac, bool fresh, double* total, int cnt0, double mass0, int e0, int shift, int open, int* above_cnt,
+    // are in units of 2^-power (power < 0: of 2^-bin_power(bin)), and zero from bin `open` on.
+    __device__ __forceinline__ int pick_bin(int want, double frac, bool fresh, double* total, int cnt0, double mass0, int power, int open, int* above_cnt,
                                             double* above_mass, int* bin_cnt) {
         constexpr int PER = kBins / NT;
         uint32_t c[PER];
@@ -679,12 +781,12 @@ struct Row {
         for (int i = 0; i < PER; i++) {
             const int b = threadIdx.x * PER + i;
             c[i] = sh.cnt[b];
-            m[i] = want < 0 && c[i] && b < open ? of_fixed(sh.mass[b], c[i], e0 - (b >> shift)) : 0.0;
+            m[i] = want < 0 && c[i] && b < open ? of_fixed(sh.mass[b], c[i], -(power < 0 ? bin_power(b) : power)) : 0.0;
             ct += (int)c[i];
             mt += m[i];
         }
-        const int ci = wave_scan(ct, lane);
-        const double mi = wave_scan(mt, lane);
+        const int ci = wave_scan(ct);
+        const double mi = wave_scan(mt);
         if (lane == 63) {
             sh.wi[wave] = ci;
             sh.wd[wave] = mi;
@@ -701,9 +803,8 @@ struct Row {
         }
         if (fresh) *total = all;
         const double target = want < 0 ? frac * *total : 0.0;
-        const double mprev = __shfl_up(mi, 1);
         cb += ci - ct;
-        mb += lane ? mprev : 0.0;
+        mb += one_lane_up(mi);
         int mine = -1, mcb = 0;
         double mmb = 0;
 #pragma unroll
@@ -736,7 +837,7 @@ struct Row {
     // *small: set when everything down to the border's bin is a list of <= 256 entries: sh.list holds it, *mass the whole mass.
     __device__ __forceinline__ Border select(int want, double frac, const Border b0, bool* small, int* list_n, double* mass) {
         const bool wm = want < 0;
-        int above = 0, cnt = 0, shift = 0, n_bin = 0;
+        int above = 0, cnt = 0, shift = 0, power = 0;
         double above_mass = 0;
         uint32_t klo = kNoKey + 1, khi = key_of((float)sc.zmax);
         bool open = false;
@@ -746,27 +847,49 @@ struct Row {
             clear_hist(wm);
             const float zl = of_key(klo), zh = of_key(khi);
             const uint32_t kh = khi;
-            wave_pass(view, v0, v1, lane, [&](const Vec<T>& x) {
+            if (level == 0) {
+                wave_pass(view, v0, v1, lane, [&](const Vec<T>& x) {
+                    int b[N];
+                    double f[N];
+                    bool in[N];
 #pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const float z = x.z[i];
-                    if (z >= zl && z <= zh && inside(z, x.i0 + i, b0)) {
-                        double f;
-                        int b = bin_of(z, sc, &f);
-                        const bool heavy = wm && b < kBins - 1;      // the open bin: below 2^-63 of the maximum each, no mass
-                        if (level) b = (int)((kh - key_of(z)) >> shift);
-                        atomicAdd(&sh.cnt[b], 1u);
-                        if (heavy) atomicAdd(&sh.mass[b], fixed_bits(exp2_frac(f)));
+                    for (int i = 0; i < N; i++) {
+                        b[i] = bin_of(x.z[i], sc, &f[i]);
+                        in[i] = inside(x.z[i], x.i0 + i, b0);
                     }
-                }
-            });
+                    if (wm) {
+                        double p[N];
+                        exp2_fracs(f, p);
+#pragma unroll
+                        for (int i = 0; i < N; i++)
+                            if (in[i]) atomicAdd(&sh.mass[b[i]], fixed_bits(p[i]));   // of the open bin: not used
+                    }
+#pragma unroll
+                    for (int i = 0; i < N; i++)
+                        if (in[i]) atomicAdd(&sh.cnt[b[i]], 1u);
+                });
+            } else {
+                wave_pass(view, v0, v1, lane, [&](const Vec<T>& x) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const float z = x.z[i];
+                        if (z >= zl && z <= zh && inside(z, x.i0 + i, b0)) {   // few
+                            double f;
+                            bin_of(z, sc, &f);
+                            const int b = (int)((kh - key_of(z)) >> shift);
+                            atomicAdd(&sh.cnt[b], 1u);
+                            if (wm) atomicAdd(&sh.mass[b], fixed_bits(exp2_frac(f)));
+                        }
+                    }
+                });
+            }
             __syncthreads();
             if (level == 0) {
-                const int bin = pick_bin(want, frac, true, mass, 0, 0.0, 0, 5, kBins - 1, &above, &above_mass, &cnt);
-                n_bin = bin >> 5;
-                open = bin == kBins - 1;
+                const int bin = pick_bin(want, frac, true, mass, 0, 0.0, -1, kOpen, &above, &above_mass, &cnt);
+                power = bin_power(bin);
+                open = bin == kOpen;
                 // the bin's range of keys
-                const double zb = sc.zmax + (0.5 - bin / 32.0) / sc.c, za = sc.zmax + (0.5 - (bin + 1) / 32.0) / sc.c;
+                const double zb = sc.zmax - (bin - 0.5) / 32.0 / sc.c, za = sc.zmax - (bin + 0.5) / 32.0 / sc.c;
                 const Scale s = sc;
                 const uint32_t top = khi;
                 if (!open) klo = first_key(klo, top, (float)za, lane, [=](float z) { double f; return bin_of(z, s, &f) <= bin; });
@@ -779,7 +902,7 @@ struct Row {
             } else {
                 const int a0 = above;
                 const double m0 = above_mass;
-                const int rb = pick_bin(want, frac, false, mass, a0, m0, -n_bin, 30, open ? 0 : kBins, &above, &above_mass, &cnt);
+                const int rb = pick_bin(want, frac, false, mass, a0, m0, power, open ? 0 : kBins, &above, &above_mass, &cnt);
                 khi = khi - ((uint32_t)rb << shift);
                 const uint32_t width = (1u << shift) - 1;
                 klo = khi - klo > width ? khi - width : klo;
@@ -821,8 +944,11 @@ struct Row {
             double tot;
             float zz;
             const Border bb = b0;
-            b.i0 = locate<NT>(view, sh, [=](float z, int i) { return z == zv && inside(z, i, bb) ? 1.0 : 0.0; }, [=](double) { return (double)ties - 1.0; },
-                              [](float, int) {}, &tot, &zz);
+            b.i0 = locate<NT>(view, sh, [=](const Vec<T>& x, double (&w)[N]) {
+#pragma unroll
+                for (int i = 0; i < N; i++) w[i] = x.z[i] == zv && inside(x.z[i], x.i0 + i, bb) ? 1.0 : 0.0;
+            }, [=](double) { return (double)ties - 1.0; },
+                              [](const Vec<T>&) {}, &tot, &zz);
         }
         return b;
     }
@@ -831,7 +957,7 @@ struct Row {
 // Smallest float whose weight is at least m: min-p as a border (the weights are monotone in z)
 __device__ __forceinline__ float min_p_border(double m, double T, const Scale& sc, int lane) {
     if (!(m > 0)) return -FLT_MAX;
-    if (sc.zmax == (double)INFINITY) return INFINITY;
+    if (sc.zmax == 0x1p128) return INFINITY;
     const float guess = (float)fmax(sc.zmax + T * log(m), -(double)FLT_MAX);
     return of_key(first_key(kNoKey + 1, key_of((float)sc.zmax), guess, lane, [=](float z) { return weight(z, sc) >= m; }));
 }
@@ -864,19 +990,17 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
     });
     {
         tmax += 0.0f;
-        const float m = wave_max(tmax);
+        const float m = wave_max(tmax, lane);
         const int c = wave_sum(tcnt);
         if (lane == 0) {
             sh.wf[wave] = m;
             sh.wi[wave] = c;
         }
         // 256 partial maxima
-        float g = tmax;
-        if (NT == 1024) {
-            g = fmaxf(g, __shfl_xor(g, 1));
-            g = fmaxf(g, __shfl_xor(g, 2));
-        }
-        if (tid % (NT / 256) == 0) sh.group[tid / (NT / 256)] = key_of(g);
+        uint32_t g = key_of(tmax);
+        if (NT >= 512) g = max(g, xor_lane<1>(g, lane));
+        if (NT == 1024) g = max(g, xor_lane<2>(g, lane));
+        if (tid % (NT / 256) == 0) sh.group[tid / (NT / 256)] = g;
     }
     __syncthreads();
     float zmax = -INFINITY;
@@ -892,7 +1016,10 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         int pick = -1;
         if (!none) {
             float zp;
-            pick = locate<NT>(view, sh, [=](float z, int) { return z == zmax ? 1.0 : 0.0; }, [](double) { return 0.0; }, [](float, int) {}, &total, &zp);
+            pick = locate<NT>(view, sh, [=](const Vec<T>& x, double (&w)[N]) {
+#pragma unroll
+                for (int i = 0; i < N; i++) w[i] = x.z[i] == zmax ? 1.0 : 0.0;
+            }, [](double) { return 0.0; }, [](const Vec<T>&) {}, &total, &zp);
         }
         if (tid == 0) write_row(op, row, pick, 0.0, none ? 0 : 1);
         if (probs)
@@ -946,8 +1073,8 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         RowParams q = rp;
         q.k = mass >= 0 ? 0 : k;   // a list from top-p's histogram has been cut by top-k before; its whole mass is `mass`
         if (wave == 0) {
-            if (ln <= W) finish_list<NT, 1>(op, row, sh, ln, q, sc, mass, lane);
-            else finish_list<NT, kList / W>(op, row, sh, ln, q, sc, mass, lane);
+            if (ln <= W) finish_list<NT, 1>(op, row, sh, ln, q, sc, zmax, mass, lane);
+            else finish_list<NT, kList / W>(op, row, sh, ln, q, sc, zmax, mass, lane);
         }
         __syncthreads();
         if (probs) {
@@ -957,25 +1084,30 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
         }
     } else {
         int kn = 0;
+        if (zcut > b.z0) b = Border{zcut, 0x7fffffff};
         const Border bb = b;
         float zp;
-        const int pick = locate<NT>(
-            view, sh, [=](float z, int i) { return z >= zcut && inside(z, i, bb) ? weight(z, sc) : 0.0; }, [&](double t) { return rp.u * t; },
-            [&](float z, int i) { kn += z >= zcut && inside(z, i, bb); }, &total, &zp);
+        const int pick = locate<NT>(view, sh, [=](const Vec<T>& x, double (&w)[N]) {
+            weights(x.z, sc, w);
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = inside(x.z[i], x.i0 + i, bb) ? w[i] : 0.0;
+        }, [&](double t) { return rp.u * t; }, [&](const Vec<T>& x) {
+#pragma unroll
+            for (int i = 0; i < N; i++) kn += inside(x.z[i], x.i0 + i, bb);
+        }, &total, &zp);
         kn = wave_sum(kn);
         if (lane == 0) sh.wi[wave] = kn;
         __syncthreads();
         if (tid == 0) {
             int n = 0;
             for (int i = 0; i < NW; i++) n += sh.wi[i];
-            const double x = (double)zp == sc.zmax ? 0.0 : (double)zp - sc.zmax;
-            write_row(op, row, pick, x / rp.T - log(total), n);
+            write_row(op, row, pick, log_share(zp, zmax, rp.T, total), n);
         }
     }
     if (probs)
         for (int i = tid; i < A; i += NT) {
             const float z = clean(to_float(view.src[i]), !view.legal || view.legal[i]);
-            probs[i] = z >= zcut && inside(z, i, b) ? (float)(weight(z, sc) / total) : 0.f;
+            probs[i] = inside(z, i, b) ? (float)(weight(z, sc) / total) : 0.f;
         }
 }
 
