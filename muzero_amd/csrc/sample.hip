@@ -126,8 +126,7 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((int)k < 0 ? 0x80000000u : 0xffffffffu)); }
 constexpr uint32_t kNoKey = 0x007fffffu;   // key of -inf: an entry that takes no part
 // ranking as an unsigned 64-bit order: larger z first, then smaller index; 0 = no entry
-__device__ __forceinline__ u64 rank_of(float z, int i) { return z > -INFINITY ? ((u64)key_of(z) << 32) | (uint32_t)~i : 0ull; }
-__device__ __forceinline__ float z_of_rank(u64 r) { return of_key((uint32_t)(r >> 32)); }
+__device__ __forceinline__ u64 rank_of(float z, int i) { return z > -INFINITY ? ((u64)key_of(z + 0.0f) << 32) | (uint32_t)~i : 0ull; }
 __device__ __forceinline__ int index_of_rank(u64 r) { return (int)~(uint32_t)r; }
 
 // ---- wave primitives -----------------------------------------------------------------------------------------------------
@@ -439,9 +438,9 @@ __device__ __forceinline__ Raw<T> load_raw(const RowView<T>& r, int v) {
     if (r.legal) __builtin_memcpy(o.legal, r.legal + i0, N);
     return o;
 }
-// Entries without a part in the draw - masked, NaN, -inf, and in the last vector those that the vector before has - become -inf;
-// a vector behind the last (v >= end) is all that.  CLEAN = false leaves NaN and -0 in.
-template <bool CLEAN, typename T>
+// Masked entries, and in the last vector those that the vector before has, become -inf; a vector behind the last (v >= end) is
+// all that.  NaN and -0 are left in: every use compares (NaN is above and equal to nothing), and rank_of takes -0 for 0.
+template <typename T>
 __device__ __forceinline__ Vec<T> unpack(const RowView<T>& r, const Raw<T>& raw, int v, int end) {
     constexpr int N = Vec<T>::N;
     Vec<T> o;
@@ -469,14 +468,10 @@ __device__ __forceinline__ Vec<T> unpack(const RowView<T>& r, const Raw<T>& raw,
         for (int i = 0; i < N; i++)
             if (i < skip) o.z[i] = -INFINITY;
     }
-    if constexpr (CLEAN) {
-#pragma unroll
-        for (int i = 0; i < N; i++) o.z[i] = fmaxf(o.z[i], -INFINITY) + 0.0f;   // NaN -> -inf, -0 -> +0
-    }
     return o;
 }
 // f(vector) over this wave's vectors [v0, v1): lanes take consecutive vectors, all lanes take part in every call
-template <bool CLEAN = true, typename T, typename F>
+template <typename T, typename F>
 __device__ __forceinline__ void wave_pass(const RowView<T>& r, int v0, int v1, int lane, F f) {
     if (v0 >= v1) return;
     Raw<T> n0 = load_raw(r, v0 + lane), n1 = load_raw(r, v0 + W + lane);   // two loads ahead (behind the last vector: the last again)
@@ -485,7 +480,7 @@ __device__ __forceinline__ void wave_pass(const RowView<T>& r, int v0, int v1, i
         const Raw<T> c = n0;
         n0 = n1;
         n1 = load_raw(r, v + 2 * W + lane);
-        f(unpack<CLEAN>(r, c, v + lane, v1));
+        f(unpack(r, c, v + lane, v1));
     }
 }
 
@@ -569,7 +564,7 @@ __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf
         float fz = 0, lz = 0;
 #pragma unroll 1
         for (int v = lo; v < hi && found < 0; v += W) {
-            const Vec<T> x = unpack<true>(r, load_raw(r, v + lane), v + lane, hi);
+            const Vec<T> x = unpack(r, load_raw(r, v + lane), v + lane, hi);
             double w[N], s = 0;
             wf(x, w);
 #pragma unroll
@@ -620,6 +615,24 @@ __device__ __forceinline__ int locate(const RowView<T>& r, Shared<NT>& sh, WF wf
     return res;
 }
 
+// The first `keep` of ranked[], again in index order, and the draw among them.
+template <int NT, int E>
+__device__ __forceinline__ void draw_ranked(const SampleOp& op, int row, Shared<NT>& sh, const u64 (&ranked)[E], int keep, const RowParams& rp, const Scale& sc, float zmax, int lane) {
+    u64 o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = e * W + lane < keep ? (ranked[e] << 32) | (ranked[e] >> 32) : 0ull;   // ~index first: descending = index ascending
+    wave_sort<E>(o, lane);
+    double w[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) w[e] = o[e] ? weight(of_key((uint32_t)o[e]), sc) : 0.0;
+    double total;
+    const int pos = wave_draw<E>(w, rp.u, &total);
+    const u64 d = at_position<E>(o, pos);
+    if (lane == 0) {
+        write_row(op, row, (int)~(uint32_t)(d >> 32), log_share(of_key((uint32_t)d), zmax, rp.T, total), keep);
+        sh.out_d = total;
+    }
+}
 // The list (unordered, n <= 64 E) finished by one wave: prefix, draw, output.  All entries of the row that can be kept are in it.
 template <int NT, int E>
 __device__ __forceinline__ void finish_list(const SampleOp& op, int row, Shared<NT>& sh, int n, const RowParams& rp, const Scale& sc, float zmax, double mass, int lane) {
@@ -629,23 +642,12 @@ __device__ __forceinline__ void finish_list(const SampleOp& op, int row, Shared<
     wave_sort<E>(r, lane);
     const int keep = kept_prefix<E>(r, n, rp, sc, mass, lane);
     const u64 border = at_position<E>(r, keep - 1);
-    // the kept ones again, in index order
-    u64 o[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = e * W + lane < keep ? (r[e] << 32) | (r[e] >> 32) : 0ull;   // ~index first: descending = index ascending
-    wave_sort<E>(o, lane);
-    double w[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) w[e] = o[e] ? weight(of_key((uint32_t)o[e]), sc) : 0.0;
-    double total;
-    const int pos = wave_draw<E>(w, rp.u, &total);
-    const u64 d = at_position<E>(o, pos);
-    const int pick = (int)~(uint32_t)(d >> 32);
-    const float zp = of_key((uint32_t)d);
-    if (lane == 0) {
-        write_row(op, row, pick, log_share(zp, zmax, rp.T, total), keep);
-        sh.out_r = border;
-        sh.out_d = total;
+    if (lane == 0) sh.out_r = border;
+    if (E > 1 && keep <= W) {
+        const u64 first[1] = {r[0]};
+        draw_ranked<NT, 1>(op, row, sh, first, keep, rp, sc, zmax, lane);
+    } else {
+        draw_ranked<NT, E>(op, row, sh, r, keep, rp, sc, zmax, lane);
     }
 }
 // The border inside a crossing bin whose entries are listed: its rank value.
@@ -876,7 +878,7 @@ struct Row {
                         if (z >= zl && z <= zh && inside(z, x.i0 + i, b0)) {   // few
                             double f;
                             bin_of(z, sc, &f);
-                            const int b = (int)((kh - key_of(z)) >> shift);
+                            const int b = (int)((kh - key_of(z + 0.0f)) >> shift);
                             atomicAdd(&sh.cnt[b], 1u);
                             if (wm) atomicAdd(&sh.mass[b], fixed_bits(exp2_frac(f)));
                         }
@@ -919,7 +921,7 @@ struct Row {
                 if (lane == 0) sh.out_r = border;
             }
             __syncthreads();
-            b.z0 = z_of_rank(sh.out_r);
+            b.z0 = z_of(sh.out_r);
             b.i0 = index_of_rank(sh.out_r);
             __syncthreads();
             return b;
@@ -962,157 +964,295 @@ __device__ __forceinline__ float min_p_border(double m, double T, const Scale& s
     return of_key(first_key(kNoKey + 1, key_of((float)sc.zmax), guess, lane, [=](float z) { return weight(z, sc) >= m; }));
 }
 
+// The k-th largest (k <= 128) of the 256 partial maxima in sh.group, as a key: at least k entries are not below it.  One wave.
+template <int NT>
+__device__ __forceinline__ uint32_t kth_partial(const Shared<NT>& sh, int k, int lane) {
+    uint32_t g[4], t = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) g[e] = sh.group[e * W + lane];
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t c = t | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) n += __popcll(__ballot(g[e] >= c));
+        if (n >= k) t = c;
+    }
+    return t;
+}
+// maximum, number of entries and 2^LOG partial maxima (keys, to group[]) of this workgroup's vectors [a, b)
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
+__device__ __forceinline__ void partial_maxima(const RowView<T>& view, int a, int b, Shared<NT>& sh, uint32_t* group, int log_groups, float* zmax, int* count) {
     constexpr int NW = NT / W, N = Vec<T>::N;
-    __shared__ Shared<NT> sh;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int A = op.actions;
-    RowView<T> view;
-    view.src = static_cast<const T*>(op.logits) + row * op.row_stride;
-    view.legal = op.legal ? op.legal + row * op.legal_stride : nullptr;
-    view.A = A;
-    view.nvec = (A + N - 1) / N;
-    const int per = ((view.nvec + NW - 1) / NW + W - 1) / W * W;
-    const int v0 = min(view.nvec, wave * per), v1 = min(view.nvec, v0 + per);
-    const RowParams rp = row_params(op, row);
-    float* probs = op.probs ? op.probs + row * op.probs_stride : nullptr;
-
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int per = ((b - a + NW - 1) / NW + W - 1) / W * W, v0 = min(b, a + wave * per), v1 = min(b, v0 + per);
     float tmax = -INFINITY;
     int tcnt = 0;
-    wave_pass<false>(view, v0, v1, lane, [&](const Vec<T>& x) {
+    wave_pass(view, v0, v1, lane, [&](const Vec<T>& x) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             tmax = fmaxf(tmax, x.z[i]);
             tcnt += x.z[i] > -INFINITY;
         }
     });
-    {
-        tmax += 0.0f;
-        const float m = wave_max(tmax, lane);
-        const int c = wave_sum(tcnt);
-        if (lane == 0) {
-            sh.wf[wave] = m;
-            sh.wi[wave] = c;
-        }
-        // 256 partial maxima
-        uint32_t g = key_of(tmax);
-        if (NT >= 512) g = max(g, xor_lane<1>(g, lane));
-        if (NT == 1024) g = max(g, xor_lane<2>(g, lane));
-        if (tid % (NT / 256) == 0) sh.group[tid / (NT / 256)] = g;
+    tmax += 0.0f;
+    const float m = wave_max(tmax, lane);
+    const int c = wave_sum(tcnt);
+    if (lane == 0) {
+        sh.wf[wave] = m;
+        sh.wi[wave] = c;
     }
+    uint32_t g = key_of(tmax);
+    const int lanes = NT >> log_groups;   // 1 .. 64 neighbouring threads share a group
+    if (lanes > 1) g = max(g, xor_lane<1>(g, lane));
+    if (lanes > 2) g = max(g, xor_lane<2>(g, lane));
+    if (lanes > 4) g = max(g, xor_lane<4>(g, lane));
+    if (lanes > 8) g = max(g, xor_lane<8>(g, lane));
+    if (lanes > 16) g = max(g, xor_lane<16>(g, lane));
+    if (lanes > 32) g = max(g, xor_lane<32>(g, lane));
+    if (tid % lanes == 0) group[tid / lanes] = g;
     __syncthreads();
-    float zmax = -INFINITY;
-    int count = 0;
+    *zmax = -INFINITY;
+    *count = 0;
     for (int i = 0; i < NW; i++) {
-        zmax = fmaxf(zmax, sh.wf[i]);
-        count += sh.wi[i];
+        *zmax = fmaxf(*zmax, sh.wf[i]);
+        *count += sh.wi[i];
     }
     __syncthreads();
-    const bool none = !rp.valid || count == 0;
-    double total = 1.0;
-    if (none || rp.T == 0) {
-        int pick = -1;
-        if (!none) {
-            float zp;
-            pick = locate<NT>(view, sh, [=](const Vec<T>& x, double (&w)[N]) {
-#pragma unroll
-                for (int i = 0; i < N; i++) w[i] = x.z[i] == zmax ? 1.0 : 0.0;
-            }, [](double) { return 0.0; }, [](const Vec<T>&) {}, &total, &zp);
-        }
-        if (tid == 0) write_row(op, row, pick, 0.0, none ? 0 : 1);
-        if (probs)
-            for (int i = tid; i < A; i += NT) probs[i] = i == pick ? 1.f : 0.f;
-        return;
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ RowView<T> view_of(const SampleOp& op, int row) {
+    RowView<T> v;
+    v.src = static_cast<const T*>(op.logits) + row * op.row_stride;
+    v.legal = op.legal ? op.legal + row * op.legal_stride : nullptr;
+    v.A = op.actions;
+    v.nvec = (op.actions + Vec<T>::N - 1) / Vec<T>::N;
+    return v;
+}
+// A row without an entry, or with parameters out of range
+template <int NT>
+__device__ __forceinline__ void write_none(const SampleOp& op, int row) {
+    if (threadIdx.x == 0) write_row(op, row, -1, 0.0, 0);
+    if (op.probs)
+        for (int i = threadIdx.x; i < op.actions; i += NT) op.probs[row * op.probs_stride + i] = 0.f;
+}
+template <typename T, int NT>
+__device__ __forceinline__ void write_probs(const SampleOp& op, int row, const RowView<T>& view, const Scale& sc, const Border& b, double total) {
+    const double share = 1.0 / total;
+    for (int i = threadIdx.x; i < op.actions; i += NT) {
+        const float z = clean(to_float(view.src[i]), !view.legal || view.legal[i]);
+        op.probs[row * op.probs_stride + i] = inside(z, i, b) ? (float)(weight(z, sc) * share) : 0.f;
+    }
+}
+// The row's answer from sh.list, its ln <= 256 candidates (see finish_list for `mass`)
+template <typename T, int NT>
+__device__ __forceinline__ void answer_from_list(const SampleOp& op, int row, Shared<NT>& sh, const RowView<T>& view, int ln, const RowParams& rp, const Scale& sc, float zmax,
+                                                 double mass) {
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < W) {
+        if (ln <= W) finish_list<NT, 1>(op, row, sh, ln, rp, sc, zmax, mass, lane);
+        else if (ln <= 2 * W) finish_list<NT, 2>(op, row, sh, ln, rp, sc, zmax, mass, lane);
+        else finish_list<NT, kList / W>(op, row, sh, ln, rp, sc, zmax, mass, lane);
+    }
+    __syncthreads();
+    if (op.probs) write_probs<T, NT>(op, row, view, sc, Border{z_of(sh.out_r), index_of_rank(sh.out_r)}, sh.out_d);
+}
+// Short cuts: a lower bound of all that can be kept, from top-k or min-p, that mostly leaves few candidates
+__device__ __forceinline__ bool short_cut(const RowParams& rp, int k) { return (k && k <= kFastK) || (rp.m > 0 && rp.p >= 1); }
+template <int NT>
+__device__ __forceinline__ float short_cut_bound(Shared<NT>& sh, const RowParams& rp, int k, const Scale& sc) {
+    if (threadIdx.x < W) {
+        const uint32_t t = k && k <= kFastK ? kth_partial(sh, k, threadIdx.x) : 0;
+        if (threadIdx.x == 0) sh.bound = t;
+    }
+    __syncthreads();
+    const float zl = sh.bound > kNoKey ? of_key(sh.bound) : -FLT_MAX;
+    // (top-p needs the mass of all of the first k)
+    return rp.p >= 1 && !k ? fmaxf(zl, min_p_border(rp.m, rp.T, sc, threadIdx.x & 63)) : zl;
+}
+
+// A row whose maximum, number of entries and partial maxima are known, by a workgroup.  tried: the short cut left too many.
+template <typename T, int NT>
+__device__ __forceinline__ void answer_row(const SampleOp& op, int row, Shared<NT>& sh, const RowView<T>& view, RowParams rp, float zmax, int count, bool tried) {
+    constexpr int NW = NT / W, N = Vec<T>::N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    if (rp.T == 0) {   // the first of the ranking
+        rp.T = 1;
+        rp.k = 1;
+        rp.p = 1;
+        rp.m = 0;
     }
     const Scale sc = make_scale(zmax, rp.T);
+    const int per = ((view.nvec + NW - 1) / NW + W - 1) / W * W;
+    const int v0 = min(view.nvec, wave * per), v1 = min(view.nvec, v0 + per);
     Row<T, NT> R{sh, view, sc, lane, wave, v0, v1};
-    const int k = rp.k > 0 && rp.k < count ? rp.k : 0;
-    const float zcut = min_p_border(rp.m, rp.T, sc, lane);
+    rp.k = rp.k > 0 && rp.k < count ? rp.k : 0;
     Border b{-FLT_MAX, 0x7fffffff};
     bool small = false;
     int ln = 0;
     double mass = -1.0;
-    // short cuts: a lower bound of all that can be kept, from top-k or min-p, that leaves few candidates
-    const bool by_k = k && k <= kFastK;
-    if (by_k || (rp.m > 0 && rp.p >= 1)) {
-        if (wave == 0) {
-            uint32_t t = 0;
-            if (by_k) {   // the k-th largest partial maximum: at least k entries are not below it
-                uint32_t g[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) g[e] = sh.group[e * W + lane];
-                for (int bit = 31; bit >= 0; bit--) {
-                    const uint32_t c = t | (1u << bit);
-                    int n = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) n += __popcll(__ballot(g[e] >= c));
-                    if (n >= k) t = c;
-                }
-            }
-            if (lane == 0) sh.bound = t;
-        }
-        __syncthreads();
-        float zl = sh.bound > kNoKey ? of_key(sh.bound) : -FLT_MAX;
-        if (rp.p >= 1) zl = fmaxf(zl, zcut);   // top-p needs the mass of all of the first k
-        ln = R.gather(zl, INFINITY, b);
+    if (!tried && short_cut(rp, rp.k)) {
+        ln = R.gather(short_cut_bound(sh, rp, rp.k, sc), INFINITY, b);
         small = ln <= kList;
     }
 #pragma unroll 1
     for (int step = 0; step < 2; step++) {   // top-k, then top-p within it
-        if (small || (step == 0 ? !k : rp.p >= 1)) continue;
+        if (small || (step == 0 ? !rp.k : rp.p >= 1)) continue;
         bool s2 = false;
         double mm;
-        const Border nb = R.select(step == 0 ? k : -1, rp.p, b, &s2, &ln, &mm);
+        const Border nb = R.select(step == 0 ? rp.k : -1, rp.p, b, &s2, &ln, &mm);
         small = s2;
         b = nb;
         if (step) mass = mm;
     }
     if (small) {
-        RowParams q = rp;
-        q.k = mass >= 0 ? 0 : k;   // a list from top-p's histogram has been cut by top-k before; its whole mass is `mass`
-        if (wave == 0) {
-            if (ln <= W) finish_list<NT, 1>(op, row, sh, ln, q, sc, zmax, mass, lane);
-            else finish_list<NT, kList / W>(op, row, sh, ln, q, sc, zmax, mass, lane);
-        }
-        __syncthreads();
-        if (probs) {
-            b.z0 = z_of_rank(sh.out_r);
-            b.i0 = index_of_rank(sh.out_r);
-            total = sh.out_d;
-        }
-    } else {
-        int kn = 0;
-        if (zcut > b.z0) b = Border{zcut, 0x7fffffff};
-        const Border bb = b;
-        float zp;
-        const int pick = locate<NT>(view, sh, [=](const Vec<T>& x, double (&w)[N]) {
-            weights(x.z, sc, w);
-#pragma unroll
-            for (int i = 0; i < N; i++) w[i] = inside(x.z[i], x.i0 + i, bb) ? w[i] : 0.0;
-        }, [&](double t) { return rp.u * t; }, [&](const Vec<T>& x) {
-#pragma unroll
-            for (int i = 0; i < N; i++) kn += inside(x.z[i], x.i0 + i, bb);
-        }, &total, &zp);
-        kn = wave_sum(kn);
-        if (lane == 0) sh.wi[wave] = kn;
-        __syncthreads();
-        if (tid == 0) {
-            int n = 0;
-            for (int i = 0; i < NW; i++) n += sh.wi[i];
-            write_row(op, row, pick, log_share(zp, zmax, rp.T, total), n);
-        }
+        if (mass >= 0) rp.k = 0;   // a list from top-p's histogram has been cut by top-k before; its whole mass is `mass`
+        answer_from_list<T, NT>(op, row, sh, view, ln, rp, sc, zmax, mass);
+        return;
     }
-    if (probs)
-        for (int i = tid; i < A; i += NT) {
-            const float z = clean(to_float(view.src[i]), !view.legal || view.legal[i]);
-            probs[i] = inside(z, i, b) ? (float)(weight(z, sc) / total) : 0.f;
+    int kn = 0;
+    const float zcut = min_p_border(rp.m, rp.T, sc, lane);
+    if (zcut > b.z0) b = Border{zcut, 0x7fffffff};
+    const Border bb = b;
+    float zp;
+    double total;
+    const int pick = locate<NT>(view, sh, [=](const Vec<T>& x, double (&w)[N]) {
+        weights(x.z, sc, w);
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = inside(x.z[i], x.i0 + i, bb) ? w[i] : 0.0;
+    }, [&](double t) { return rp.u * t; }, [&](const Vec<T>& x) {
+#pragma unroll
+        for (int i = 0; i < N; i++) kn += inside(x.z[i], x.i0 + i, bb);
+    }, &total, &zp);
+    kn = wave_sum(kn);
+    if (lane == 0) sh.wi[wave] = kn;
+    __syncthreads();
+    if (tid == 0) {
+        int n = 0;
+        for (int i = 0; i < NW; i++) n += sh.wi[i];
+        write_row(op, row, pick, log_share(zp, zmax, rp.T, total), n);
+    }
+    if (op.probs) write_probs<T, NT>(op, row, view, sc, b, total);
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
+    __shared__ Shared<NT> sh;
+    const int row = blockIdx.x;
+    const RowView<T> view = view_of<T, NT>(op, row);
+    const RowParams rp = row_params(op, row);
+    float zmax;
+    int count;
+    partial_maxima<T, NT>(view, 0, view.nvec, sh, sh.group, 8, &zmax, &count);
+    if (!rp.valid || count == 0) write_none<NT>(op, row);
+    else answer_row<T, NT>(op, row, sh, view, rp, zmax, count, false);
+}
+
+// ---- few long rows: 2^LOG_SPLITS workgroups per row, in two launches ---------------------------------------------------------
+// k_sample_maxima leaves each part's share of the 256 partial maxima; k_sample_split bounds and gathers the part's candidates
+// into the row's list, and the last workgroup of a row to arrive finishes it (nothing waits).  Rows the short cut does not serve
+// are answered by one of their workgroups.
+struct SplitRow {
+    uint32_t group[256];
+    u64 list[kList];
+    float part_max[16];
+    int part_cnt[16];
+    int list_n, arrived;
+};
+constexpr int kSplitThreads = 1024;
+template <typename T>
+__device__ __forceinline__ void part_of(const RowView<T>& v, int part, int log_splits, int* a, int* b) {
+    const int per = ((v.nvec + (1 << log_splits) - 1) >> log_splits) + 63 & ~63;
+    *a = min(v.nvec, part * per);
+    *b = min(v.nvec, *a + per);
+}
+template <typename T>
+__global__ __launch_bounds__(kSplitThreads) void k_sample_maxima(SampleOp op, SplitRow* rows, int log_splits) {
+    __shared__ Shared<kSplitThreads> sh;
+    const int row = blockIdx.x >> log_splits, part = blockIdx.x & ((1 << log_splits) - 1);
+    const RowView<T> view = view_of<T, kSplitThreads>(op, row);
+    SplitRow& s = rows[row];
+    int a, b, count;
+    float zmax;
+    part_of(view, part, log_splits, &a, &b);
+    partial_maxima<T, kSplitThreads>(view, a, b, sh, s.group + (part << (8 - log_splits)), 8 - log_splits, &zmax, &count);
+    if (threadIdx.x == 0) {
+        s.part_max[part] = zmax;
+        s.part_cnt[part] = count;
+        if (part == 0) s.list_n = s.arrived = 0;
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(kSplitThreads) void k_sample_split(SampleOp op, SplitRow* rows, int log_splits) {
+    constexpr int NT = kSplitThreads, NW = NT / W;
+    __shared__ Shared<NT> sh;
+    const int row = blockIdx.x >> log_splits, part = blockIdx.x & ((1 << log_splits) - 1), tid = threadIdx.x;
+    const int lane = tid & 63, wave = uniform(tid >> 6);
+    const RowView<T> view = view_of<T, NT>(op, row);
+    RowParams rp = row_params(op, row);
+    SplitRow& s = rows[row];
+    float zmax = -INFINITY;
+    int count = 0;
+    for (int i = 0; i < 1 << log_splits; i++) {
+        zmax = fmaxf(zmax, s.part_max[i]);
+        count += s.part_cnt[i];
+    }
+    if (!rp.valid || count == 0) {
+        if (part == 0) write_none<NT>(op, row);
+        return;
+    }
+    if (tid < 256) sh.group[tid] = s.group[tid];
+    __syncthreads();
+    RowParams q = rp;
+    if (q.T == 0) {   // as in answer_row
+        q.T = 1;
+        q.k = 1;
+        q.p = 1;
+        q.m = 0;
+    }
+    q.k = q.k > 0 && q.k < count ? q.k : 0;
+    const bool quick = short_cut(q, q.k);
+    if (quick) {
+        const Scale sc = make_scale(zmax, q.T);
+        const float zl = short_cut_bound(sh, q, q.k, sc);
+        int a, b;
+        part_of(view, part, log_splits, &a, &b);
+        const int per = ((b - a + NW - 1) / NW + W - 1) / W * W, v0 = min(b, a + wave * per), v1 = min(b, v0 + per);
+        Row<T, NT> R{sh, view, sc, lane, wave, v0, v1};
+        const int n = R.gather(zl, INFINITY, Border{-FLT_MAX, 0x7fffffff});
+        if (tid == 0) sh.out_i = __hip_atomic_fetch_add(&s.list_n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const int base = sh.out_i;
+        // The workgroups of a row run on several XCDs, whose L2s do not see one another's writes.  What they exchange is written
+        // and read by device-scope atomics, which go past the L2s, and a wait for the writes stands before the count of arrivals:
+        // a release fence would write back the whole L2 (measured: 100 us instead of a few).
+        if (tid < min(n, kList) && base + tid < kList) __hip_atomic_store(&s.list[base + tid], sh.list[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) sh.bin = __hip_atomic_fetch_add(&s.arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (sh.bin != (1 << log_splits) - 1) return;
+        const int ln = __hip_atomic_load(&s.list_n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (ln <= kList) {
+            if (tid < ln) sh.list[tid] = __hip_atomic_load(&s.list[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            answer_from_list<T, NT>(op, row, sh, view, ln, q, sc, zmax, -1.0);
+            return;
         }
+    } else if (part) return;
+    answer_row<T, NT>(op, row, sh, view, rp, zmax, count, quick);
+}
+
+// 0: a workgroup per row.  Splitting pays while workgroups of one row each leave most of the chip idle, and a row is long enough
+// to be worth a second launch.
+inline int log_splits(const SampleOp& op) {
+    if (op.actions < 16384 || op.rows > 128) return 0;
+    return op.rows <= 16 ? 4 : op.rows <= 32 ? 3 : op.rows <= 64 ? 2 : 1;
 }
 
 template <typename T>
-hipError_t launch_typed(hipStream_t st, const SampleOp& op) {
+hipError_t launch_typed(hipStream_t st, const SampleOp& op, void* workspace) {
     if (op.actions <= 4 * W) {
         const dim3 grid((op.rows + kWaveRows - 1) / kWaveRows), block(W * kWaveRows);
         if (op.actions <= W) k_sample_wave<T, 1><<<grid, block, 0, st>>>(op);
@@ -1120,6 +1260,11 @@ hipError_t launch_typed(hipStream_t st, const SampleOp& op) {
         else k_sample_wave<T, 4><<<grid, block, 0, st>>>(op);
     } else if (op.actions <= 8192) {
         k_sample_block<T, 256><<<dim3(op.rows), dim3(256), 0, st>>>(op);
+    } else if (const int ls = log_splits(op)) {
+        SplitRow* rows = static_cast<SplitRow*>(workspace);
+        k_sample_maxima<T><<<dim3(op.rows << ls), dim3(kSplitThreads), 0, st>>>(op, rows, ls);
+        if (hipError_t e = hipGetLastError()) return e;
+        k_sample_split<T><<<dim3(op.rows << ls), dim3(kSplitThreads), 0, st>>>(op, rows, ls);
     } else {
         k_sample_block<T, 1024><<<dim3(op.rows), dim3(1024), 0, st>>>(op);
     }
@@ -1128,13 +1273,13 @@ hipError_t launch_typed(hipStream_t st, const SampleOp& op) {
 
 }  // namespace
 
-size_t sample_workspace_bytes(const SampleOp&) { return 0; }
+size_t sample_workspace_bytes(const SampleOp& op) { return log_splits(op) ? (size_t)op.rows * sizeof(SplitRow) : 0; }
 
-hipError_t launch_sample(hipStream_t st, const SampleOp& op, void*) {
+hipError_t launch_sample(hipStream_t st, const SampleOp& op, void* workspace) {
     switch (op.type) {
-        case kFp32: return launch_typed<float>(st, op);
-        case kBf16: return launch_typed<bf16_t>(st, op);
-        default: return launch_typed<_Float16>(st, op);
+        case kFp32: return launch_typed<float>(st, op, workspace);
+        case kBf16: return launch_typed<bf16_t>(st, op, workspace);
+        default: return launch_typed<_Float16>(st, op, workspace);
     }
 }
 
