@@ -490,7 +490,7 @@ struct Shared {
     u64 mass[kBins];
     uint32_t cnt[kBins];
     u64 list[kList];
-    uint32_t group[256];
+    alignas(16) uint32_t group[256];
     double wd[NW];
     int wi[NW];
     float wf[NW];
@@ -964,21 +964,39 @@ __device__ __forceinline__ float min_p_border(double m, double T, const Scale& s
     return of_key(first_key(kNoKey + 1, key_of((float)sc.zmax), guess, lane, [=](float z) { return weight(z, sc) >= m; }));
 }
 
-// The k-th largest (k <= 128) of the 256 partial maxima in sh.group, as a key: at least k entries are not below it.  One wave.
+// The k-th largest (k <= 128) of the 256 partial maxima in sh.group, as a key (at least k entries are not below it), to sh.bound:
+// every thread counts, for one of them, how many of a share of the others are not below it.  Begins and ends with a barrier.
 template <int NT>
-__device__ __forceinline__ uint32_t kth_partial(const Shared<NT>& sh, int k, int lane) {
-    uint32_t g[4], t = 0;
+__device__ __forceinline__ void kth_partial(Shared<NT>& sh, int k) {
+    constexpr int SHARE = 256 * 256 / NT;
+    const int tid = threadIdx.x;
+    if (tid < 256) sh.cnt[tid] = 0;
+    __syncthreads();
+    const uint32_t mine = sh.group[tid & 255];
+    const u32x4* others = reinterpret_cast<const u32x4*>(sh.group + (tid >> 8) * SHARE);
+    uint32_t n = 0;
+#pragma unroll 8
+    for (int i = 0; i < SHARE / 4; i++) {
+        const u32x4 o = others[i];
 #pragma unroll
-    for (int e = 0; e < 4; e++) g[e] = sh.group[e * W + lane];
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t c = t | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) n += __popcll(__ballot(g[e] >= c));
-        if (n >= k) t = c;
+        for (int e = 0; e < 4; e++) n += o[e] >= mine;
     }
-    return t;
+    atomicAdd(&sh.cnt[tid & 255], n);
+    __syncthreads();
+    if (tid < W) {
+        uint32_t t = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if ((int)sh.cnt[e * W + tid] >= k) t = max(t, sh.group[e * W + tid]);
+        t = max(t, xor_lane<1>(t, tid));
+        t = max(t, xor_lane<2>(t, tid));
+        t = max(t, xor_lane<4>(t, tid));
+        t = max(t, xor_lane<8>(t, tid));
+        t = max(t, xor_lane<16>(t, tid));
+        t = max(t, xor_lane<32>(t, tid));
+        if (tid == 0) sh.bound = t;
+    }
+    __syncthreads();
 }
 // maximum, number of entries and 2^LOG partial maxima (keys, to group[]) of this workgroup's vectors [a, b)
 template <typename T, int NT>
@@ -1062,14 +1080,11 @@ __device__ __forceinline__ void answer_from_list(const SampleOp& op, int row, Sh
 __device__ __forceinline__ bool short_cut(const RowParams& rp, int k) { return (k && k <= kFastK) || (rp.m > 0 && rp.p >= 1); }
 template <int NT>
 __device__ __forceinline__ float short_cut_bound(Shared<NT>& sh, const RowParams& rp, int k, const Scale& sc) {
-    if (threadIdx.x < W) {
-        const uint32_t t = k && k <= kFastK ? kth_partial(sh, k, threadIdx.x) : 0;
-        if (threadIdx.x == 0) sh.bound = t;
+    if (k && k <= kFastK) {
+        kth_partial(sh, k);
+        return sh.bound > kNoKey ? of_key(sh.bound) : -FLT_MAX;
     }
-    __syncthreads();
-    const float zl = sh.bound > kNoKey ? of_key(sh.bound) : -FLT_MAX;
-    // (top-p needs the mass of all of the first k)
-    return rp.p >= 1 && !k ? fmaxf(zl, min_p_border(rp.m, rp.T, sc, threadIdx.x & 63)) : zl;
+    return min_p_border(rp.m, rp.T, sc, threadIdx.x & 63);
 }
 
 // A row whose maximum, number of entries and partial maxima are known, by a workgroup.  tried: the short cut left too many.
@@ -1153,12 +1168,13 @@ __global__ __launch_bounds__(NT) void k_sample_block(SampleOp op) {
 // k_sample_maxima leaves each part's share of the 256 partial maxima; k_sample_split bounds and gathers the part's candidates
 // into the row's list, and the last workgroup of a row to arrive finishes it (nothing waits).  Rows the short cut does not serve
 // are answered by one of their workgroups.
+constexpr int kSlots = 512;      // candidates of a row, shared out evenly over its parts
 struct SplitRow {
+    u64 slot[kSlots];
     uint32_t group[256];
-    u64 list[kList];
     float part_max[16];
     int part_cnt[16];
-    int list_n, arrived;
+    uint32_t arrived;            // parts, + 2^8 per candidate
 };
 constexpr int kSplitThreads = 1024;
 template <typename T>
@@ -1180,7 +1196,7 @@ __global__ __launch_bounds__(kSplitThreads) void k_sample_maxima(SampleOp op, Sp
     if (threadIdx.x == 0) {
         s.part_max[part] = zmax;
         s.part_cnt[part] = count;
-        if (part == 0) s.list_n = s.arrived = 0;
+        if (part == 0) s.arrived = 0;
     }
 }
 template <typename T>
@@ -1190,19 +1206,20 @@ __global__ __launch_bounds__(kSplitThreads) void k_sample_split(SampleOp op, Spl
     const int row = blockIdx.x >> log_splits, part = blockIdx.x & ((1 << log_splits) - 1), tid = threadIdx.x;
     const int lane = tid & 63, wave = uniform(tid >> 6);
     const RowView<T> view = view_of<T, NT>(op, row);
-    RowParams rp = row_params(op, row);
     SplitRow& s = rows[row];
-    float zmax = -INFINITY;
-    int count = 0;
-    for (int i = 0; i < 1 << log_splits; i++) {
-        zmax = fmaxf(zmax, s.part_max[i]);
-        count += s.part_cnt[i];
-    }
+    // everything that is read first, in one go
+    const uint32_t g = s.group[tid & 255];
+    const int p16 = lane & ((1 << log_splits) - 1);
+    float zmax = s.part_max[p16];
+    int count = lane < 1 << log_splits ? s.part_cnt[p16] : 0;
+    const RowParams rp = row_params(op, row);
+    zmax = wave_max(zmax, lane);
+    count = wave_sum(count);
     if (!rp.valid || count == 0) {
         if (part == 0) write_none<NT>(op, row);
         return;
     }
-    if (tid < 256) sh.group[tid] = s.group[tid];
+    if (tid < 256) sh.group[tid] = g;
     __syncthreads();
     RowParams q = rp;
     if (q.T == 0) {   // as in answer_row
@@ -1221,21 +1238,27 @@ __global__ __launch_bounds__(kSplitThreads) void k_sample_split(SampleOp op, Spl
         const int per = ((b - a + NW - 1) / NW + W - 1) / W * W, v0 = min(b, a + wave * per), v1 = min(b, v0 + per);
         Row<T, NT> R{sh, view, sc, lane, wave, v0, v1};
         const int n = R.gather(zl, INFINITY, Border{-FLT_MAX, 0x7fffffff});
-        if (tid == 0) sh.out_i = __hip_atomic_fetch_add(&s.list_n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        const int base = sh.out_i;
         // The workgroups of a row run on several XCDs, whose L2s do not see one another's writes.  What they exchange is written
         // and read by device-scope atomics, which go past the L2s, and a wait for the writes stands before the count of arrivals:
         // a release fence would write back the whole L2 (measured: 100 us instead of a few).
-        if (tid < min(n, kList) && base + tid < kList) __hip_atomic_store(&s.list[base + tid], sh.list[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int slots = kSlots >> log_splits;
+        if (tid < slots) __hip_atomic_store(&s.slot[part * slots + tid], tid < min(n, kList) ? sh.list[tid] : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (tid == 0) sh.bin = __hip_atomic_fetch_add(&s.arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) {
+            const uint32_t add = 1u + ((uint32_t)(n <= min(slots, kList) ? n : kSlots + 1) << 8);   // one that did not fit: too many in all
+            sh.bound = add + __hip_atomic_fetch_add(&s.arrived, add, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sh.list_n = 0;
+        }
         __syncthreads();
-        if (sh.bin != (1 << log_splits) - 1) return;
-        const int ln = __hip_atomic_load(&s.list_n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t seen = sh.bound;
+        if ((seen & 255u) != 1u << log_splits) return;
+        const int ln = (int)(seen >> 8);
         if (ln <= kList) {
-            if (tid < ln) sh.list[tid] = __hip_atomic_load(&s.list[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (tid < kSlots) {
+                const u64 r = __hip_atomic_load(&s.slot[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (r) sh.list[atomicAdd(&sh.list_n, 1)] = r;
+            }
             __syncthreads();
             answer_from_list<T, NT>(op, row, sh, view, ln, q, sc, zmax, -1.0);
             return;
