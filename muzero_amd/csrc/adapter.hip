@@ -92,24 +92,28 @@ __device__ __forceinline__ int adapter_of(const AdapterOp& op, int m) {
 }
 
 // Orders the rows [m0, m0 + count) of a workgroup by adapter (rows of none last): order[p] = row, key[p] = its adapter, kNone or
-// kForeign (p >= count: kNoRow), nth[p] = how many rows of that key are in front of it.  count <= BR <= threads; ends with a barrier.
+// kForeign (p >= count: kNoRow), nth[p] = how many rows of that key are in front of it.  count <= BR <= threads; raw is 16-byte
+// aligned; ends with a barrier.
 template <int BR>
 __device__ __forceinline__ void order_rows(const AdapterOp& op, int m0, int count, int* raw, int* order, int* key, int* nth) {
     const int tid = threadIdx.x;
     if (tid < BR) raw[tid] = tid < count ? adapter_of(op, m0 + tid) : kNoRow;
     __syncthreads();
     if (tid < BR) {
-        const unsigned mine = (unsigned)raw[tid];   // negative values are the largest
-        int pos = 0, eq = 0;
-#pragma unroll 8
-        for (int j = 0; j < BR; j++) {
-            const unsigned o = (unsigned)raw[j];
-            pos += o < mine || (o == mine && j < tid);
-            eq += o == mine && j < tid;
+        const unsigned mine = (unsigned)raw[tid];
+        int less = 0, eq = 0;
+#pragma unroll 4
+        for (int j = 0; j < BR / 4; j++) {
+            const u32x4 o = reinterpret_cast<const u32x4*>(raw)[j];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                less += o[e] < mine;
+                eq += (int)(o[e] == mine) & (int)(4 * j + e < tid);
+            }
         }
-        order[pos] = tid;
-        key[pos] = (int)mine;
-        nth[pos] = eq;
+        order[less + eq] = tid;
+        key[less + eq] = (int)mine;
+        nth[less + eq] = eq;
     }
     __syncthreads();
 }
@@ -134,47 +138,52 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
 
 // ---- t = x A^T -------------------------------------------------------------------------------------------------------------
 // Workgroup (block of BR rows, part of K): jobs of up to 16 rows of one adapter, a wave each.  part[s][row][padded rank].
+// 16 rows: a wave for every job there can be.
+template <int BR>
+constexpr int kShrinkWaves = BR == 16 ? 16 : 4;
 template <typename T, int RT, int BR>
-__global__ __launch_bounds__(256) void k_shrink(AdapterOp op, float* part, int splits) {
+__global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, float* part, int splits) {
     constexpr int CE = kChunk<T>;
-    __shared__ int raw[BR], order[BR], key[BR], nth[BR], job[BR], jobs;
+    static_assert(BR <= 128, "starts are counted in two waves");
+    __shared__ alignas(16) int raw[BR];
+    __shared__ int order[BR], key[BR], nth[BR], job[BR], starts[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, kq = lane >> 4;
     const int m0 = blockIdx.x * BR, count = min(BR, op.rows - m0), split = blockIdx.y;
     order_rows<BR>(op, m0, count, raw, order, key, nth);
-    if (tid < BR) {
-        const bool start = key[tid] >= 0 && nth[tid] % 16 == 0;
-        int id = 0;
-        for (int j = 0; j < tid; j++) id += key[j] >= 0 && nth[j] % 16 == 0;
-        if (start) job[id] = tid;
-        if (tid == BR - 1) jobs = id + start;
-    }
+    const bool start = tid < BR && key[tid < BR ? tid : 0] >= 0 && nth[tid < BR ? tid : 0] % 16 == 0;
+    const unsigned long long sb = __ballot(start);
+    if (wave < 2 && lane == 0) starts[wave] = __popcll(sb);
+    __syncthreads();
+    if (start) job[__builtin_amdgcn_mbcnt_hi((unsigned)(sb >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)sb, 0)) + (wave ? starts[0] : 0)] = tid;
+    const int jobs = starts[0] + starts[1];
     __syncthreads();
     const int rp = padded_rank(op.rank);
     const int pairs = (op.K + 8 * CE - 1) / (8 * CE);           // 128-byte steps of k
     const int p0 = (int)((long long)pairs * split / splits), p1 = (int)((long long)pairs * (split + 1) / splits);
     const int pf = min(p1, op.K / (8 * CE));                    // whole ones
-    for (int j = wave; j < jobs; j += 4) {
+    for (int j = wave; j < jobs; j += kShrinkWaves<BR>) {
         const int at = job[j], i = key[at], p = at + lr;
         const bool mine = p < count && key[p] == i;
         const int m = m0 + order[mine ? p : at];
-        const T* x = static_cast<const T*>(op.x) + m * op.x_stride + kq * 2 * CE;
+        const T* x = static_cast<const T*>(op.x) + m * op.x_stride + kq * CE;
         const T* a[RT];
 #pragma unroll
         for (int q = 0; q < RT; q++)   // ranks beyond the last: a row that is there, its results are dropped
-            a[q] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min(q * 16 + lr, op.rank - 1)) * op.K + kq * 2 * CE;
+            a[q] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min(q * 16 + lr, op.rank - 1)) * op.K + kq * CE;
         f32x4 acc[RT] = {};
         int k = p0;
-        constexpr int U = RT <= 2 ? 4 : 2;
+        constexpr int U = RT == 1 ? 4 : RT == 2 ? (BR == 16 ? 3 : 4) : RT == 8 && BR == 16 ? 1 : 2;   // what the registers hold
         for (; k + U <= pf; k += U) {
             u32x4 fx[U][2], fa[U][RT][2];
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    fx[u][h] = load16(x + (k + u) * 8 * CE + h * CE);
+                    fx[u][h] = load16(x + (k + u) * 8 * CE + h * 4 * CE);
 #pragma unroll
-                    for (int q = 0; q < RT; q++) fa[u][q][h] = load16(a[q] + (k + u) * 8 * CE + h * CE);
+                    for (int q = 0; q < RT; q++) fa[u][q][h] = load16(a[q] + (k + u) * 8 * CE + h * 4 * CE);
                 }
+            __builtin_amdgcn_sched_barrier(0);   // all loads in flight before the first use
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
@@ -185,10 +194,10 @@ __global__ __launch_bounds__(256) void k_shrink(AdapterOp op, float* part, int s
         for (; k < p1; k++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int left = op.K - kq * 2 * CE;             // x and a already stand at this lane's first chunk
-                const u32x4 fx = load_chunk(x, k * 8 * CE + h * CE, left);
+                const int left = op.K - kq * CE;             // x and a already stand at this lane's first chunk
+                const u32x4 fx = load_chunk(x, k * 8 * CE + h * 4 * CE, left);
 #pragma unroll
-                for (int q = 0; q < RT; q++) acc[q] = mma<T>(load_chunk(a[q], k * 8 * CE + h * CE, left), fx, acc[q]);
+                for (int q = 0; q < RT; q++) acc[q] = mma<T>(load_chunk(a[q], k * 8 * CE + h * 4 * CE, left), fx, acc[q]);
             }
         if (mine) {
             float* dst = part + ((long long)split * op.rows + m) * rp + kq * 4;
@@ -242,16 +251,26 @@ __device__ __forceinline__ void store4(const AdapterOp& op, int m, int n, f32x4 
 }
 
 // ---- up to 64 rows -----------------------------------------------------------------------------------------------------------
-// Workgroup: 16 NT rows of W, all 16 MT rows of x; 8 waves split K by 128-byte steps; partial sums meet in LDS.
+// Workgroup: 16 NT rows of W, all 16 MT rows of x; the waves split K by 128-byte steps; partial sums meet in LDS.
 // FJ > 0: t is computed here, FJ >= rows * rank tiles more tiles of 16 rows (of A).
-constexpr int kSkinnyWaves = 8;
+template <int MT>
+constexpr int kSkinnyWaves = MT == 1 ? 16 : 8;
 template <int MT, int NT, int FJ>
 constexpr size_t skinny_lds() {
-    return (size_t)kSkinnyWaves * (MT * NT + FJ) * 64 * 16;
+    return (size_t)kSkinnyWaves<MT> * (MT * NT + FJ) * 64 * 16;
+}
+template <typename T>
+__device__ __forceinline__ float dot_chunk(const float* t, u32x4 c) {
+    T h[kChunk<T>];
+    __builtin_memcpy(h, &c, 16);
+    float d = 0;
+#pragma unroll
+    for (int k = 0; k < kChunk<T>; k++) d = fmaf(t[k], to_float(h[k]), d);
+    return d;
 }
 template <typename T, int MT, int NT, int FJ>
-__global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, const float* part, int splits) {
-    constexpr int CE = kChunk<T>, NW = kSkinnyWaves, TILES = MT * NT;
+__global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, const float* part, int splits) {
+    constexpr int CE = kChunk<T>, NW = kSkinnyWaves<MT>, TILES = MT * NT, NTH = 64 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     f32x4* red = reinterpret_cast<f32x4*>(smem);                              // [NW][TILES + FJ][64]
     float* tl = reinterpret_cast<float*>(smem + skinny_lds<MT, NT, FJ>());    // [rows][padded rank]
@@ -259,17 +278,30 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, cons
     const int n0 = blockIdx.x * 16 * NT, rp = padded_rank(op.rank), rt = rp / 16;
     const T *w[NT], *x[MT], *a[FJ ? FJ : 1];
 #pragma unroll
-    for (int i = 0; i < NT; i++) w[i] = static_cast<const T*>(op.w) + min(n0 + i * 16 + lr, op.N - 1) * op.w_stride + kq * 2 * CE;
+    for (int i = 0; i < NT; i++) w[i] = static_cast<const T*>(op.w) + min(n0 + i * 16 + lr, op.N - 1) * op.w_stride + kq * CE;
 #pragma unroll
-    for (int i = 0; i < MT; i++) x[i] = static_cast<const T*>(op.x) + min(i * 16 + lr, op.rows - 1) * op.x_stride + kq * 2 * CE;
+    for (int i = 0; i < MT; i++) x[i] = static_cast<const T*>(op.x) + min(i * 16 + lr, op.rows - 1) * op.x_stride + kq * CE;
 #pragma unroll
     for (int j = 0; j < FJ; j++) {
         const int m = min(j / rt, op.rows - 1), i = max(adapter_of(op, m), 0);   // of none: some A, its t is not used
-        a[j] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min((j % rt) * 16 + lr, op.rank - 1)) * op.K + kq * 2 * CE;
+        a[j] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min((j % rt) * 16 + lr, op.rank - 1)) * op.K + kq * CE;
     }
+    // Up to 16 rows: t B^T is shared out as items (row, column, chunk of ranks), one per thread if there are that many; a
+    // thread's first B chunk is fetched here, long before it is used.
+    const int chunks = (op.rank + CE - 1) / CE, items = op.rows * 16 * NT * chunks;
+    const bool spread = MT == 1 && items * 4 <= (int)skinny_lds<MT, NT, FJ>();
+    auto b_chunk = [&](int it) {
+        const int c = it % chunks, n = it / chunks % (16 * NT), i = adapter_of(op, it / chunks / (16 * NT));
+        u32x4 v = {0, 0, 0, 0};
+        if (i >= 0 && n0 + n < op.N) v = load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + n0 + n) * op.rank, c * CE, op.rank);
+        return v;
+    };
+    u32x4 b0 = {0, 0, 0, 0};
+    if (spread && tid < items) b0 = b_chunk(tid);
+
     f32x4 acc[NT][MT] = {}, ta[FJ ? FJ : 1] = {};
     const int pairs = (op.K + 8 * CE - 1) / (8 * CE), pf = op.K / (8 * CE);
-    constexpr int U = TILES + FJ <= 3 ? 4 : MT + NT <= 4 ? 2 : 1;
+    constexpr int U = MT + NT + FJ <= 2 ? 4 : MT + NT + FJ == 3 ? (MT == 1 ? 3 : 4) : MT == 1 && NT + FJ > 4 ? 1 : 2;   // what the registers hold
     int p = wave;
     for (; p + (U - 1) * NW < pf; p += U * NW) {
         u32x4 fw[U][NT][2], fx[U][MT][2], fa[U][FJ ? FJ : 1][2];
@@ -277,7 +309,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, cons
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int k = (p + u * NW) * 8 * CE + h * CE;
+                const int k = (p + u * NW) * 8 * CE + h * 4 * CE;
 #pragma unroll
                 for (int i = 0; i < NT; i++) fw[u][i][h] = load16(w[i] + k);
 #pragma unroll
@@ -285,6 +317,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, cons
 #pragma unroll
                 for (int i = 0; i < MT; i++) fx[u][i][h] = load16(x[i] + k);
             }
+        __builtin_amdgcn_sched_barrier(0);   // all loads in flight before the first use
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -300,7 +333,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, cons
     for (; p < pairs; p += NW)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int k = p * 8 * CE + h * CE, left = op.K - kq * 2 * CE;
+            const int k = p * 8 * CE + h * 4 * CE, left = op.K - kq * CE;
             u32x4 fx[MT];
 #pragma unroll
             for (int j = 0; j < MT; j++) fx[j] = load_chunk(x[j], k, left);
@@ -320,47 +353,66 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void k_skinny(AdapterOp op, cons
 #pragma unroll
     for (int j = 0; j < FJ; j++) red[(wave * (TILES + FJ) + TILES + j) * 64 + lane] = ta[j];
     if (!FJ) {
-        for (int q = tid; q < op.rows * (rp / 4); q += 64 * NW) {
+        for (int q = tid; q < op.rows * (rp / 4); q += NTH) {
             const int m = q / (rp / 4), r = q % (rp / 4) * 4;
             *reinterpret_cast<f32x4*>(tl + m * rp + r) = sum_parts(part, splits, op.rows, m, rp, r);
         }
     }
     __syncthreads();
     if (FJ) {   // column m of job (m, rank tile) holds t[m]
-        for (int q = tid; q < op.rows * rp; q += 64 * NW) {
+        for (int q = tid; q < op.rows * rp; q += NTH) {
             const int m = q / rp, r = q % rp, j = m * rt + r / 16;
             float v = 0;
+#pragma unroll
             for (int s = 0; s < NW; s++) v += red[(s * (TILES + FJ) + TILES + j) * 64 + (r % 16 / 4) * 16 + m][r & 3];
             tl[m * rp + r] = r < op.rank ? v : 0.f;
         }
-        __syncthreads();
     }
-    for (int q = tid; q < TILES * 64; q += 64 * NW) {
-        const int tile = q / 64, l = q % 64, m = (tile % MT) * 16 + (l & 15), n = n0 + (tile / MT) * 16 + (l >> 4) * 4;
-        if (m >= op.rows || n >= op.N) continue;
+    // results (row m, columns n ..): four neighbours a thread
+    auto total = [&](int q) {
         f32x4 v = {};
 #pragma unroll
-        for (int s = 0; s < NW; s++) v += red[(s * (TILES + FJ) + tile) * 64 + l];
+        for (int s = 0; s < NW; s++) v += red[(s * (TILES + FJ) + q / 64) * 64 + q % 64];
+        return v;
+    };
+    auto finish = [&](int q, f32x4 v, auto term) {
+        const int tile = q / 64, l = q % 64, m = (tile % MT) * 16 + (l & 15), nl = (tile / MT) * 16 + (l >> 4) * 4;
+        if (m >= op.rows || n0 + nl >= op.N) return;
         const int i = adapter_of(op, m);
         if (i >= 0) {
             const float sc = op.scale ? op.scale[i] : 1.f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + min(n + e, op.N - 1)) * op.rank;
-                float d = 0;
-                for (int r = 0; r < op.rank; r += CE) {
-                    const u32x4 c = load_chunk(b, r, op.rank);
-                    T h[CE];
-                    __builtin_memcpy(h, &c, 16);
-#pragma unroll
-                    for (int k = 0; k < CE; k++) d = fmaf(tl[m * rp + r + k], to_float(h[k]), d);
-                }
-                v[e] = fmaf(sc, d, v[e]);
-            }
+            for (int e = 0; e < 4; e++) v[e] = fmaf(sc, term(m, nl + e, i), v[e]);
         } else if (i == kForeign) {
             v = f32x4{NAN, NAN, NAN, NAN};
         }
-        store4<T>(op, m, n, v);
+        store4<T>(op, m, n0 + nl, v);
+    };
+    if (spread) {
+        f32x4 v = {};
+        if (tid < TILES * 64) v = total(tid);
+        __syncthreads();
+        float* ex = reinterpret_cast<float*>(smem);   // [item], where the partial sums were
+        for (int it = tid; it < items; it += NTH) {
+            const u32x4 c = it == tid ? b0 : b_chunk(it);
+            ex[it] = dot_chunk<T>(tl + it / chunks / (16 * NT) * rp + it % chunks * CE, c);
+        }
+        __syncthreads();
+        if (tid < TILES * 64)
+            finish(tid, v, [&](int m, int n, int) {
+                float d = 0;
+                for (int c = 0; c < chunks; c++) d += ex[(m * 16 * NT + n) * chunks + c];
+                return d;
+            });
+    } else {
+        __syncthreads();
+        for (int q = tid; q < TILES * 64; q += NTH)
+            finish(q, total(q), [&](int m, int n, int i) {
+                const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + min(n0 + n, op.N - 1)) * op.rank;
+                float d = 0;
+                for (int r = 0; r < op.rank; r += CE) d += dot_chunk<T>(tl + m * rp + r, load_chunk(b, r, op.rank));
+                return d;
+            });
     }
 }
 
@@ -608,10 +660,14 @@ Plan make_plan(const AdapterOp& op) {
     p.skinny = op.rows <= 64;
     if (p.skinny) {
         p.mt = (op.rows + 15) / 16;
-        // more rows of W per workgroup once there are enough workgroups: x is read once per workgroup
-        p.nt = p.mt == 1 ? (op.N > 16 * 2 * kCus ? 2 : 1) : p.mt == 2 ? 2 : 4;
+        // rows of W per workgroup: what leaves the fewest rounds of workgroups on the chip; among equals the most, as every
+        // workgroup reads x
+        auto rounds = [&](int nt) { return ((op.N + 16 * nt - 1) / (16 * nt) + kCus - 1) / kCus * nt; };
+        p.nt = 3;
+        for (int nt = 2; nt >= 1; nt--)
+            if (rounds(nt) < rounds(p.nt)) p.nt = nt;
         // every workgroup reads the A of all rows: only while that is little
-        p.fused = p.mt == 1 && op.rows * rt <= 2;
+        p.fused = op.rows * rt <= 2;
         p.block = 16;
     } else {
         p.block = op.rows <= 1024 ? 16 : 128;
@@ -630,7 +686,13 @@ template <typename T, int MT, int NT, int FJ>
 void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
     const size_t lds = skinny_lds<MT, NT, FJ>() + (size_t)op.rows * padded_rank(op.rank) * 4;
     lds_optin((const void*)k_skinny<T, MT, NT, FJ>);
-    k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT)), dim3(64 * kSkinnyWaves), lds, st>>>(op, part, splits);
+    k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT)), dim3(64 * kSkinnyWaves<MT>), lds, st>>>(op, part, splits);
+}
+template <typename T, int MT, int FJ>
+void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits, int nt) {
+    if (nt == 1) launch_skinny<T, MT, 1, FJ>(st, op, part, splits);
+    else if (nt == 2) launch_skinny<T, MT, 2, FJ>(st, op, part, splits);
+    else launch_skinny<T, MT, 3, FJ>(st, op, part, splits);
 }
 template <typename T, int B, int WM, int WN>
 void launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
@@ -649,12 +711,13 @@ void launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int spl
 }
 template <typename T, int BR>
 void launch_shrink(hipStream_t st, const AdapterOp& op, float* part, int splits) {
+    constexpr int NTH = 64 * kShrinkWaves<BR>;
     const dim3 grid((op.rows + BR - 1) / BR, splits);
     const int rt = padded_rank(op.rank) / 16;
-    if (rt == 1) k_shrink<T, 1, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
-    else if (rt == 2) k_shrink<T, 2, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
-    else if (rt <= 4) k_shrink<T, 4, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
-    else k_shrink<T, 8, BR><<<grid, dim3(256), 0, st>>>(op, part, splits);
+    if (rt == 1) k_shrink<T, 1, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
+    else if (rt == 2) k_shrink<T, 2, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
+    else if (rt <= 4) k_shrink<T, 4, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
+    else k_shrink<T, 8, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
 }
 
 template <typename T>
@@ -667,13 +730,12 @@ hipError_t launch_typed(hipStream_t st, const AdapterOp& op, void* workspace) {
         if (hipError_t e = hipGetLastError()) return e;
     }
     if (p.skinny) {
-        if (p.fused && p.nt == 1) launch_skinny<T, 1, 1, 2>(st, op, part, p.splits);
-        else if (p.fused) launch_skinny<T, 1, 2, 2>(st, op, part, p.splits);
-        else if (p.mt == 1 && p.nt == 1) launch_skinny<T, 1, 1, 0>(st, op, part, p.splits);
-        else if (p.mt == 1) launch_skinny<T, 1, 2, 0>(st, op, part, p.splits);
-        else if (p.mt == 2) launch_skinny<T, 2, 2, 0>(st, op, part, p.splits);
-        else if (p.mt == 3) launch_skinny<T, 3, 4, 0>(st, op, part, p.splits);
-        else launch_skinny<T, 4, 4, 0>(st, op, part, p.splits);
+        if (p.fused && op.rows * padded_rank(op.rank) == 16) launch_skinny<T, 1, 1>(st, op, part, p.splits, p.nt);
+        else if (p.fused) launch_skinny<T, 1, 2>(st, op, part, p.splits, p.nt);
+        else if (p.mt == 1) launch_skinny<T, 1, 0>(st, op, part, p.splits, p.nt);
+        else if (p.mt == 2) launch_skinny<T, 2, 0>(st, op, part, p.splits, p.nt);
+        else if (p.mt == 3) launch_skinny<T, 3, 0>(st, op, part, p.splits, p.nt);
+        else launch_skinny<T, 4, 0>(st, op, part, p.splits, p.nt);
     } else if (p.tile == 256) {
         launch_tile<T, 256, 4, 2>(st, op, part, p.splits);
     } else if (p.tile == 128) {
