@@ -13,8 +13,16 @@
 
 #include <math.h>
 
+#include <utility>
+
 namespace mz {
 namespace {
+
+// f(0), f(1), .. with constant arguments: accumulators indexed by them stay in registers however long f is
+template <typename F, int... I>
+__device__ __forceinline__ void static_for(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -92,28 +100,58 @@ __device__ __forceinline__ int adapter_of(const AdapterOp& op, int m) {
 }
 
 // Orders the rows [m0, m0 + count) of a workgroup by adapter (rows of none last): order[p] = row, key[p] = its adapter, kNone or
-// kForeign (p >= count: kNoRow), nth[p] = how many rows of that key are in front of it.  count <= BR <= threads; raw is 16-byte
-// aligned; ends with a barrier.
-template <int BR>
+// kForeign (p >= count: kNoRow), nth[p] = how many rows of that key are in front of it.  A row's place is the number of rows that
+// go before it, counted by NTH / BR threads each; rows that stand in order already, as the tokens of one request after the other,
+// are left there.  All arrays 16-byte aligned; ends with a barrier.
+template <int BR, int NTH, bool NEED_NTH>
 __device__ __forceinline__ void order_rows(const AdapterOp& op, int m0, int count, int* raw, int* order, int* key, int* nth) {
-    const int tid = threadIdx.x;
-    if (tid < BR) raw[tid] = tid < count ? adapter_of(op, m0 + tid) : kNoRow;
-    __syncthreads();
+    constexpr int SHARE = BR * BR / NTH < 4 ? 4 : BR * BR / NTH;
+    static_assert(NTH % BR == 0 && SHARE % 4 == 0, "threads");
+    const int tid = threadIdx.x, r = tid % BR, first = tid / BR * SHARE;   // (a share behind the last row: nothing)
     if (tid < BR) {
-        const unsigned mine = (unsigned)raw[tid];
+        raw[tid] = tid < count ? adapter_of(op, m0 + tid) : kNoRow;
+        order[tid] = 0;      // (counters until the end)
+        nth[tid] = 0;
+    }
+    __syncthreads();
+    const unsigned mine = (unsigned)raw[r];
+    if (tid < BR && r + 1 < BR && mine > (unsigned)raw[r + 1]) order[0] = 1;
+    __syncthreads();
+    const bool sorted = order[0] == 0;
+    if (!sorted || NEED_NTH) {
+        __syncthreads();
+        if (tid == 0) order[0] = 0;
+        __syncthreads();
         int less = 0, eq = 0;
 #pragma unroll 4
-        for (int j = 0; j < BR / 4; j++) {
-            const u32x4 o = reinterpret_cast<const u32x4*>(raw)[j];
+        for (int j = first; j < min(first + SHARE, BR); j += 4) {
+            const u32x4 o = *reinterpret_cast<const u32x4*>(raw + j);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 less += o[e] < mine;
-                eq += (int)(o[e] == mine) & (int)(4 * j + e < tid);
+                eq += (int)(o[e] == mine) & (int)(j + e < r);
             }
         }
-        order[less + eq] = tid;
-        key[less + eq] = (int)mine;
-        nth[less + eq] = eq;
+        atomicAdd(&order[r], less + eq);
+        if (NEED_NTH) atomicAdd(&nth[r], eq);
+        __syncthreads();
+        int pos = 0, n = 0;
+        if (tid < BR) {
+            pos = order[r];
+            n = nth[r];
+        }
+        __syncthreads();
+        if (tid < BR) {
+            order[pos] = r;
+            key[pos] = (int)mine;
+            nth[pos] = n;
+        }
+    } else {
+        __syncthreads();
+        if (tid < BR) {
+            order[r] = r;
+            key[r] = (int)mine;
+        }
     }
     __syncthreads();
 }
@@ -138,9 +176,9 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
 
 // ---- t = x A^T -------------------------------------------------------------------------------------------------------------
 // Workgroup (block of BR rows, part of K): jobs of up to 16 rows of one adapter, a wave each.  part[s][row][padded rank].
-// 16 rows: a wave for every job there can be.
+// 16 rows: a wave for every job there can be; 128 rows: 8 waves, as many as 8 rank tiles leave registers for.
 template <int BR>
-constexpr int kShrinkWaves = BR == 16 ? 16 : 4;
+constexpr int kShrinkWaves = BR == 16 ? 16 : 8;
 template <typename T, int RT, int BR>
 __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, float* part, int splits) {
     constexpr int CE = kChunk<T>;
@@ -149,7 +187,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, 
     __shared__ int order[BR], key[BR], nth[BR], job[BR], starts[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, kq = lane >> 4;
     const int m0 = blockIdx.x * BR, count = min(BR, op.rows - m0), split = blockIdx.y;
-    order_rows<BR>(op, m0, count, raw, order, key, nth);
+    order_rows<BR, 64 * kShrinkWaves<BR>, true>(op, m0, count, raw, order, key, nth);
     const bool start = tid < BR && key[tid < BR ? tid : 0] >= 0 && nth[tid < BR ? tid : 0] % 16 == 0;
     const unsigned long long sb = __ballot(start);
     if (wave < 2 && lane == 0) starts[wave] = __popcll(sb);
@@ -212,10 +250,19 @@ __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, 
         }
     }
 }
-// the parts of four ranks of a row, added in order
+// the parts of four ranks of a row, added in order; up to 8 loads in flight
 __device__ __forceinline__ f32x4 sum_parts(const float* part, int splits, long long rows, long long m, int rp, int r) {
     f32x4 v = {};
-    for (int s = 0; s < splits; s++) v += *reinterpret_cast<const f32x4*>(part + (s * rows + m) * rp + r);
+    const float* p = part + m * rp + r;
+    const long long step = rows * rp;
+    for (int s = 0; s < splits; s += 8) {
+        f32x4 t[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = *reinterpret_cast<const f32x4*>(p + min(s + i, splits - 1) * step);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (s + i < splits) v += t[i];
+    }
     return v;
 }
 
@@ -273,7 +320,8 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
     constexpr int CE = kChunk<T>, NW = kSkinnyWaves<MT>, TILES = MT * NT, NTH = 64 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     f32x4* red = reinterpret_cast<f32x4*>(smem);                              // [NW][TILES + FJ][64]
-    float* tl = reinterpret_cast<float*>(smem + skinny_lds<MT, NT, FJ>());    // [rows][padded rank]
+    int* adapter = reinterpret_cast<int*>(smem + skinny_lds<MT, NT, FJ>());   // [16 MT]
+    float* tl = reinterpret_cast<float*>(adapter + 16 * MT);                  // [rows][padded rank]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, kq = lane >> 4;
     const int n0 = blockIdx.x * 16 * NT, rp = padded_rank(op.rank), rt = rp / 16;
     const T *w[NT], *x[MT], *a[FJ ? FJ : 1];
@@ -281,42 +329,39 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
     for (int i = 0; i < NT; i++) w[i] = static_cast<const T*>(op.w) + min(n0 + i * 16 + lr, op.N - 1) * op.w_stride + kq * CE;
 #pragma unroll
     for (int i = 0; i < MT; i++) x[i] = static_cast<const T*>(op.x) + min(i * 16 + lr, op.rows - 1) * op.x_stride + kq * CE;
+    f32x4 acc[NT][MT] = {}, ta[FJ ? FJ : 1] = {};
+    const int pairs = (op.K + 8 * CE - 1) / (8 * CE), pf = op.K / (8 * CE);
+    constexpr int U = MT + NT + FJ <= 2 ? 4 : MT + NT + FJ == 3 ? (MT == 1 ? 3 : 4) : MT == 1 && NT + FJ > 4 ? 1 : 2;   // what the registers hold
+    int p = wave;
+    u32x4 fw[U][NT][2], fx[U][MT][2], fa[U][FJ ? FJ : 1][2];
+    const auto k_of = [&](int u, int h) { return (p + u * NW) * 8 * CE + h * 4 * CE; };
+    const auto fetch = [&] {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int i = 0; i < NT; i++) fw[u][i][h] = load16(w[i] + k_of(u, h));
+#pragma unroll
+                for (int i = 0; i < MT; i++) fx[u][i][h] = load16(x[i] + k_of(u, h));
+            }
+    };
+    const auto more = [&] { return p + (U - 1) * NW < pf; };
+    if (more()) fetch();                    // before anything that waits for the rows' adapters
+    __builtin_amdgcn_sched_barrier(0);
+    if (tid < op.rows) adapter[tid] = adapter_of(op, tid);
 #pragma unroll
     for (int j = 0; j < FJ; j++) {
         const int m = min(j / rt, op.rows - 1), i = max(adapter_of(op, m), 0);   // of none: some A, its t is not used
         a[j] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min((j % rt) * 16 + lr, op.rank - 1)) * op.K + kq * CE;
     }
-    // Up to 16 rows: t B^T is shared out as items (row, column, chunk of ranks), one per thread if there are that many; a
-    // thread's first B chunk is fetched here, long before it is used.
-    const int chunks = (op.rank + CE - 1) / CE, items = op.rows * 16 * NT * chunks;
-    const bool spread = MT == 1 && items * 4 <= (int)skinny_lds<MT, NT, FJ>();
-    auto b_chunk = [&](int it) {
-        const int c = it % chunks, n = it / chunks % (16 * NT), i = adapter_of(op, it / chunks / (16 * NT));
-        u32x4 v = {0, 0, 0, 0};
-        if (i >= 0 && n0 + n < op.N) v = load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + n0 + n) * op.rank, c * CE, op.rank);
-        return v;
-    };
-    u32x4 b0 = {0, 0, 0, 0};
-    if (spread && tid < items) b0 = b_chunk(tid);
-
-    f32x4 acc[NT][MT] = {}, ta[FJ ? FJ : 1] = {};
-    const int pairs = (op.K + 8 * CE - 1) / (8 * CE), pf = op.K / (8 * CE);
-    constexpr int U = MT + NT + FJ <= 2 ? 4 : MT + NT + FJ == 3 ? (MT == 1 ? 3 : 4) : MT == 1 && NT + FJ > 4 ? 1 : 2;   // what the registers hold
-    int p = wave;
-    for (; p + (U - 1) * NW < pf; p += U * NW) {
-        u32x4 fw[U][NT][2], fx[U][MT][2], fa[U][FJ ? FJ : 1][2];
+    while (more()) {
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int k = (p + u * NW) * 8 * CE + h * 4 * CE;
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < NT; i++) fw[u][i][h] = load16(w[i] + k);
-#pragma unroll
-                for (int j = 0; j < FJ; j++) fa[u][j][h] = load16(a[j] + k);
-#pragma unroll
-                for (int i = 0; i < MT; i++) fx[u][i][h] = load16(x[i] + k);
-            }
+                for (int j = 0; j < FJ; j++) fa[u][j][h] = load16(a[j] + k_of(u, h));
         __builtin_amdgcn_sched_barrier(0);   // all loads in flight before the first use
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -329,6 +374,8 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
 #pragma unroll
                 for (int j = 0; j < FJ; j++) ta[j] = mma<T>(fa[u][j][h], fx[u][0][h], ta[j]);
             }
+        p += U * NW;
+        if (more()) fetch();
     }
     for (; p < pairs; p += NW)
 #pragma unroll
@@ -368,51 +415,64 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
             tl[m * rp + r] = r < op.rank ? v : 0.f;
         }
     }
-    // results (row m, columns n ..): four neighbours a thread
-    auto total = [&](int q) {
-        f32x4 v = {};
+    // Results (row m, columns n ..), four neighbours a thread.  t B^T is shared out as items (row, column, chunk of ranks): a thread
+    // keeps its column and chunk and walks the rows, four loads at a time; the items' sums go where the partial sums were.
+    const int chunks = (op.rank + CE - 1) / CE, per = 16 * NT * chunks;
+    const int wide = per <= NTH ? NTH / per : 1;   // rows at a time
+    const bool items = op.rows * per * 4 <= (int)skinny_lds<MT, NT, FJ>();
+    constexpr int QN = (TILES * 64 + NTH - 1) / NTH;
+    f32x4 v[QN];
 #pragma unroll
-        for (int s = 0; s < NW; s++) v += red[(s * (TILES + FJ) + q / 64) * 64 + q % 64];
-        return v;
-    };
-    auto finish = [&](int q, f32x4 v, auto term) {
-        const int tile = q / 64, l = q % 64, m = (tile % MT) * 16 + (l & 15), nl = (tile / MT) * 16 + (l >> 4) * 4;
-        if (m >= op.rows || n0 + nl >= op.N) return;
-        const int i = adapter_of(op, m);
+    for (int k = 0; k < QN; k++) {
+        const int q = tid + k * NTH;
+        v[k] = f32x4{};
+        if (q < TILES * 64)
+#pragma unroll
+            for (int s = 0; s < NW; s++) v[k] += red[(s * (TILES + FJ) + q / 64) * 64 + q % 64];
+    }
+    __syncthreads();
+    float* ex = reinterpret_cast<float*>(smem);   // [row][column][chunk]
+    if (items) {
+        const int m0 = per <= NTH ? tid / per : 0;
+        for (int it = per <= NTH ? tid % per : tid; it < per && m0 < wide; it += per <= NTH ? per : NTH) {
+            const int c = it % chunks, n = it / chunks;
+            const long long at = (long long)min(n0 + n, op.N - 1) * op.rank;
+            for (int m = m0; m < op.rows; m += 4 * wide) {
+                u32x4 b[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int i = max(adapter[min(m + u * wide, op.rows - 1)], 0);
+                    b[u] = load_chunk(static_cast<const T*>(op.b) + (long long)i * op.N * op.rank + at, c * CE, op.rank);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (m + u * wide < op.rows) ex[(m + u * wide) * per + it] = dot_chunk<T>(tl + (m + u * wide) * rp + c * CE, b[u]);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < QN; k++) {
+        const int q = tid + k * NTH, tile = q / 64, l = q % 64, m = (tile % MT) * 16 + (l & 15), nl = (tile / MT) * 16 + (l >> 4) * 4;
+        if (q >= TILES * 64 || m >= op.rows || n0 + nl >= op.N) continue;
+        const int i = adapter[m];
         if (i >= 0) {
             const float sc = op.scale ? op.scale[i] : 1.f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = fmaf(sc, term(m, nl + e, i), v[e]);
+            for (int e = 0; e < 4; e++) {
+                float d = 0;
+                if (items) {
+                    for (int c = 0; c < chunks; c++) d += ex[m * per + (nl + e) * chunks + c];
+                } else {
+                    const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + min(n0 + nl + e, op.N - 1)) * op.rank;
+                    for (int r = 0; r < op.rank; r += CE) d += dot_chunk<T>(tl + m * rp + r, load_chunk(b, r, op.rank));
+                }
+                v[k][e] = fmaf(sc, d, v[k][e]);
+            }
         } else if (i == kForeign) {
-            v = f32x4{NAN, NAN, NAN, NAN};
+            v[k] = f32x4{NAN, NAN, NAN, NAN};
         }
-        store4<T>(op, m, n0 + nl, v);
-    };
-    if (spread) {
-        f32x4 v = {};
-        if (tid < TILES * 64) v = total(tid);
-        __syncthreads();
-        float* ex = reinterpret_cast<float*>(smem);   // [item], where the partial sums were
-        for (int it = tid; it < items; it += NTH) {
-            const u32x4 c = it == tid ? b0 : b_chunk(it);
-            ex[it] = dot_chunk<T>(tl + it / chunks / (16 * NT) * rp + it % chunks * CE, c);
-        }
-        __syncthreads();
-        if (tid < TILES * 64)
-            finish(tid, v, [&](int m, int n, int) {
-                float d = 0;
-                for (int c = 0; c < chunks; c++) d += ex[(m * 16 * NT + n) * chunks + c];
-                return d;
-            });
-    } else {
-        __syncthreads();
-        for (int q = tid; q < TILES * 64; q += NTH)
-            finish(q, total(q), [&](int m, int n, int i) {
-                const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + min(n0 + n, op.N - 1)) * op.rank;
-                float d = 0;
-                for (int r = 0; r < op.rank; r += CE) d += dot_chunk<T>(tl + m * rp + r, load_chunk(b, r, op.rank));
-                return d;
-            });
+        store4<T>(op, m, n0 + nl, v[k]);
     }
 }
 
@@ -430,7 +490,7 @@ template <int BM>
 constexpr int kOrderBytes = 4 * BM * (int)sizeof(int);
 
 template <typename T, int BM, int BN, int WM, int WN, bool DMA>
-__global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float* part, int splits) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const float* part, int splits) {
     constexpr int CE = kChunk<T>, NW = WM * WN, NTH = 64 * NW, MI = BM / WM / 16, NI = BN / WN / 16;
     constexpr int STAGE = (int)tile_stage_bytes<BM, BN>();
     extern __shared__ __attribute__((aligned(16))) char lds[];   // (all of it dynamic: the opt-in covers 160 KiB of that)
@@ -449,14 +509,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
     const int group = tile / (G * ntn), gm = min(G, ntm - group * G), in = tile - group * G * ntn;
     const int m0 = (group * G + in % gm) * BM, n0 = in / gm * BN;
     const int count = min(BM, op.rows - m0);
-    order_rows<BM>(op, m0, count, raw, order, key, nth);
+    order_rows<BM, NTH, false>(op, m0, count, raw, order, key, nth);
 
     const T* xb = static_cast<const T*>(op.x) + m0 * op.x_stride;
     const T* wb = static_cast<const T*>(op.w) + n0 * op.w_stride;
     f32x4 acc[NI][MI] = {};
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
-    auto compute = [&](const char* st) {
-        u32x4 fx[MI], fw[NI];
+    const auto read = [&](const char* st, u32x4 (&fx)[MI], u32x4 (&fw)[NI]) {
 #pragma unroll
         for (int j = 0; j < MI; j++) {
             const int r = wm + j * 16 + lr;
@@ -467,10 +526,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
             const int r = wn + i * 16 + lr;
             fw[i] = *reinterpret_cast<const u32x4*>(st + (BM + r) * 64 + ((kq ^ (r >> 1 & 3)) << 4));
         }
+    };
+    const auto multiply = [&](const u32x4 (&fx)[MI], const u32x4 (&fw)[NI]) {
 #pragma unroll
         for (int i = 0; i < NI; i++)
 #pragma unroll
             for (int j = 0; j < MI; j++) acc[i][j] = mma<T>(fw[i], fx[j], acc[i][j]);
+    };
+    const auto compute = [&](const char* st) {
+        u32x4 fx[MI], fw[NI];
+        read(st, fx, fw);
+        multiply(fx, fw);
     };
     constexpr int LX = BM / 16 / NW, LW = BN / 16 / NW;   // 16-row pieces of each operand that a wave brings
     static_assert(LX * NW * 16 == BM && LW * NW * 16 == BN, "pieces");
@@ -506,16 +572,39 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
         };
         constexpr int PER = LX + LW;
         const int full = op.K / (4 * CE);
-#pragma unroll
-        for (int s = 0; s < kRing - 1; s++)
-            if (s < full) issue(s);
-        for (int s = 0; s < full; s++) {
-            // this wave's loads of stage s have arrived (those of the next two may be in flight), then everyone's
-            if (s + 2 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER) : "memory");
-            else if (s + 1 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER) : "memory");
+        // stage s + 1 has arrived in this wave's share (those behind it may be in flight) and this wave has read stage s; then
+        // everyone's
+        const auto arrive = [&](int s) {
+            if (s + 3 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER) : "memory");
+            else if (s + 2 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (s + kRing - 1 < full) issue(s + kRing - 1);   // into the slot of stage s - 1, which everyone has left
-            compute(smem + (s % kRing) * STAGE);
+        };
+        // While the matrix instructions work on stage s from registers, stage s + 1 is read from LDS and stage s + 4 goes where
+        // stage s was.
+        u32x4 fx[2][MI], fw[2][NI];
+        const auto step = [&](int s, u32x4 (&cx)[MI], u32x4 (&cw)[NI], u32x4 (&nx)[MI], u32x4 (&nw)[NI]) {
+            arrive(s);
+            if (s + kRing < full) issue(s + kRing);
+            if (s + 1 < full) read(smem + ((s + 1) % kRing) * STAGE, nx, nw);
+            multiply(cx, cw);
+#pragma unroll
+            for (int g = 0; g < MI + NI; g++) {   // an LDS read between every few matrix instructions
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, MI * NI * (sizeof(T) == 4 ? 4 : 1) / (MI + NI), 0);
+            }
+        };
+        if (full > 0) {
+#pragma unroll
+            for (int s = 0; s < kRing; s++)
+                if (s < full) issue(s);
+            // (stage 0 of `arrive(-1)`: the ring holds one stage more than from then on)
+            if (full >= kRing) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * PER) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            read(smem, fx[0], fw[0]);
+            for (int s = 0; s < full; s += 2) {
+                step(s, fx[0], fw[0], fx[1], fw[1]);
+                if (s + 1 < full) step(s + 1, fx[1], fw[1], fx[0], fw[0]);
+            }
         }
     }
     {
@@ -526,15 +615,23 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
         for (int i = 0; i < LX; i++) px[i] = xb + min(order[(wave * LX + i) * 16 + (lane >> 2)], count - 1) * op.x_stride;
 #pragma unroll
         for (int i = 0; i < LW; i++) pw[i] = wb + min((wave * LW + i) * 16 + (lane >> 2), op.N - 1 - n0) * op.w_stride;
-        u32x4 vx[LX], vw[LW];
-        auto fetch = [&](int s) {
+        constexpr int D = BM == 64 ? 4 : 2;   // stages on their way
+        u32x4 vx[D][LX], vw[D][LW];
+        const auto fetch = [&](int s, u32x4 (&vx)[LX], u32x4 (&vw)[LW]) {
             const int k = s * 4 * CE + slot * CE;
+            if ((s + 1) * 4 * CE <= op.K) {
 #pragma unroll
-            for (int i = 0; i < LX; i++) vx[i] = load_chunk(px[i], k, op.K);
+                for (int i = 0; i < LX; i++) vx[i] = load16(px[i] + k);
 #pragma unroll
-            for (int i = 0; i < LW; i++) vw[i] = load_chunk(pw[i], k, op.K);
+                for (int i = 0; i < LW; i++) vw[i] = load16(pw[i] + k);
+            } else if (s < last) {
+#pragma unroll
+                for (int i = 0; i < LX; i++) vx[i] = load_chunk(px[i], k, op.K);
+#pragma unroll
+                for (int i = 0; i < LW; i++) vw[i] = load_chunk(pw[i], k, op.K);
+            }
         };
-        auto put = [&](char* st) {
+        const auto put = [&](char* st, const u32x4 (&vx)[LX], const u32x4 (&vw)[LW]) {
 #pragma unroll
             for (int i = 0; i < LX; i++) {
                 const int r = (wave * LX + i) * 16 + (lane >> 2);
@@ -547,15 +644,22 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
             }
         };
         if (first < last) {
-            fetch(first);
+#pragma unroll
+            for (int d = 0; d < D; d++) fetch(first + d, vx[d], vw[d]);
             if (DMA) __syncthreads();   // the ring has been read
-            put(smem);
-        }
-        for (int s = first; s < last; s++) {
-            if (s + 1 < last) fetch(s + 1);
-            __syncthreads();            // stage s is there, and stage s - 1 has been read
-            compute(smem + ((s - first) & 1) * STAGE);
-            if (s + 1 < last) put(smem + ((s + 1 - first) & 1) * STAGE);
+            put(smem, vx[0], vw[0]);
+            fetch(first + D, vx[0], vw[0]);
+            for (int s = first; s < last; s += D)
+#pragma unroll
+                for (int d = 0; d < D; d++)
+                    if (s + d < last) {
+                        __syncthreads();        // stage s + d is there, and the one before it has been read
+                        compute(smem + (d & 1) * STAGE);
+                        if (s + d + 1 < last) {
+                            put(smem + ((d + 1) & 1) * STAGE, vx[(d + 1) % D], vw[(d + 1) % D]);
+                            fetch(s + d + 1 + D, vx[(d + 1) % D], vw[(d + 1) % D]);
+                        }
+                    }
         }
     }
 
@@ -570,10 +674,36 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
         *reinterpret_cast<f32x4*>(tl + p * ts + r) = v;
     }
     __syncthreads();
-    int em = 0;   // fp16: t scaled into [0.5, 1) by a power of two per row
-#pragma unroll
-    for (int j = 0; j < MI; j++) {
+    // With few rows per adapter (by the numbers of both, not by the data: the two ways round differently, and a row's result must
+    // not depend on its neighbours) every lane takes the B of its own row; else the matrix instructions take 16 rows at a time.
+    const bool per_row = op.rank <= 32 && BM < 8 * op.adapters;
+    const auto finish = [&](auto J) __attribute__((always_inline)) {
+        constexpr int j = J.value;
         const int p = wm + j * 16 + lr, mine = key[p];
+        if (per_row && mine >= 0) {
+            const float sc = op.scale ? op.scale[mine] : 1.f;
+            f32x4 d[NI] = {};
+            for (int r = 0; r < op.rank; r += CE) {
+                float t[CE];
+#pragma unroll
+                for (int k = 0; k < CE; k++) t[k] = tl[p * ts + r + k];
+#pragma unroll
+                for (int ni = 0; ni < NI; ni++) {
+                    u32x4 c[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int n = min(n0 + wn + ni * 16 + kq * 4 + e, op.N - 1);
+                        c[e] = load_chunk(static_cast<const T*>(op.b) + ((long long)mine * op.N + n) * op.rank, r, op.rank);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) d[ni][e] += dot_chunk<T>(t, c[e]);
+                }
+            }
+#pragma unroll
+            for (int ni = 0; ni < NI; ni++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[ni][j][e] = fmaf(sc, d[ni][e], acc[ni][j][e]);
+        }
         float back = 1.f, to = 1.f;
         if constexpr (__is_same(T, _Float16)) {
             float mx = 0;
@@ -582,12 +712,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
                 for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(tl[p * ts + r + e]));
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            em = mx > 0 && mx < INFINITY ? max(-100, min(100, ilogbf(mx) + 1)) : 0;
+            // scaled into [0.5, 1) by a power of two
+            const int em = mx > 0 && mx < INFINITY ? max(-100, min(100, ilogbf(mx) + 1)) : 0;
             back = ldexpf(1.f, em);
             to = ldexpf(1.f, -em);
         }
         // per adapter among the 16 rows
-        unsigned long long todo = __ballot(mine >= 0);
+        unsigned long long todo = __ballot(mine >= 0 && !per_row);
         while (todo) {
             const int i = __shfl(mine, __ffsll(todo) - 1);
             const bool use = mine == i;
@@ -641,7 +772,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tile(AdapterOp op, const float
                 if (n < op.N) store4<T>(op, m, n, mine == kForeign ? f32x4{NAN, NAN, NAN, NAN} : acc[ni][j]);
             }
         }
-    }
+    };
+    static_for(finish, std::make_integer_sequence<int, MI>{});
 }
 
 // ---- launch ------------------------------------------------------------------------------------------------------------------
@@ -684,7 +816,7 @@ Plan make_plan(const AdapterOp& op) {
 
 template <typename T, int MT, int NT, int FJ>
 void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
-    const size_t lds = skinny_lds<MT, NT, FJ>() + (size_t)op.rows * padded_rank(op.rank) * 4;
+    const size_t lds = skinny_lds<MT, NT, FJ>() + 16 * MT * 4 + (size_t)op.rows * padded_rank(op.rank) * 4;
     lds_optin((const void*)k_skinny<T, MT, NT, FJ>);
     k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT)), dim3(64 * kSkinnyWaves<MT>), lds, st>>>(op, part, splits);
 }
