@@ -355,6 +355,23 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
         const int m = min(j / rt, op.rows - 1), i = max(adapter_of(op, m), 0);   // of none: some A, its t is not used
         a[j] = static_cast<const T*>(op.a) + ((long long)i * op.rank + min((j % rt) * 16 + lr, op.rank - 1)) * op.K + kq * CE;
     }
+    // t B^T is shared out as items (row, column, chunk of ranks): a thread keeps its column and chunk and walks the rows
+    const int chunks = (op.rank + CE - 1) / CE, per = 16 * NT * chunks;
+    const int wide = per <= NTH ? NTH / per : 1;   // rows at a time
+    const bool items = op.rows * per * 4 <= (int)skinny_lds<MT, NT, FJ>();
+    const int im0 = per <= NTH ? tid / per : 0, it0 = per <= NTH ? tid % per : tid;
+    const auto b_chunk = [&](int m, int it) {
+        const int i = max(adapter_of(op, min(m, op.rows - 1)), 0);
+        return load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + min(n0 + it / chunks, op.N - 1)) * op.rank, it % chunks * CE, op.rank);
+    };
+    u32x4 b0 = {0, 0, 0, 0};
+    if (items && im0 < wide && it0 < per) b0 = b_chunk(im0, it0);
+    if (!FJ) {
+        for (int q = tid; q < op.rows * (rp / 4); q += NTH) {
+            const int m = q / (rp / 4), r = q % (rp / 4) * 4;
+            *reinterpret_cast<f32x4*>(tl + m * rp + r) = sum_parts(part, splits, op.rows, m, rp, r);
+        }
+    }
     while (more()) {
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -399,12 +416,6 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
         for (int j = 0; j < MT; j++) red[(wave * (TILES + FJ) + i * MT + j) * 64 + lane] = acc[i][j];
 #pragma unroll
     for (int j = 0; j < FJ; j++) red[(wave * (TILES + FJ) + TILES + j) * 64 + lane] = ta[j];
-    if (!FJ) {
-        for (int q = tid; q < op.rows * (rp / 4); q += NTH) {
-            const int m = q / (rp / 4), r = q % (rp / 4) * 4;
-            *reinterpret_cast<f32x4*>(tl + m * rp + r) = sum_parts(part, splits, op.rows, m, rp, r);
-        }
-    }
     __syncthreads();
     if (FJ) {   // column m of job (m, rank tile) holds t[m]
         for (int q = tid; q < op.rows * rp; q += NTH) {
@@ -415,11 +426,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
             tl[m * rp + r] = r < op.rank ? v : 0.f;
         }
     }
-    // Results (row m, columns n ..), four neighbours a thread.  t B^T is shared out as items (row, column, chunk of ranks): a thread
-    // keeps its column and chunk and walks the rows, four loads at a time; the items' sums go where the partial sums were.
-    const int chunks = (op.rank + CE - 1) / CE, per = 16 * NT * chunks;
-    const int wide = per <= NTH ? NTH / per : 1;   // rows at a time
-    const bool items = op.rows * per * 4 <= (int)skinny_lds<MT, NT, FJ>();
+    // results (row m, columns n ..), four neighbours a thread; the items' sums go where the partial sums were
     constexpr int QN = (TILES * 64 + NTH - 1) / NTH;
     f32x4 v[QN];
 #pragma unroll
@@ -433,19 +440,20 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
     __syncthreads();
     float* ex = reinterpret_cast<float*>(smem);   // [row][column][chunk]
     if (items) {
-        const int m0 = per <= NTH ? tid / per : 0;
-        for (int it = per <= NTH ? tid % per : tid; it < per && m0 < wide; it += per <= NTH ? per : NTH) {
+        constexpr int BATCH = 8;
+        for (int it = it0; it < per && im0 < wide; it += per <= NTH ? per : NTH) {
             const int c = it % chunks, n = it / chunks;
             const long long at = (long long)min(n0 + n, op.N - 1) * op.rank;
-            for (int m = m0; m < op.rows; m += 4 * wide) {
-                u32x4 b[4];
+            for (int m = im0; m < op.rows; m += BATCH * wide) {
+                u32x4 b[BATCH];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
+                for (int u = 0; u < BATCH; u++) {
                     const int i = max(adapter[min(m + u * wide, op.rows - 1)], 0);
-                    b[u] = load_chunk(static_cast<const T*>(op.b) + (long long)i * op.N * op.rank + at, c * CE, op.rank);
+                    if (u == 0 && m == im0 && it == it0) b[u] = b0;
+                    else if (m + u * wide < op.rows) b[u] = load_chunk(static_cast<const T*>(op.b) + (long long)i * op.N * op.rank + at, c * CE, op.rank);
                 }
 #pragma unroll
-                for (int u = 0; u < 4; u++)
+                for (int u = 0; u < BATCH; u++)
                     if (m + u * wide < op.rows) ex[(m + u * wide) * per + it] = dot_chunk<T>(tl + (m + u * wide) * rp + c * CE, b[u]);
             }
         }
@@ -609,28 +617,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
     }
     {
         // through registers: all of K without DMA, what is left of a stage with it
-        const int first = DMA ? op.K / (4 * CE) : 0, last = (op.K + 4 * CE - 1) / (4 * CE);
         const T *px[LX], *pw[LW];
 #pragma unroll
-        for (int i = 0; i < LX; i++) px[i] = xb + min(order[(wave * LX + i) * 16 + (lane >> 2)], count - 1) * op.x_stride;
+        for (int i = 0; i < LX; i++) px[i] = xb + min(order[(wave * LX + i) * 16 + (lane >> 2)], count - 1) * op.x_stride + slot * CE;
 #pragma unroll
-        for (int i = 0; i < LW; i++) pw[i] = wb + min((wave * LW + i) * 16 + (lane >> 2), op.N - 1 - n0) * op.w_stride;
-        constexpr int D = BM == 64 ? 4 : 2;   // stages on their way
-        u32x4 vx[D][LX], vw[D][LW];
-        const auto fetch = [&](int s, u32x4 (&vx)[LX], u32x4 (&vw)[LW]) {
-            const int k = s * 4 * CE + slot * CE;
-            if ((s + 1) * 4 * CE <= op.K) {
-#pragma unroll
-                for (int i = 0; i < LX; i++) vx[i] = load16(px[i] + k);
-#pragma unroll
-                for (int i = 0; i < LW; i++) vw[i] = load16(pw[i] + k);
-            } else if (s < last) {
-#pragma unroll
-                for (int i = 0; i < LX; i++) vx[i] = load_chunk(px[i], k, op.K);
-#pragma unroll
-                for (int i = 0; i < LW; i++) vw[i] = load_chunk(pw[i], k, op.K);
-            }
-        };
+        for (int i = 0; i < LW; i++) pw[i] = wb + min((wave * LW + i) * 16 + (lane >> 2), op.N - 1 - n0) * op.w_stride + slot * CE;
         const auto put = [&](char* st, const u32x4 (&vx)[LX], const u32x4 (&vw)[LW]) {
 #pragma unroll
             for (int i = 0; i < LX; i++) {
@@ -643,23 +634,41 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
                 *reinterpret_cast<u32x4*>(st + (BM + r) * 64 + ((slot ^ (r >> 1 & 3)) << 4)) = vw[i];
             }
         };
-        if (first < last) {
+        const int full = op.K / (4 * CE);
+        if (!DMA && full > 0) {
+            constexpr int D = BM == 64 ? 4 : 2;   // stages on their way; behind the last whole one: that one again
+            u32x4 vx[D][LX], vw[D][LW];
+            const auto fetch = [&](int s, u32x4 (&vx)[LX], u32x4 (&vw)[LW]) {
+                const int k = min(s, full - 1) * 4 * CE;
 #pragma unroll
-            for (int d = 0; d < D; d++) fetch(first + d, vx[d], vw[d]);
-            if (DMA) __syncthreads();   // the ring has been read
-            put(smem, vx[0], vw[0]);
-            fetch(first + D, vx[0], vw[0]);
-            for (int s = first; s < last; s += D)
+                for (int i = 0; i < LX; i++) vx[i] = load16(px[i] + k);
 #pragma unroll
-                for (int d = 0; d < D; d++)
-                    if (s + d < last) {
-                        __syncthreads();        // stage s + d is there, and the one before it has been read
-                        compute(smem + (d & 1) * STAGE);
-                        if (s + d + 1 < last) {
-                            put(smem + ((d + 1) & 1) * STAGE, vx[(d + 1) % D], vw[(d + 1) % D]);
-                            fetch(s + d + 1 + D, vx[(d + 1) % D], vw[(d + 1) % D]);
-                        }
-                    }
+                for (int i = 0; i < LW; i++) vw[i] = load16(pw[i] + k);
+            };
+#pragma unroll
+            for (int d = 0; d < D; d++) fetch(d, vx[d], vw[d]);
+            for (int s = 0; s < full; s += D)
+#pragma unroll
+                for (int d = 0; d < D; d++) {
+                    // (a step behind the last stage only turns the barrier)
+                    put(smem + (d & 1) * STAGE, vx[d], vw[d]);
+                    fetch(s + d + D, vx[d], vw[d]);
+                    // the fetches stay in flight over the barrier; LDS: the slot that is written next was read a step ago
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (s + d < full) compute(smem + (d & 1) * STAGE);
+                }
+        }
+        if (full * 4 * CE < op.K) {
+            u32x4 vx[LX], vw[LW];
+            const int k = full * 4 * CE, left = op.K - slot * CE;
+#pragma unroll
+            for (int i = 0; i < LX; i++) vx[i] = load_chunk(px[i], k, left);
+#pragma unroll
+            for (int i = 0; i < LW; i++) vw[i] = load_chunk(pw[i], k, left);
+            __syncthreads();   // the stages before have been read
+            put(smem, vx, vw);
+            __syncthreads();
+            compute(smem);
         }
     }
 
@@ -677,7 +686,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
     // With few rows per adapter (by the numbers of both, not by the data: the two ways round differently, and a row's result must
     // not depend on its neighbours) every lane takes the B of its own row; else the matrix instructions take 16 rows at a time.
     const bool per_row = op.rank <= 32 && BM < 8 * op.adapters;
-    const auto finish = [&](auto J) __attribute__((always_inline)) {
+    const auto add_term = [&](auto J) __attribute__((always_inline)) {
         constexpr int j = J.value;
         const int p = wm + j * 16 + lr, mine = key[p];
         if (per_row && mine >= 0) {
@@ -748,13 +757,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
 #pragma unroll
                 for (int ni = 0; ni < NI; ni++) {
                     const int n = min(n0 + wn + ni * 16 + lr, op.N - 1);
-                    const T* b = static_cast<const T*>(op.b) + ((long long)i * op.N + n) * op.rank;
-                    u32x4 fb = load_chunk(b, rb, op.rank);
+                    u32x4 v = load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + n) * op.rank, rb, op.rank);
                     if constexpr (sizeof(T) == 2) {
                         // an inf of B times the rest of t, which may have the other sign, is not wanted beside inf times its leading part
-                        if (kq >= 2) fb = finite_only<T>(fb);
+                        if (kq >= 2) v = finite_only<T>(v);
                     }
-                    d[ni] = mma<T>(fb, ft, d[ni]);
+                    d[ni] = mma<T>(v, ft, d[ni]);
                 }
             }
             if (use) {
@@ -764,8 +772,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
                     for (int e = 0; e < 4; e++) acc[ni][j][e] = fmaf(sc, d[ni][e], acc[ni][j][e]);
             }
         }
+    };
+    static_for(add_term, std::make_integer_sequence<int, MI>{});
+    // (stores last: a load behind a store would wait for it)
+    const auto store = [&](auto J) __attribute__((always_inline)) {
+        constexpr int j = J.value;
+        const int p = wm + j * 16 + lr;
         if (p < count) {
-            const int m = m0 + order[p];
+            const int m = m0 + order[p], mine = key[p];
 #pragma unroll
             for (int ni = 0; ni < NI; ni++) {
                 const int n = n0 + wn + ni * 16 + kq * 4;
@@ -773,7 +787,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
             }
         }
     };
-    static_for(finish, std::make_integer_sequence<int, MI>{});
+    static_for(store, std::make_integer_sequence<int, MI>{});
 }
 
 // ---- launch ------------------------------------------------------------------------------------------------------------------
