@@ -176,9 +176,11 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
 
 // ---- t = x A^T -------------------------------------------------------------------------------------------------------------
 // Workgroup (block of BR rows, part of K): jobs of up to 16 rows of one adapter, a wave each.  part[s][row][padded rank].
-// 16 rows: a wave for every job there can be; 128 rows: 8 waves, as many as 8 rank tiles leave registers for.
+// 16 rows: a wave for every job there can be, in 4 workgroups; 128 rows: 8 waves, as many as 8 rank tiles leave registers for.
 template <int BR>
-constexpr int kShrinkWaves = BR == 16 ? 16 : 8;
+constexpr int kShrinkWaves = BR == 16 ? 4 : 8;
+template <int BR>
+constexpr int kShrinkParts = BR == 16 ? 4 : 1;   // workgroups that share the jobs of a block
 template <typename T, int RT, int BR>
 __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, float* part, int splits) {
     constexpr int CE = kChunk<T>;
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, 
     const int pairs = (op.K + 8 * CE - 1) / (8 * CE);           // 128-byte steps of k
     const int p0 = (int)((long long)pairs * split / splits), p1 = (int)((long long)pairs * (split + 1) / splits);
     const int pf = min(p1, op.K / (8 * CE));                    // whole ones
-    for (int j = wave; j < jobs; j += kShrinkWaves<BR>) {
+    for (int j = wave + kShrinkWaves<BR> * blockIdx.z; j < jobs; j += kShrinkWaves<BR> * kShrinkParts<BR>) {
         const int at = job[j], i = key[at], p = at + lr;
         const bool mine = p < count && key[p] == i;
         const int m = m0 + order[mine ? p : at];
@@ -644,6 +646,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
                 for (int i = 0; i < LX; i++) vx[i] = load16(px[i] + k);
 #pragma unroll
                 for (int i = 0; i < LW; i++) vw[i] = load16(pw[i] + k);
+                __builtin_amdgcn_sched_barrier(0);   // loads in the order of the stages: the waits count them
             };
 #pragma unroll
             for (int d = 0; d < D; d++) fetch(d, vx[d], vw[d]);
@@ -858,7 +861,7 @@ void launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int spl
 template <typename T, int BR>
 void launch_shrink(hipStream_t st, const AdapterOp& op, float* part, int splits) {
     constexpr int NTH = 64 * kShrinkWaves<BR>;
-    const dim3 grid((op.rows + BR - 1) / BR, splits);
+    const dim3 grid((op.rows + BR - 1) / BR, splits, kShrinkParts<BR>);
     const int rt = padded_rank(op.rank) / 16;
     if (rt == 1) k_shrink<T, 1, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
     else if (rt == 2) k_shrink<T, 2, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
