@@ -201,6 +201,35 @@ int mz_seed_gumbel(mz_ctx* ctx, uint64_t seed, uint64_t move_counter);
  * recorded reference noise vector n is replayed as dirichlet[order[j]] = n[j].  Pure host function, ctx may be NULL. */
 int mz_child_order(const uint8_t* legal /* [A] */, int A, int32_t* order /* [A] */);
 
+/* ---- raw-policy moves: justInitialInferencePolicy for B games in lock-step -----------------------
+ * (P/agent/c_planning/PlanAction.java:85-87,174-193: initial inference, the move drawn from the policy over the legal
+ *  actions.)  Here the draw takes temperature, top-k, top-p and min-p (mz_sample_args has the definition; the defaults
+ *  1, 0, 1, 0 draw from the renormalised policy), and each game may play with a low-rank adapter of its own on the policy
+ *  head's last linear, so that a population of players or fine-tuned opponents shares one network in one batch:
+ *      logits[g] = W f_g + bias + scale[i] * B[i] (A[i] f_g),  i = adapter[g]   (mz_adapter_args has the definition)
+ *  f_g the head's 2 * height * width features, W and bias the network's pred.p.fc as last loaded or committed.
+ *  mz_load_policy_adapters replaces the context's adapters: a [n][rank][2 * height * width], b [n][action_space][rank],
+ *  scale [n] or NULL (1), fp32, copied; n = 0 removes them.  They stay when weights are loaded or broadcast.
+ *  mz_play_policy: B <= max_games; obs, legal as for mz_search_moves; adapter [B] (-1: the network's own head) or NULL (all);
+ *  u [B]; any output pointer may be NULL; action -1 for a game without a legal action.  Uses the roots' hidden-state slots, so
+ *  trees of an earlier search keep their statistics but cannot be continued. */
+typedef struct mz_policy_sampling {
+    double temperature, top_p, min_p;
+    int32_t top_k;
+    int32_t reserved0;
+} mz_policy_sampling;
+typedef struct mz_policy_outputs {
+    int32_t* action;        /* [B] */
+    float* logprob;         /* [B] of the drawn action in the playout policy */
+    int32_t* kept;          /* [B] actions the filters kept */
+    float* playout_policy;  /* [B*A] the distribution the action was drawn from (GameDTO.playoutPolicy) */
+    float* logits;          /* [B*A] NetworkIO.logits, with the adapters */
+    double* value;          /* [B] */
+} mz_policy_outputs;
+int mz_load_policy_adapters(mz_ctx* ctx, int n, int rank, const float* a, const float* b, const float* scale);
+int mz_play_policy(mz_ctx* ctx, int B, const float* obs, const uint8_t* legal, const int32_t* adapter,
+                   const mz_policy_sampling* sampling, const double* u, const mz_policy_outputs* out);
+
 /* ---- introspection: Game.getSearchManager().getRoot() / Node getters (GumbelSearch.java:37,
  * Node.java:48-78; used by renderers TicTacToeGame.java:192-206, GoGame.java:186-204) --------------
  * Expanded node `slot` (0 = root, s+1 = leaf of simulation s) of game g after the last move search.

@@ -64,6 +64,15 @@ class AdapterArgs(C.Structure):
                 ("y", C.c_void_p), ("y_stride", C.c_int64)]
 
 
+class PolicySampling(C.Structure):
+    _fields_ = [("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", C.c_int32),
+                ("reserved0", C.c_int32)]
+
+
+class PolicyOutputs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("action", "logprob", "kept", "playout_policy", "logits", "value")]
+
+
 EXPORTS = (
     "mz_create", "mz_destroy", "mz_last_error", "mz_set_action_cells", "mz_load_weights", "mz_num_params",
     "mz_weights_device_ptr", "mz_commit_weights", "mz_initial_inference", "mz_recurrent_inference",
@@ -72,7 +81,7 @@ EXPORTS = (
     "mz_synchronize", "mz_version", "mz_comm_unique_id", "mz_comm_init", "mz_comm_destroy", "mz_broadcast_weights",
     "mz_gather_stats", "mz_comm_barrier", "mz_get_recording_games", "mz_get_gumbel", "mz_seed_gumbel",
     "mz_child_order", "mz_noalloc_scratch_bytes", "mz_search_moves_injected_noalloc", "mz_set_stream_split",
-    "mz_sample_workspace_bytes", "mz_sample_actions", "mz_adapter_workspace_bytes", "mz_adapter_linear")
+    "mz_sample_workspace_bytes", "mz_sample_actions", "mz_adapter_workspace_bytes", "mz_adapter_linear", "mz_load_policy_adapters", "mz_play_policy")
 NOALLOC_SCRATCH_BYTES = 16 << 20
 COMM_ID_BYTES = 128
 
@@ -127,6 +136,8 @@ def lib():
         L.mz_noalloc_scratch_bytes.argtypes = [vp, C.c_int]
         L.mz_noalloc_scratch_bytes.restype = C.c_size_t
         L.mz_search_moves_injected_noalloc.argtypes = L.mz_search_moves_injected.argtypes
+        L.mz_load_policy_adapters.argtypes = [vp, C.c_int, C.c_int, vp, vp, vp]
+        L.mz_play_policy.argtypes = [vp, C.c_int, vp, vp, vp, C.POINTER(PolicySampling), vp, C.POINTER(PolicyOutputs)]
         L.mz_sample_workspace_bytes.argtypes = [C.POINTER(SampleArgs)]
         L.mz_sample_workspace_bytes.restype = C.c_size_t
         L.mz_sample_actions.argtypes = [C.POINTER(SampleArgs), vp, C.c_size_t, vp]
@@ -286,6 +297,37 @@ class Context:
         out = np.empty((n.channels, n.height, n.width), np.float32)
         self._check(lib().mz_read_hidden(self._h, int(slot), _ptr(out)))
         return out
+
+    # --- raw-policy moves (justInitialInferencePolicy, PlanAction.java:174-193) --------------------
+    def load_policy_adapters(self, a=None, b=None, scale=None):
+        """a [n, rank, 2 * H * W], b [n, A, rank], scale [n] or None, fp32: low-rank adapters of the policy head's last linear
+        for play_policy.  No arguments: none."""
+        if a is None:
+            self._check(lib().mz_load_policy_adapters(self._h, 0, 0, None, None, None))
+            return
+        a, b, scale = _np(a, np.float32), _np(b, np.float32), _np(scale, np.float32)
+        n, rank, hw = a.shape
+        if hw != 2 * self.cfg.net.height * self.cfg.net.width or tuple(b.shape) != (n, self.A, rank):
+            raise MuZeroError("a must be [n, rank, 2 * height * width] and b [n, action_space, rank]")
+        if scale is not None and tuple(scale.shape) != (n,):
+            raise MuZeroError("scale must be [n]")
+        for v in (a, b, scale):
+            if v is not None and not isinstance(v, np.ndarray) and "float32" not in str(v.dtype):
+                raise MuZeroError("adapters must be float32")
+        self._check(lib().mz_load_policy_adapters(self._h, n, rank, _ptr(a), _ptr(b), _ptr(scale)))
+
+    def play_policy(self, B, obs, legal, u, adapter=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, outputs=None):
+        """One raw-policy move per game.  outputs: dict of preallocated numpy arrays / torch CUDA tensors (any subset of
+        action, logprob, kept, playout_policy, logits, value), or None for numpy arrays of everything."""
+        A = self.A
+        o = dict(action=np.empty(B, np.int32), logprob=np.empty(B, np.float32), kept=np.empty(B, np.int32),
+                 playout_policy=np.empty((B, A), np.float32), logits=np.empty((B, A), np.float32),
+                 value=np.empty(B, np.float64)) if outputs is None else outputs
+        po = PolicyOutputs(*[_ptr(o.get(name)) for name, _ in PolicyOutputs._fields_])
+        s = PolicySampling(temperature, top_p, min_p, top_k, 0)
+        self._check(lib().mz_play_policy(self._h, B, _ptr(_np(obs, np.float32)), _ptr(_np(legal, np.uint8)),
+                                         _ptr(_np(adapter, np.int32)), C.byref(s), _ptr(_np(u, np.float64)), C.byref(po)))
+        return o
 
     # --- move level (PlanAction.planAction for B games) -------------------------------------------
     def _alloc_outputs(self, B):

@@ -132,6 +132,10 @@ struct mz_ctx {
     size_t comm_buf_count = 0;
     // device outputs
     DeviceMoveOutputs dout{};
+    // raw-policy moves (mz_play_policy): adapters of the policy head, its features and adapted logits, operator workspaces
+    int ad_n = 0, ad_rank = 0;
+    bool ad_scaled = false;
+    DevBuf ad_a, ad_b, ad_scale, pol_feat, pol_logits, pol_ws;
     // timing
     bool timing = false;
     std::vector<EventPair> events;
@@ -237,6 +241,16 @@ int stage_out(mz_ctx* ctx, size_t slot, void* user, size_t bytes, OutSlot* o) {
 }
 int copy_out(mz_ctx* ctx, const OutSlot& o) {
     if (o.copy) HIP_TRY(hipMemcpyAsync(o.user, o.dev, o.bytes, hipMemcpyDeviceToHost, ctx->stream));
+    return 0;
+}
+
+// a buffer of at least `bytes` that the context keeps
+int grow(mz_ctx* ctx, DevBuf& b, size_t bytes) {
+    if (b.bytes >= bytes && b.p) return 0;
+    if (b.p) (void)hipFree(b.p);   // waits for what uses it
+    b = DevBuf{};
+    HIP_TRY(hipMalloc(&b.p, std::max<size_t>(bytes, 256)));
+    b.bytes = bytes;
     return 0;
 }
 
@@ -959,6 +973,8 @@ void mz_destroy(mz_ctx* ctx) {
     if (ctx->mfma) mfma_destroy(ctx->mfma);
     if (ctx->comm) (void)rccl()->CommDestroy((ncclComm_t)ctx->comm);
     if (ctx->comm_buf) (void)hipFree(ctx->comm_buf);
+    for (DevBuf* b : {&ctx->ad_a, &ctx->ad_b, &ctx->ad_scale, &ctx->pol_feat, &ctx->pol_logits, &ctx->pol_ws})
+        if (b->p) (void)hipFree(b->p);
     for (auto& e : ctx->events) {
         (void)hipEventDestroy(e.a);
         (void)hipEventDestroy(e.b);
@@ -1225,6 +1241,119 @@ int mz_read_hidden(mz_ctx* ctx, int32_t slot, float* out) {
         return 0;
     }
     HIP_TRY(hipMemcpy(out, ctx->pool + (size_t)(base + slot) * n, n * sizeof(float), hipMemcpyDefault));
+    return 0;
+}
+
+int mz_load_policy_adapters(mz_ctx* ctx, int n, int rank, const float* a, const float* b, const float* scale) {
+    if (!ctx) return -1;
+    if (n < 0 || (n > 0 && (rank < 1 || rank > 128))) return ctx_fail(ctx, "need n >= 0 and a rank of 1 .. 128");
+    if (n > 0 && (!a || !b)) return ctx_fail(ctx, "null argument");
+    HIP_TRY(hipSetDevice(ctx->device));
+    HIP_TRY(hipStreamSynchronize(ctx->stream));
+    const size_t K = 2 * (size_t)ctx->nd.HW, A = ctx->nd.A, r = (size_t)std::max(rank, 0);
+    ctx->ad_n = 0;   // none, should a step below fail
+    if (n == 0) return 0;
+    if (grow(ctx, ctx->ad_a, n * r * K * sizeof(float)) || grow(ctx, ctx->ad_b, n * A * r * sizeof(float)) || grow(ctx, ctx->ad_scale, n * sizeof(float)))
+        return -1;
+    HIP_TRY(hipMemcpy(ctx->ad_a.p, a, n * r * K * sizeof(float), hipMemcpyDefault));
+    HIP_TRY(hipMemcpy(ctx->ad_b.p, b, n * A * r * sizeof(float), hipMemcpyDefault));
+    if (scale) HIP_TRY(hipMemcpy(ctx->ad_scale.p, scale, n * sizeof(float), hipMemcpyDefault));
+    ctx->ad_scaled = scale != nullptr;
+    ctx->ad_rank = rank;
+    ctx->ad_n = n;
+    return 0;
+}
+
+int mz_play_policy(mz_ctx* ctx, int B, const float* obs, const uint8_t* legal, const int32_t* adapter, const mz_policy_sampling* sampling, const double* u,
+                   const mz_policy_outputs* out) {
+    if (check_B(ctx, B)) return -1;
+    if (!obs || !legal || !sampling || !u || !out) return ctx_fail(ctx, "null argument");
+    if (!ctx->weights_loaded) return ctx_fail(ctx, "weights not loaded");
+    if (adapter && ctx->ad_n == 0) return ctx_fail(ctx, "no policy adapters are loaded");
+    if (adapter && !is_device_ptr(adapter))
+        for (int g = 0; g < B; g++)
+            if (adapter[g] < -1 || adapter[g] >= ctx->ad_n) return ctx_fail(ctx, "adapter index out of range");
+    HIP_TRY(hipSetDevice(ctx->device));
+    timing_begin(ctx);
+    const NetDims& d = ctx->nd;
+    const size_t A = d.A, K = 2 * (size_t)d.HW;
+    const void *d_obs, *d_legal, *d_adapter, *d_u;
+    if (stage_in(ctx, 0, obs, (size_t)B * d.O * d.HW * sizeof(float), &d_obs) || stage_in(ctx, 1, legal, B * A, &d_legal) ||
+        stage_in(ctx, 2, adapter, B * sizeof(int), &d_adapter) || stage_in(ctx, 3, u, B * sizeof(double), &d_u))
+        return -1;
+    OutSlot o[6];
+    void* const user[6] = {out->action, out->logprob, out->kept, out->playout_policy, out->logits, out->value};
+    const size_t bytes[6] = {B * sizeof(int), B * sizeof(float), B * sizeof(int), B * A * sizeof(float), B * A * sizeof(float), B * sizeof(double)};
+    for (int i = 0; i < 6; i++)
+        if (stage_out(ctx, 16 + i, user[i], bytes[i], &o[i])) return -1;
+
+    NetIO io{};
+    io.obs = (const float*)d_obs;
+    io.B = B;
+    io.pool = ctx->pool;
+    io.logits = ctx->net_logits;
+    io.policy = ctx->net_policy;
+    io.value = ctx->net_value;
+    io.action_cells = ctx->action_cells;
+    io.dst_slot = ctx->root_slots;
+    if (adapter) {
+        if (grow(ctx, ctx->pol_feat, (size_t)ctx->cfg.max_games * K * sizeof(float)) || grow(ctx, ctx->pol_logits, (size_t)ctx->cfg.max_games * A * sizeof(float)))
+            return -1;
+        io.feat = (float*)ctx->pol_feat.p;
+    }
+    if (run_net(ctx, true, io)) return -1;
+    float* logits = ctx->net_logits;
+    if (adapter) {
+        logits = (float*)ctx->pol_logits.p;
+        // the end of the blob: fc [A][2 HW], bias [A], then the value head
+        const size_t value_head = d.C + 2 * (size_t)d.HW + (size_t)d.C * d.HW + 2 * (size_t)d.C + 1;
+        const float* fc = ctx->w_master + ctx->n_params - value_head - A - A * K;
+        mz_adapter_args a{};
+        a.rows = B;
+        a.in_features = (int)K;
+        a.out_features = (int)A;
+        a.rank = ctx->ad_rank;
+        a.adapters = ctx->ad_n;
+        a.dtype = a.out_dtype = MZ_DTYPE_FP32;
+        a.x = ctx->pol_feat.p;
+        a.x_stride = a.weight_stride = (int64_t)K;
+        a.weight = fc;
+        a.bias = fc + A * K;
+        a.a = ctx->ad_a.p;
+        a.b = ctx->ad_b.p;
+        a.scale = ctx->ad_scaled ? (const float*)ctx->ad_scale.p : nullptr;
+        a.index = (const int32_t*)d_adapter;
+        a.y = logits;
+        a.y_stride = (int64_t)A;
+        const size_t need = mz_adapter_workspace_bytes(&a);
+        if (grow(ctx, ctx->pol_ws, need)) return -1;
+        if (mz_adapter_linear(&a, ctx->pol_ws.p, ctx->pol_ws.bytes, ctx->stream)) return ctx_fail(ctx, g_create_error);
+    }
+    mz_sample_args s{};
+    s.rows = B;
+    s.actions = (int)A;
+    s.dtype = MZ_DTYPE_FP32;
+    s.top_k = sampling->top_k;
+    s.temperature = sampling->temperature;
+    s.top_p = sampling->top_p;
+    s.min_p = sampling->min_p;
+    s.logits = logits;
+    s.row_stride = s.legal_stride = s.probs_stride = (int64_t)A;
+    s.legal = (const uint8_t*)d_legal;
+    s.u = (const double*)d_u;
+    s.action = o[0].dev ? (int32_t*)o[0].dev : ctx->net_action;
+    s.logprob = (float*)o[1].dev;
+    s.kept = (int32_t*)o[2].dev;
+    s.probs = (float*)o[3].dev;
+    const size_t need = mz_sample_workspace_bytes(&s);
+    if (grow(ctx, ctx->pol_ws, need)) return -1;
+    if (mz_sample_actions(&s, ctx->pol_ws.p, ctx->pol_ws.bytes, ctx->stream)) return ctx_fail(ctx, g_create_error);
+    if (o[4].dev) HIP_TRY(hipMemcpyAsync(o[4].dev, logits, bytes[4], hipMemcpyDefault, ctx->stream));
+    if (o[5].dev) HIP_TRY(hipMemcpyAsync(o[5].dev, ctx->net_value, bytes[5], hipMemcpyDefault, ctx->stream));
+    for (int i = 0; i < 6; i++)
+        if (copy_out(ctx, o[i])) return -1;
+    HIP_TRY(hipStreamSynchronize(ctx->stream));
+    timing_end(ctx);
     return 0;
 }
 

@@ -47,6 +47,7 @@ struct NetIO {
     float* logits;            // [B][A]
     float* policy;            // [B][A]
     double* value;            // [B]
+    float* feat;              // [B][2 HW] the policy head's features (LayerNorm + ReLU, what pred.p.fc multiplies), or nullptr
     int B;
     int g_base;               // position of sample 0 in the context's per-sample scratch (two half batches in flight at once)
 };

@@ -741,6 +741,9 @@ __global__ __launch_bounds__(NT) void k_net_fp32(NetDims d, const NetProgramF32*
 #if defined(MZ_FP32_STAMPS)
     tmark = __builtin_amdgcn_s_memtime();
 #endif
+    if (io.feat) {
+        for (int i = tid; i < 2 * HW; i += NT) io.feat[(long long)g * 2 * HW + i] = pc[i];
+    }
     float* lgt = T2;                 // logits staged in LDS for the softmax
     float* fc_part = T2 + ((A + 3) & ~3);
     {

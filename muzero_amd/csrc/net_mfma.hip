@@ -1162,6 +1162,9 @@ __global__ __launch_bounds__(HT) void k_heads(NetDims d, HeadDev hd, NetIO io) {
         }
     }
     __syncthreads();
+    if (io.feat && live) {
+        for (int i = lane; i < K1; i += 64) io.feat[(long long)g * K1 + i] = feat[wave * 3 * HPMAX + i];
+    }
     // the two linears, split over K into chunks of HKC; chunk partials are summed in a fixed order
     for (int it = tid; it < items; it += HT) {
         const Item q = item(it);

@@ -525,6 +525,43 @@ std::vector<NetworkIO> ModelService::recurrentInference(const std::vector<int>& 
     return out;
 }
 
+ModelService::PolicyMoves ModelService::playPolicy(const std::vector<const Game*>& games, const mz_policy_sampling& sampling, const std::vector<double>& u) {
+    if (!ctx) throw MuZeroException("inference: this ModelService has no device context");
+    const int B = static_cast<int>(games.size()), A = config.actionSpaceSize;
+    if (u.size() != games.size()) throw MuZeroException("playPolicy: one random number per game");
+    std::vector<float> obs;
+    std::vector<uint8_t> legal(static_cast<size_t>(B) * A);
+    for (int g = 0; g < B; g++) {
+        const ObservationModelInput in = games[g]->getObservationModelInput();
+        obs.insert(obs.end(), in.value.begin(), in.value.end());
+        for (const Action& a : games[g]->legalActions()) legal[static_cast<size_t>(g) * A + a.getIndex()] = 1;
+    }
+    PolicyMoves m;
+    m.action.resize(B);
+    std::vector<float> logits(static_cast<size_t>(B) * A), playout(static_cast<size_t>(B) * A);
+    std::vector<double> value(B);
+    mz_policy_outputs out{};
+    out.action = m.action.data();
+    out.playout_policy = playout.data();
+    out.logits = logits.data();
+    out.value = value.data();
+    check(mz_play_policy(ctx, B, obs.data(), legal.data(), nullptr, &sampling, u.data(), &out), "mz_play_policy");
+    m.io.resize(B);
+    for (int g = 0; g < B; g++) {
+        const float* l = logits.data() + static_cast<size_t>(g) * A;
+        NetworkIO& io = m.io[g];
+        io.logits.assign(l, l + A);
+        io.value = value[g];
+        // InitialInferenceListTranslator's softmax
+        const float mx = *std::max_element(l, l + A);
+        float s = 0.f;
+        for (int a = 0; a < A; a++) s += std::exp(l[a] - mx);
+        for (int a = 0; a < A; a++) io.policyValues.push_back(std::exp(l[a] - mx) / s);
+        m.playoutPolicy.emplace_back(playout.begin() + static_cast<size_t>(g) * A, playout.begin() + static_cast<size_t>(g + 1) * A);
+    }
+    return m;
+}
+
 // ---- PlanAction (P/agent/c_planning/PlanAction.java:68-171), batched -------------------------------------------
 std::vector<Action> PlanAction::planActions(const std::vector<Game*>& games, const PlayParameters& p) {
     const MuZeroConfig& config = modelService.getConfig();
@@ -673,12 +710,20 @@ std::vector<Action> PlanAction::planActionsFastRules(const std::vector<Game*>& g
 
 // justInitialInferencePolicy (PlanAction.playAfterJustWithInitialInference, PlanAction.java:174-193): the root is expanded
 // from the initial inference, the move is drawn from the renormalised priors, the priors are the policy target.
-std::vector<Action> PlanAction::planActionsJustInitialInference(const std::vector<Game*>& games, const PlayParameters&) {
+std::vector<Action> PlanAction::planActionsJustInitialInference(const std::vector<Game*>& games, const PlayParameters& p) {
     const MuZeroConfig& config = modelService.getConfig();
     const int A = config.actionSpaceSize;
     std::vector<const Game*> cg(games.begin(), games.end());
     modelService.startScope();   // the hidden states are not kept: reuse the pool from its start
-    const std::vector<NetworkIO> io = modelService.initialInference(cg);
+    std::vector<double> us;
+    ModelService::PolicyMoves drawn;
+    if (p.samplePolicy) {
+        for (const Game* g : cg)
+            if (g->legalActions().empty()) throw MuZeroException("planAction on a game without legal actions");
+        for (size_t g = 0; g < games.size(); g++) us.push_back(rng.nextDouble());
+        drawn = modelService.playPolicy(cg, p.policySampling, us);
+    }
+    const std::vector<NetworkIO> io = p.samplePolicy ? drawn.io : modelService.initialInference(cg);
     std::vector<Action> result;
     for (size_t g = 0; g < games.size(); g++) {
         Game& game = *games[g];
@@ -710,10 +755,11 @@ std::vector<Action> PlanAction::planActionsJustInitialInference(const std::vecto
         // walks the cumulative sums in list order (= child order); the uniform draw is this class's Rng
         double total = 0.0;
         for (double x : prior) total += x;
-        const double u = rng.nextDouble();
+        const double u = p.samplePolicy ? us[g] : rng.nextDouble();
         double cum = 0.0;
-        int pick = order.back();
-        for (size_t i = 0; i < order.size(); i++) {
+        int pick = p.samplePolicy ? drawn.action[g] : order.back();
+        if (p.samplePolicy) dto.playoutPolicy.push_back(drawn.playoutPolicy[g]);
+        for (size_t i = 0; i < order.size() && !p.samplePolicy; i++) {
             cum += prior[i] / total;
             if (u < cum) {
                 pick = order[i];

@@ -272,6 +272,15 @@ public:
     const MuZeroConfig& getConfig() const { return config; }
     int maxGames() const { return maxGames_; }
 
+    // One raw-policy move per game (mz_play_policy): NetworkIO without a hidden state, the drawn actions and the distribution
+    // they were drawn from; `u` holds a uniform number per game.
+    struct PolicyMoves {
+        std::vector<NetworkIO> io;
+        std::vector<int32_t> action;
+        std::vector<std::vector<float>> playoutPolicy;
+    };
+    PolicyMoves playPolicy(const std::vector<const Game*>& games, const mz_policy_sampling& sampling, const std::vector<double>& u);
+
 private:
     void check(int rc, const char* what);
     MuZeroConfig config;
@@ -290,6 +299,10 @@ struct PlayParameters {
     int averageGameLength = 0;
     double pRandomActionRawAverage = 0;
     bool replay = false;
+    // No counterpart in the reference: justInitialInferencePolicy with the move drawn on the device after temperature, top-k,
+    // top-p and min-p (mz_play_policy) instead of from the renormalised policy on the host.
+    bool samplePolicy = false;
+    mz_policy_sampling policySampling{1.0, 1.0, 0.0, 0, 0};
 };
 
 // P/agent/c_planning/PlanAction.java:68-171, batched: one planned move for every game of `games`.

@@ -2,7 +2,8 @@
 // prints one JSON line of episode statistics.  The counterpart of the reference's
 // games/tictactoe/src/test/java/ai/enpasos/muzero/tictactoe/PlayTest.java:62-72 (testMultiGameStarter_Basic).
 // usage: selfplay_main <weights.f32> <numGames> <seed> <playType: PLAYOUT|HYBRID> <precision: fp32|bf16> [mode]
-// mode: play (default) | initial (justInitialInferencePolicy) | reanalyse (play, then PlayService.reanalyseGames on
+// mode: play (default) | initial (justInitialInferencePolicy) | policy (the same, drawn on the device: temperature 0.8, top-k 6, top-p
+// 0.95, min-p 0.01) | reanalyse (play, then PlayService.reanalyseGames on
 // copies) | justreplay (play, then justReplayGamesWithInitialInference on copies)
 #include <cmath>
 #include <cstdio>
@@ -35,16 +36,18 @@ int main(int argc, char** argv) {
         if (raw.empty()) throw MuZeroException("cannot read the weight blob");
 
         const std::string mode = argc > 6 ? argv[6] : "play";
-        ModelService modelService(config, numGames, precision, 0, mode == "play" || mode == "reanalyse" ? 0 : numGames);
+        ModelService modelService(config, numGames, precision, 0, mode == "play" || mode == "reanalyse" || mode == "policy" ? 0 : numGames);
         modelService.loadWeights(reinterpret_cast<const float*>(raw.data()), raw.size() / sizeof(float));
         PlayService playService(modelService, seed);
         playService.maxGameLength = 9;
         PlayParameters p;
         p.render = false;
         p.withGumbel = hybrid;   // self-play passes withGumbel = true (PlayParameters.java:23-24); PLAYOUT uses the config's false
-        p.justInitialInferencePolicy = mode == "initial";
+        p.justInitialInferencePolicy = mode == "initial" || mode == "policy";
+        p.samplePolicy = mode == "policy";
+        p.policySampling = mz_policy_sampling{0.8, 0.95, 0.01, 6, 0};
         std::vector<std::unique_ptr<Game>> games = playService.playNewGames(numGames, p);
-        const bool searched = mode != "initial";
+        const bool searched = mode != "initial" && mode != "policy";
 
         // second pass over copies of the finished episodes (PlayService.java:53-85)
         long replayActionMismatch = 0, replayLengthMismatch = 0, replayTargetsEqual = 0, replayPlayoutGrew = 0, replayValues = 0;

@@ -1,6 +1,7 @@
 """The library's operators on torch tensors (mz_sample_actions, mz_adapter_linear of include/muzero_hip.h): checks of types, shapes and
 devices, then one call of the C ABI on torch's current stream of the tensors' device.  Nothing is copied, converted or
-synchronised; a call can be captured into a torch.cuda.graph.  Errors are capi.MuZeroError."""
+synchronised; a call can be captured into a torch.cuda.graph.  There are no gradients: inputs that ask for them are refused
+while torch's grad mode is on.  Errors are capi.MuZeroError."""
 from ctypes import byref
 
 import torch
@@ -41,6 +42,11 @@ def _stream(device):
     return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise capi.MuZeroError("an input requires a gradient and this operator has none: call it under torch.no_grad()")
+
+
 def _fail():
     raise capi.MuZeroError(capi.lib().mz_last_error(None).decode())
 
@@ -77,6 +83,7 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     t, dev = logits.dtype, logits.device
     if not logits.is_cuda or t not in DTYPES:
         raise capi.MuZeroError(f"logits: must be on a GPU and float32, bfloat16 or float16, not {t} on {dev}")
+    _no_grad(logits)
     shape = logits.shape
     B, A = shape
     rows = (B,)
@@ -126,6 +133,7 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
     t, dev = x.dtype, x.device
     if not x.is_cuda or t not in DTYPES:
         raise capi.MuZeroError(f"x: must be on a GPU and float32, bfloat16 or float16, not {t} on {dev}")
+    _no_grad(x, weight, a, b, bias, scale)
     M, K = x.shape
     n, r, _ = a.shape
     N = weight.shape[0]

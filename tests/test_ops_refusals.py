@@ -92,3 +92,7 @@ def test_adapter_of_no_rows():
                          weight_stride=64, y_stride=32)
     assert capi.lib().mz_adapter_workspace_bytes(C.byref(a)) == 0
     assert capi.lib().mz_adapter_linear(C.byref(a), None, 0, None) == 0
+
+
+def test_policy_struct_layouts():
+    assert C.sizeof(capi.PolicySampling) == 32 and C.sizeof(capi.PolicyOutputs) == 48

@@ -7,5 +7,5 @@ name=$1; shift
 cd "$(dirname "$0")/../muzero_amd/csrc"
 mkdir -p ../../gpurun_abl
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC "$@" -c net_fp32.hip -o /tmp/nf_$name.o
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../../gpurun_abl/libmz_$name.so tree.o /tmp/nf_$name.o net_mfma.o net_mfma_f16.o api.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../../gpurun_abl/libmz_$name.so tree.o /tmp/nf_$name.o net_mfma.o net_mfma_f16.o api.o sample.o adapter.o ops_api.o
 echo built gpurun_abl/libmz_$name.so

@@ -7,5 +7,5 @@ name=$1; shift
 cd "$(dirname "$0")/../muzero_amd/csrc"
 mkdir -p ../../gpurun_abl
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -DMZ_FAST_BUILD -DMZ_F16=1 "$@" -c net_mfma.hip -o /tmp/nm_$name.o
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../../gpurun_abl/libmz_$name.so tree.o net_fp32.o net_mfma.o /tmp/nm_$name.o api.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../../gpurun_abl/libmz_$name.so tree.o net_fp32.o net_mfma.o /tmp/nm_$name.o api.o sample.o adapter.o ops_api.o
 echo built gpurun_abl/libmz_$name.so
