@@ -7,7 +7,7 @@
 set -e
 cd "$(dirname "$0")/../muzero_amd/csrc"
 mkdir -p ../../gpurun_abl/asan /tmp/asan
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O1 -Xclang -target-feature -Xclang -packed-fp32-ops -g -std=c++17 -fPIC -Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer -c api.cpp -o /tmp/asan/api_asan.o sample.o adapter.o ops_api.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O1 -Xclang -target-feature -Xclang -packed-fp32-ops -g -std=c++17 -fPIC -Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer -c api.cpp -o /tmp/asan/api_asan.o
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -Xarch_host -fsanitize=address -o ../../gpurun_abl/asan/libmuzero_hip.so tree.o net_fp32.o net_mfma.o net_mfma_f16.o /tmp/asan/api_asan.o sample.o adapter.o ops_api.o
 cd ../host
 /opt/rocm/lib/llvm/bin/clang++ -O1 -g -std=c++17 -fsanitize=address -fno-omit-frame-pointer -I../../include selfplay_main.cpp muzero_host.cpp \
