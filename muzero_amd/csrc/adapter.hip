@@ -618,56 +618,73 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
         }
     }
     {
-        // through registers: all of K without DMA, what is left of a stage with it
-        const T *px[LX], *pw[LW];
+        // Through registers: all of K without DMA, what is left of a stage with it.  By 4-byte words, 16 lanes to the 64 bytes of a
+        // row: a 16-byte load that is not aligned to 16 takes the time of four, and here rows need not be aligned to anything.
+        constexpr int RX = BM / NW / 4, RW = BN / NW / 4, E = 4 / (int)sizeof(T);   // rows of each operand per lane; elements of a word
+        const int word = lane & 15;
+        const T *px[RX], *pw[RW];
+        int to[RX], tw[RW];     // where the words go in a stage
 #pragma unroll
-        for (int i = 0; i < LX; i++) px[i] = xb + min(order[(wave * LX + i) * 16 + (lane >> 2)], count - 1) * op.x_stride + slot * CE;
+        for (int i = 0; i < RX; i++) {
+            const int r = (wave * RX + i) * 4 + (lane >> 4);
+            px[i] = xb + min(order[r], count - 1) * op.x_stride + word * E;
+            to[i] = r * 64 + (((word >> 2) ^ (r >> 1 & 3)) << 4) + (word & 3) * 4;
+        }
 #pragma unroll
-        for (int i = 0; i < LW; i++) pw[i] = wb + min((wave * LW + i) * 16 + (lane >> 2), op.N - 1 - n0) * op.w_stride + slot * CE;
-        const auto put = [&](char* st, const u32x4 (&vx)[LX], const u32x4 (&vw)[LW]) {
+        for (int i = 0; i < RW; i++) {
+            const int r = (wave * RW + i) * 4 + (lane >> 4);
+            pw[i] = wb + min(r, op.N - 1 - n0) * op.w_stride + word * E;
+            tw[i] = (BM + r) * 64 + (((word >> 2) ^ (r >> 1 & 3)) << 4) + (word & 3) * 4;
+        }
+        const auto put = [&](char* st, const uint32_t (&vx)[RX], const uint32_t (&vw)[RW]) {
 #pragma unroll
-            for (int i = 0; i < LX; i++) {
-                const int r = (wave * LX + i) * 16 + (lane >> 2);
-                *reinterpret_cast<u32x4*>(st + r * 64 + ((slot ^ (r >> 1 & 3)) << 4)) = vx[i];
-            }
+            for (int i = 0; i < RX; i++) *reinterpret_cast<uint32_t*>(st + to[i]) = vx[i];
 #pragma unroll
-            for (int i = 0; i < LW; i++) {
-                const int r = (wave * LW + i) * 16 + (lane >> 2);
-                *reinterpret_cast<u32x4*>(st + (BM + r) * 64 + ((slot ^ (r >> 1 & 3)) << 4)) = vw[i];
-            }
+            for (int i = 0; i < RW; i++) *reinterpret_cast<uint32_t*>(st + tw[i]) = vw[i];
         };
         const int full = op.K / (4 * CE);
         if (!DMA && full > 0) {
             constexpr int D = BM == 64 ? 4 : 2;   // stages on their way; behind the last whole one: that one again
-            u32x4 vx[D][LX], vw[D][LW];
-            const auto fetch = [&](int s, u32x4 (&vx)[LX], u32x4 (&vw)[LW]) {
+            uint32_t vx[D][RX], vw[D][RW];
+            const auto fetch = [&](int s, uint32_t (&vx)[RX], uint32_t (&vw)[RW]) {
                 const int k = min(s, full - 1) * 4 * CE;
 #pragma unroll
-                for (int i = 0; i < LX; i++) vx[i] = load16(px[i] + k);
+                for (int i = 0; i < RX; i++) __builtin_memcpy(&vx[i], px[i] + k, 4);
 #pragma unroll
-                for (int i = 0; i < LW; i++) vw[i] = load16(pw[i] + k);
+                for (int i = 0; i < RW; i++) __builtin_memcpy(&vw[i], pw[i] + k, 4);
                 __builtin_amdgcn_sched_barrier(0);   // loads in the order of the stages: the waits count them
             };
 #pragma unroll
             for (int d = 0; d < D; d++) fetch(d, vx[d], vw[d]);
+            constexpr int G = BM == 64 ? 2 : 1;   // stages to a barrier: small tiles have little to do in one
             for (int s = 0; s < full; s += D)
 #pragma unroll
-                for (int d = 0; d < D; d++) {
+                for (int d = 0; d < D; d += G) {
                     // (a step behind the last stage only turns the barrier)
-                    put(smem + (d & 1) * STAGE, vx[d], vw[d]);
-                    fetch(s + d + D, vx[d], vw[d]);
-                    // the fetches stay in flight over the barrier; LDS: the slot that is written next was read a step ago
+#pragma unroll
+                    for (int g = 0; g < G; g++) put(smem + (d + g) % (2 * G) * STAGE, vx[d + g], vw[d + g]);
+#pragma unroll
+                    for (int g = 0; g < G; g++) fetch(s + d + g + D, vx[d + g], vw[d + g]);
+                    // the fetches stay in flight over the barrier; LDS: the slots that are written next were read a step ago
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    if (s + d < full) compute(smem + (d & 1) * STAGE);
+#pragma unroll
+                    for (int g = 0; g < G; g++)
+                        if (s + d + g < full) compute(smem + (d + g) % (2 * G) * STAGE);
                 }
         }
         if (full * 4 * CE < op.K) {
-            u32x4 vx[LX], vw[LW];
-            const int k = full * 4 * CE, left = op.K - slot * CE;
+            const int k = full * 4 * CE, left = op.K - k - word * E;   // elements of the row from this lane's word on
+            uint32_t vx[RX], vw[RW];
+            const auto rest = [&](const T* p) {
+                uint32_t v = 0;
+                if (left >= E) __builtin_memcpy(&v, p + k, 4);
+                else if (left > 0) __builtin_memcpy(&v, p + k, sizeof(T));   // half of a word: the low one
+                return v;
+            };
 #pragma unroll
-            for (int i = 0; i < LX; i++) vx[i] = load_chunk(px[i], k, left);
+            for (int i = 0; i < RX; i++) vx[i] = rest(px[i]);
 #pragma unroll
-            for (int i = 0; i < LW; i++) vw[i] = load_chunk(pw[i], k, left);
+            for (int i = 0; i < RW; i++) vw[i] = rest(pw[i]);
             __syncthreads();   // the stages before have been read
             put(smem, vx, vw);
             __syncthreads();
