@@ -2,14 +2,37 @@
 devices, then one call of the C ABI on torch's current stream of the tensors' device.  Nothing is copied, converted or
 synchronised; a call can be captured into a torch.cuda.graph.  There are no gradients: inputs that ask for them are refused
 while torch's grad mode is on.  Errors are capi.MuZeroError."""
-from ctypes import byref
+import ctypes as C
+import struct
 
 import torch
 
 from . import capi
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the same number without a Stream object around it
+# the argument structs of the C ABI as bytes (capi.SampleArgs, capi.AdapterArgs have the fields): packing costs a quarter of
+# filling a ctypes Structure, and these calls are short
+_SAMPLE = struct.Struct("=4i3d14q")
+_ADAPTER = struct.Struct("=8i11q")
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MZ_DTYPE_*
+
+
+_entries = None
+
+
+def _lib():
+    """The operators' C entries, with the structs as bytes."""
+    global _entries
+    if _entries is None:
+        capi.lib()   # fails loudly if the library is missing
+        L = C.CDLL(capi.LIB_PATH)
+        for name in ("mz_sample", "mz_adapter"):
+            f = getattr(L, name + "_workspace_bytes")
+            f.argtypes, f.restype = [C.c_char_p], C.c_size_t
+        for name in ("mz_sample_actions", "mz_adapter_linear"):
+            getattr(L, name).argtypes = [C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p]
+        _entries = L
+    return _entries
 
 
 def _need(ok, text):
@@ -18,16 +41,16 @@ def _need(ok, text):
 
 
 def _tensor(t, name, dtype, shape, device, dense=True):
-    """Address of t, a tensor of that dtype, shape and device whose rows are contiguous (dense: all of it)."""
+    """Address of t, a tensor of that dtype and shape on GPU `device` whose rows are contiguous (dense: all of it)."""
     try:   # one test for the usual case; which one failed is found out below
-        if t.dtype is dtype and t.shape == shape and t.device == device and (t.is_contiguous() or not dense and t.stride(-1) == 1):
+        if t.dtype is dtype and t.shape == shape and t.get_device() == device and (t.is_contiguous() or not dense and t.stride(-1) == 1):
             return t.data_ptr()
     except AttributeError:
         pass
     _need(isinstance(t, torch.Tensor), f"{name}: a torch tensor is needed")
     _need(t.dtype == dtype, f"{name}: {t.dtype}, needs {dtype}")
     _need(tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, needs {tuple(shape)}")
-    _need(t.device == device, f"{name}: on {t.device}, the other operands on {device}")
+    _need(t.get_device() == device, f"{name}: on {t.device}, the other operands on cuda:{device}")
     _need(not dense, f"{name}: must be contiguous")
     _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must be contiguous")
     return t.data_ptr()
@@ -38,12 +61,12 @@ def _row_stride(t):
 
 
 def _stream(device):
-    """torch's current stream of the device, as a hipStream_t."""
-    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+    """torch's current stream of GPU `device`, as a hipStream_t."""
+    return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_gradient():
+    if torch.is_grad_enabled():
         raise capi.MuZeroError("an input requires a gradient and this operator has none: call it under torch.no_grad()")
 
 
@@ -53,20 +76,20 @@ def _fail():
 
 def _setting(v, name, dtype, shape, device):
     """A number, or a tensor with one per row: (scalar, address)."""
-    if isinstance(v, torch.Tensor):
+    if type(v) is not float and type(v) is not int and isinstance(v, torch.Tensor):
         return 0, _tensor(v, name, dtype, shape, device)
-    return v, None
+    return v, 0
 
 
 def _workspace(need, given, device):
     """(tensor to keep alive, address, bytes).  torch's allocator hands the memory out per stream (and per graph)."""
     if given is not None:
-        _need(given.dtype == torch.uint8 and given.is_contiguous() and given.device == device,
-              f"workspace: a contiguous uint8 tensor on {device} is needed")
+        _need(isinstance(given, torch.Tensor) and given.dtype == torch.uint8 and given.is_contiguous() and given.get_device() == device,
+              f"workspace: a contiguous uint8 tensor on cuda:{device} is needed")
         return given, given.data_ptr(), given.numel()
     if need == 0:
         return None, None, 0
-    w = torch.empty(need, dtype=torch.uint8, device=device)
+    w = torch.empty(need, dtype=torch.uint8, device=f"cuda:{device}")
     return w, w.data_ptr(), need
 
 
@@ -80,14 +103,15 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     a dict of tensors to write into instead (action required, the others as wanted)."""
     if not (isinstance(logits, torch.Tensor) and logits.dim() == 2):
         raise capi.MuZeroError("logits: a 2-d torch tensor is needed")
-    t, dev = logits.dtype, logits.device
-    if not logits.is_cuda or t not in DTYPES:
-        raise capi.MuZeroError(f"logits: must be on a GPU and float32, bfloat16 or float16, not {t} on {dev}")
-    _no_grad(logits)
+    t, dev = logits.dtype, logits.get_device()
+    if dev < 0 or t not in DTYPES:
+        raise capi.MuZeroError(f"logits: must be on a GPU and float32, bfloat16 or float16, not {t} on {logits.device}")
+    if logits.requires_grad:
+        _no_gradient()
     shape = logits.shape
     B, A = shape
     rows = (B,)
-    p_legal, s_legal = None, 0
+    p_legal, s_legal = 0, 0
     if legal is not None:
         lt = getattr(legal, "dtype", None)
         if lt is not torch.uint8 and lt is not torch.bool:
@@ -100,25 +124,28 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     if top_k >= 2**31:
         top_k = 2**31 - 1
     if out is None:
-        out = dict(action=torch.empty(B, dtype=torch.int32, device=dev), logprob=torch.empty(B, device=dev),
-                   kept=torch.empty(B, dtype=torch.int32, device=dev))
+        on = logits.device
+        out = dict(action=torch.empty(B, dtype=torch.int32, device=on), logprob=torch.empty(B, dtype=torch.float32, device=on),
+                   kept=torch.empty(B, dtype=torch.int32, device=on))
         if probs:
-            out["probs"] = torch.empty(B, A, device=dev)
+            out["probs"] = torch.empty(B, A, dtype=torch.float32, device=on)
     get = out.get
     action, logprob, kept, pr = get("action"), get("logprob"), get("kept"), get("probs")
-    args = capi.SampleArgs(
-        B, A, DTYPES[t], top_k, temperature, top_p, min_p,
-        _tensor(logits, "logits", t, shape, dev, dense=False), _row_stride(logits), p_legal, s_legal,
-        _tensor(u, "u", torch.float64, rows, dev), p_t, p_k, p_p, p_m,
-        _tensor(action, "out['action']", torch.int32, rows, dev),
-        None if logprob is None else _tensor(logprob, "out['logprob']", torch.float32, rows, dev),
-        None if kept is None else _tensor(kept, "out['kept']", torch.int32, rows, dev),
-        None if pr is None else _tensor(pr, "out['probs']", torch.float32, shape, dev, dense=False),
-        0 if pr is None else _row_stride(pr))
-    L = capi.lib()
-    ref = byref(args)
-    keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(ref), workspace, dev)
-    if L.mz_sample_actions(ref, ws, nbytes, _stream(dev)) != 0:
+    try:
+        args = _SAMPLE.pack(
+            B, A, DTYPES[t], top_k, temperature, top_p, min_p,
+            _tensor(logits, "logits", t, shape, dev, dense=False), _row_stride(logits), p_legal, s_legal,
+            _tensor(u, "u", torch.float64, rows, dev), p_t, p_k, p_p, p_m,
+            _tensor(action, "out['action']", torch.int32, rows, dev),
+            0 if logprob is None else _tensor(logprob, "out['logprob']", torch.float32, rows, dev),
+            0 if kept is None else _tensor(kept, "out['kept']", torch.int32, rows, dev),
+            0 if pr is None else _tensor(pr, "out['probs']", torch.float32, shape, dev, dense=False),
+            0 if pr is None else _row_stride(pr))
+    except struct.error as e:
+        raise capi.MuZeroError(f"temperature, top_k, top_p and min_p must be numbers in range ({e})") from None
+    L = _lib()
+    keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(args), workspace, dev)
+    if L.mz_sample_actions(args, ws, nbytes, _stream(dev)) != 0:
         _fail()
     return out
 
@@ -130,33 +157,34 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
     for v, name, dims in ((x, "x", 2), (weight, "weight", 2), (a, "a", 3)):
         if not (isinstance(v, torch.Tensor) and v.dim() == dims):
             raise capi.MuZeroError(f"{name}: a {dims}-d torch tensor is needed")
-    t, dev = x.dtype, x.device
-    if not x.is_cuda or t not in DTYPES:
-        raise capi.MuZeroError(f"x: must be on a GPU and float32, bfloat16 or float16, not {t} on {dev}")
-    _no_grad(x, weight, a, b, bias, scale)
+    t, dev = x.dtype, x.get_device()
+    if dev < 0 or t not in DTYPES:
+        raise capi.MuZeroError(f"x: must be on a GPU and float32, bfloat16 or float16, not {t} on {x.device}")
+    if (x.requires_grad or weight.requires_grad or a.requires_grad or getattr(b, "requires_grad", False)
+            or bias is not None and bias.requires_grad or scale is not None and scale.requires_grad):
+        _no_gradient()
     M, K = x.shape
     n, r, _ = a.shape
     N = weight.shape[0]
     if out is None:
-        out = torch.empty(M, N, dtype=t if out_dtype is None else out_dtype, device=dev)
+        out = torch.empty(M, N, dtype=t if out_dtype is None else out_dtype, device=x.device)
     elif out_dtype is None:
         out_dtype = getattr(out, "dtype", None)
     if out_dtype is None:
         out_dtype = t
     if out_dtype not in DTYPES:
         raise capi.MuZeroError(f"out: {out_dtype} is not supported")
-    args = capi.AdapterArgs(
+    args = _ADAPTER.pack(
         M, K, N, r, n, DTYPES[t], DTYPES[out_dtype], 0,
         _tensor(x, "x", t, (M, K), dev, dense=False), _row_stride(x),
         _tensor(weight, "weight", t, (N, K), dev, dense=False), _row_stride(weight),
-        None if bias is None else _tensor(bias, "bias", t, (N,), dev),
+        0 if bias is None else _tensor(bias, "bias", t, (N,), dev),
         _tensor(a, "a", t, (n, r, K), dev), _tensor(b, "b", t, (n, N, r), dev),
-        None if scale is None else _tensor(scale, "scale", torch.float32, (n,), dev),
+        0 if scale is None else _tensor(scale, "scale", torch.float32, (n,), dev),
         _tensor(index, "index", torch.int32, (M,), dev), _tensor(out, "out", out_dtype, (M, N), dev, dense=False),
         _row_stride(out))
-    L = capi.lib()
-    ref = byref(args)
-    keep, ws, nbytes = _workspace(L.mz_adapter_workspace_bytes(ref), workspace, dev)
-    if L.mz_adapter_linear(ref, ws, nbytes, _stream(dev)) != 0:
+    L = _lib()
+    keep, ws, nbytes = _workspace(L.mz_adapter_workspace_bytes(args), workspace, dev)
+    if L.mz_adapter_linear(args, ws, nbytes, _stream(dev)) != 0:
         _fail()
     return out

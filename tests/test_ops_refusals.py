@@ -51,7 +51,10 @@ def test_host_memory_is_refused():
 
 
 def test_struct_layout():
-    assert C.sizeof(capi.SampleArgs) == 4 * 4 + 3 * 8 + 14 * 8
+    assert C.sizeof(capi.SampleArgs) == 4 * 4 + 3 * 8 + 14 * 8 == ops._SAMPLE.size
+    assert C.sizeof(capi.AdapterArgs) == ops._ADAPTER.size
+    a = capi.SampleArgs.from_buffer_copy(ops._SAMPLE.pack(*range(1, 5), 0.5, 0.25, 0.125, *range(11, 25)))
+    assert (a.rows, a.top_k, a.temperature, a.min_p, a.logits, a.u, a.action, a.probs_stride) == (1, 4, 0.5, 0.125, 11, 15, 20, 24)
 
 
 def test_the_restatement_on_a_row_done_by_hand():
