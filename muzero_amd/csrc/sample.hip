@@ -82,9 +82,9 @@ __device__ __forceinline__ double weight(float z, const Scale& s) {
     return scaled(exp2_frac(y - (t - kRound)), low_word(t));
 }
 
-// The same for N entries side by side, for the passes over long rows: the constants of the polynomial stay in scalar registers
-// (compiled from exp2_frac each step is a move and a two-operand FMA).  The results must not go into DPP operations directly:
-// the compiler does not see that a vector instruction wrote them.
+// The same for N entries side by side: the constants of the polynomial stay in scalar registers (compiled from exp2_frac each step
+// is a move and a two-operand FMA).  The results must not go into DPP operations directly - the compiler does not see that a
+// vector instruction wrote them - but through a selection, an addition or the like.
 __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
     double r;
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
@@ -136,7 +136,8 @@ __device__ __forceinline__ uint32_t dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_rows(uint32_t v) {   // 0 in the rows that are not written
+__device__ __forceinline__ uint32_t dpp_rows(uint32_t v) {   // 0 in the rows that are not written and from lanes that are not there
+    if constexpr (ROWS == 0xf) return dpp<CTRL>(v);
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
 template <int J>
@@ -268,10 +269,15 @@ __device__ __forceinline__ int kept_prefix(const V (&ranked)[E], int count, cons
     if (rp.p < 1 || rp.m > 0) {
         double before[E], carry = 0;
         int nm = 0;
+        float z[E];
+        double all[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) z[e] = z_of(ranked[e]);
+        weights(z, sc, all);
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const bool in = e * W + lane < n;
-            const double w = in ? weight(z_of(ranked[e]), sc) : 0.0;
+            const double w = in ? all[e] : 0.0;
             const double s = wave_scan(w);
             before[e] = carry + one_lane_up(s);
             carry += lane_value(s, 63);
@@ -386,9 +392,9 @@ __global__ __launch_bounds__(W * kWaveRows) void k_sample_wave(SampleOp op) {
     }
     double w[E];
     int before = 0, kept = 0;
+    weights(z, sc, w);
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        w[e] = weight(z[e], sc);
         const u64 eq = __ballot(key[e] == border);
         const int nth = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(eq >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)eq, 0));
         before += __popcll(eq);
@@ -622,9 +628,13 @@ __device__ __forceinline__ void draw_ranked(const SampleOp& op, int row, Shared<
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = e * W + lane < keep ? (ranked[e] << 32) | (ranked[e] >> 32) : 0ull;   // ~index first: descending = index ascending
     wave_sort<E>(o, lane);
+    float z[E];
     double w[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) w[e] = o[e] ? weight(of_key((uint32_t)o[e]), sc) : 0.0;
+    for (int e = 0; e < E; e++) z[e] = of_key((uint32_t)o[e]);
+    weights(z, sc, w);
+#pragma unroll
+    for (int e = 0; e < E; e++) w[e] = o[e] ? w[e] : 0.0;
     double total;
     const int pos = wave_draw<E>(w, rp.u, &total);
     const u64 d = at_position<E>(o, pos);
@@ -659,12 +669,16 @@ __device__ __forceinline__ u64 border_of_list(Shared<NT>& sh, int n, int want, d
     wave_sort<E>(r, lane);
     int keep = want;
     if (want < 0) {
-        double carry = before;
+        double carry = before, w[E];
+        float z[E];
         keep = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) z[e] = z_of(r[e]);
+        weights(z, sc, w);
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const bool in = e * W + lane < n;
-            const double s = wave_scan(in ? weight(z_of(r[e]), sc) : 0.0);
+            const double s = wave_scan(in ? w[e] : 0.0);
             keep += __popcll(__ballot(in && carry + one_lane_up(s) < target));
             carry += lane_value(s, 63);
         }
