@@ -499,14 +499,21 @@ constexpr int kRing = 4;
 template <int BM>
 constexpr int kOrderBytes = 4 * BM * (int)sizeof(int);
 
+// Small tiles split K over KS groups of waves, each with a ring of its own: their sums are joined before the adapters' term, of
+// which each group takes a part of the columns.
+template <int BM>
+constexpr int kTileGroups = BM == 64 ? 2 : 1;
+
 template <typename T, int BM, int BN, int WM, int WN, bool DMA>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const float* part, int splits) {
-    constexpr int CE = kChunk<T>, NW = WM * WN, NTH = 64 * NW, MI = BM / WM / 16, NI = BN / WN / 16;
+__global__ __launch_bounds__(64 * WM * WN * kTileGroups<BM>, 2) void k_tile(AdapterOp op, const float* part, int splits) {
+    constexpr int KS = kTileGroups<BM>, CE = kChunk<T>, NW = WM * WN, NTH = 64 * NW * KS, MI = BM / WM / 16, NI = BN / WN / 16;
+    constexpr int NE = NI / KS;   // tiles of columns per wave after the sums are joined
     constexpr int STAGE = (int)tile_stage_bytes<BM, BN>();
     extern __shared__ __attribute__((aligned(16))) char lds[];   // (all of it dynamic: the opt-in covers 160 KiB of that)
     int *raw = reinterpret_cast<int*>(lds), *order = raw + BM, *key = order + BM, *nth = key + BM;
     char* smem = lds + kOrderBytes<BM>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, kq = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, all = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, kq = lane >> 4;
+    const int wave = all % NW, group = all / NW;
     // tiles of 8 row blocks x all column blocks in turn, so that what runs at one time shares operands in L2; consecutive
     // workgroups go to the 8 XCDs in turn: each takes a contiguous share
     const int ntm = (op.rows + BM - 1) / BM, ntn = (op.N + BN - 1) / BN, nt = ntm * ntn;
@@ -516,8 +523,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
         tile = xcd * per + min(xcd, rem) + at;
     }
     constexpr int G = 8;
-    const int group = tile / (G * ntn), gm = min(G, ntm - group * G), in = tile - group * G * ntn;
-    const int m0 = (group * G + in % gm) * BM, n0 = in / gm * BN;
+    const int band = tile / (G * ntn), gm = min(G, ntm - band * G), in = tile - band * G * ntn;
+    const int m0 = (band * G + in % gm) * BM, n0 = in / gm * BN;
     const int count = min(BM, op.rows - m0);
     order_rows<BM, NTH, false>(op, m0, count, raw, order, key, nth);
 
@@ -525,6 +532,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
     const T* wb = static_cast<const T*>(op.w) + n0 * op.w_stride;
     f32x4 acc[NI][MI] = {};
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    // whole stages of k: all, this group's [first, first + mine), and the most that a group has
+    const int full = op.K / (4 * CE), first = full * group / KS, mine = full * (group + 1) / KS - first, steps = (full + KS - 1) / KS;
+    char* ring = smem + group * kRing * STAGE;
     const auto read = [&](const char* st, u32x4 (&fx)[MI], u32x4 (&fw)[NI]) {
 #pragma unroll
         for (int j = 0; j < MI; j++) {
@@ -554,7 +564,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
     const int slot = lane & 3;
     if constexpr (DMA) {
         unsigned ox[LX], ow[LW];
-        const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem;
+        const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)ring;
 #pragma unroll
         for (int i = 0; i < LX; i++) {
             const int r = (wave * LX + i) * 16 + (lane >> 2);
@@ -565,8 +575,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
             const int r = (wave * LW + i) * 16 + (lane >> 2);
             ow[i] = (unsigned)(min(r, op.N - 1 - n0) * op.w_stride * sizeof(T)) + ((slot ^ (r >> 1 & 3)) << 4);
         }
-        const char* gx = reinterpret_cast<const char*>(xb);
-        const char* gw = reinterpret_cast<const char*>(wb);
+        const char* gx = reinterpret_cast<const char*>(xb) + first * 64ll;
+        const char* gw = reinterpret_cast<const char*>(wb) + first * 64ll;
         // written as one statement each, M0 with it: the compiler's own waits for such loads in flight would drain them at
         // every LDS read
         auto issue = [&](int stage) {
@@ -581,12 +591,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
             gw += 64;
         };
         constexpr int PER = LX + LW;
-        const int full = op.K / (4 * CE);
         // stage s + 1 has arrived in this wave's share (those behind it may be in flight) and this wave has read stage s; then
         // everyone's
         const auto arrive = [&](int s) {
-            if (s + 3 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER) : "memory");
-            else if (s + 2 < full) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER) : "memory");
+            if (s + 3 < mine) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER) : "memory");
+            else if (s + 2 < mine) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         };
         // While the matrix instructions work on stage s from registers, stage s + 1 is read from LDS and stage s + 4 goes where
@@ -594,9 +603,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
         u32x4 fx[2][MI], fw[2][NI];
         const auto step = [&](int s, u32x4 (&cx)[MI], u32x4 (&cw)[NI], u32x4 (&nx)[MI], u32x4 (&nw)[NI]) {
             arrive(s);
-            if (s + kRing < full) issue(s + kRing);
-            if (s + 1 < full) read(smem + ((s + 1) % kRing) * STAGE, nx, nw);
-            multiply(cx, cw);
+            if (s + kRing < mine) issue(s + kRing);
+            if (s + 1 < mine) read(ring + ((s + 1) % kRing) * STAGE, nx, nw);
+            if (KS == 1 || s < mine) multiply(cx, cw);
 #pragma unroll
             for (int g = 0; g < MI + NI; g++) {   // an LDS read between every few matrix instructions
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -606,14 +615,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
         if (full > 0) {
 #pragma unroll
             for (int s = 0; s < kRing; s++)
-                if (s < full) issue(s);
+                if (s < mine) issue(s);
             // (stage 0 of `arrive(-1)`: the ring holds one stage more than from then on)
-            if (full >= kRing) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * PER) : "memory");
+            if (mine >= kRing) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * PER) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-            read(smem, fx[0], fw[0]);
-            for (int s = 0; s < full; s += 2) {
+            read(ring, fx[0], fw[0]);
+            for (int s = 0; s < steps; s += 2) {
                 step(s, fx[0], fw[0], fx[1], fw[1]);
-                if (s + 1 < full) step(s + 1, fx[1], fw[1], fx[0], fw[0]);
+                if (s + 1 < steps) step(s + 1, fx[1], fw[1], fx[0], fw[0]);
             }
         }
     }
@@ -642,12 +651,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
 #pragma unroll
             for (int i = 0; i < RW; i++) *reinterpret_cast<uint32_t*>(st + tw[i]) = vw[i];
         };
-        const int full = op.K / (4 * CE);
         if (!DMA && full > 0) {
             constexpr int D = BM == 64 ? 4 : 2;   // stages on their way; behind the last whole one: that one again
             uint32_t vx[D][RX], vw[D][RW];
             const auto fetch = [&](int s, uint32_t (&vx)[RX], uint32_t (&vw)[RW]) {
-                const int k = min(s, full - 1) * 4 * CE;
+                const int k = (first + max(min(s, mine - 1), 0)) * 4 * CE;
 #pragma unroll
                 for (int i = 0; i < RX; i++) __builtin_memcpy(&vx[i], px[i] + k, 4);
 #pragma unroll
@@ -657,19 +665,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
 #pragma unroll
             for (int d = 0; d < D; d++) fetch(d, vx[d], vw[d]);
             constexpr int G = BM == 64 ? 2 : 1;   // stages to a barrier: small tiles have little to do in one
-            for (int s = 0; s < full; s += D)
+            for (int s = 0; s < steps; s += D)
 #pragma unroll
                 for (int d = 0; d < D; d += G) {
                     // (a step behind the last stage only turns the barrier)
 #pragma unroll
-                    for (int g = 0; g < G; g++) put(smem + (d + g) % (2 * G) * STAGE, vx[d + g], vw[d + g]);
+                    for (int g = 0; g < G; g++) put(ring + (d + g) % (2 * G) * STAGE, vx[d + g], vw[d + g]);
 #pragma unroll
                     for (int g = 0; g < G; g++) fetch(s + d + g + D, vx[d + g], vw[d + g]);
                     // the fetches stay in flight over the barrier; LDS: the slots that are written next were read a step ago
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
                     for (int g = 0; g < G; g++)
-                        if (s + d + g < full) compute(smem + (d + g) % (2 * G) * STAGE);
+                        if (s + d + g < mine) compute(ring + (d + g) % (2 * G) * STAGE);
                 }
         }
         if (full * 4 * CE < op.K) {
@@ -686,11 +694,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
 #pragma unroll
             for (int i = 0; i < RW; i++) vw[i] = rest(pw[i]);
             __syncthreads();   // the stages before have been read
-            put(smem, vx, vw);
+            if (group == 0) put(ring, vx, vw);
             __syncthreads();
-            compute(smem);
+            if (group == 0) compute(ring);
         }
     }
+    f32x4 sum[NE][MI];
+    if constexpr (KS == 2) {
+        static_assert(NTH * NE * MI * 16 <= KS * kRing * STAGE, "exchange");
+        f32x4* other = reinterpret_cast<f32x4*>(smem) + tid;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NE; i++)
+#pragma unroll
+            for (int j = 0; j < MI; j++) other[(i * MI + j) * NTH] = group ? acc[i][j] : acc[NE + i][j];
+        __syncthreads();
+        other += group ? -(NTH / 2) : NTH / 2;
+#pragma unroll
+        for (int i = 0; i < NE; i++)
+#pragma unroll
+            for (int j = 0; j < MI; j++) sum[i][j] = (group ? acc[NE + i][j] : acc[i][j]) + other[(i * MI + j) * NTH];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NE; i++)
+#pragma unroll
+            for (int j = 0; j < MI; j++) sum[i][j] = acc[i][j];
+    }
+    const int we = wn + group * NE * 16;   // this wave's first column of the tile from here on
 
     // ---- the adapters' term: t of this tile's rows, in its order -> LDS
     const int rp = padded_rank(op.rank), ts = rp + 4;
@@ -708,30 +738,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
     const bool per_row = op.rank <= 32 && BM < 8 * op.adapters;
     const auto add_term = [&](auto J) __attribute__((always_inline)) {
         constexpr int j = J.value;
-        const int p = wm + j * 16 + lr, mine = key[p];
-        if (per_row && mine >= 0) {
-            const float sc = op.scale ? op.scale[mine] : 1.f;
-            f32x4 d[NI] = {};
+        const int p = wm + j * 16 + lr, own = key[p];
+        if (per_row && own >= 0) {
+            const float sc = op.scale ? op.scale[own] : 1.f;
+            f32x4 d[NE] = {};
             for (int r = 0; r < op.rank; r += CE) {
                 float t[CE];
 #pragma unroll
                 for (int k = 0; k < CE; k++) t[k] = tl[p * ts + r + k];
 #pragma unroll
-                for (int ni = 0; ni < NI; ni++) {
+                for (int ni = 0; ni < NE; ni++) {
                     u32x4 c[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int n = min(n0 + wn + ni * 16 + kq * 4 + e, op.N - 1);
-                        c[e] = load_chunk(static_cast<const T*>(op.b) + ((long long)mine * op.N + n) * op.rank, r, op.rank);
+                        const int n = min(n0 + we + ni * 16 + kq * 4 + e, op.N - 1);
+                        c[e] = load_chunk(static_cast<const T*>(op.b) + ((long long)own * op.N + n) * op.rank, r, op.rank);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; e++) d[ni][e] += dot_chunk<T>(t, c[e]);
                 }
             }
 #pragma unroll
-            for (int ni = 0; ni < NI; ni++)
+            for (int ni = 0; ni < NE; ni++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[ni][j][e] = fmaf(sc, d[ni][e], acc[ni][j][e]);
+                for (int e = 0; e < 4; e++) sum[ni][j][e] = fmaf(sc, d[ni][e], sum[ni][j][e]);
         }
         float back = 1.f, to = 1.f;
         if constexpr (__is_same(T, _Float16)) {
@@ -747,13 +777,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
             to = ldexpf(1.f, -em);
         }
         // per adapter among the 16 rows
-        unsigned long long todo = __ballot(mine >= 0 && !per_row);
+        unsigned long long todo = __ballot(own >= 0 && !per_row);
         while (todo) {
-            const int i = __shfl(mine, __ffsll(todo) - 1);
-            const bool use = mine == i;
+            const int i = __shfl(own, __ffsll(todo) - 1);
+            const bool use = own == i;
             todo &= ~__ballot(use);
             const float sc = (op.scale ? op.scale[i] : 1.f) * back;
-            f32x4 d[NI] = {};
+            f32x4 d[NE] = {};
             for (int r0 = 0; r0 < rp; r0 += 16) {
                 u32x4 ft;   // 16 bits: k = 16 ranks of the leading part of t, then the same 16 of what it leaves; fp32: the 16 ranks
                 int rb;
@@ -775,8 +805,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
                     __builtin_memcpy(&ft, h, 16);
                 }
 #pragma unroll
-                for (int ni = 0; ni < NI; ni++) {
-                    const int n = min(n0 + wn + ni * 16 + lr, op.N - 1);
+                for (int ni = 0; ni < NE; ni++) {
+                    const int n = min(n0 + we + ni * 16 + lr, op.N - 1);
                     u32x4 v = load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + n) * op.rank, rb, op.rank);
                     if constexpr (sizeof(T) == 2) {
                         // an inf of B times the rest of t, which may have the other sign, is not wanted beside inf times its leading part
@@ -787,9 +817,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
             }
             if (use) {
 #pragma unroll
-                for (int ni = 0; ni < NI; ni++)
+                for (int ni = 0; ni < NE; ni++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[ni][j][e] = fmaf(sc, d[ni][e], acc[ni][j][e]);
+                    for (int e = 0; e < 4; e++) sum[ni][j][e] = fmaf(sc, d[ni][e], sum[ni][j][e]);
             }
         }
     };
@@ -799,11 +829,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tile(AdapterOp op, const fl
         constexpr int j = J.value;
         const int p = wm + j * 16 + lr;
         if (p < count) {
-            const int m = m0 + order[p], mine = key[p];
+            const int m = m0 + order[p], own = key[p];
 #pragma unroll
-            for (int ni = 0; ni < NI; ni++) {
-                const int n = n0 + wn + ni * 16 + kq * 4;
-                if (n < op.N) store4<T>(op, m, n, mine == kForeign ? f32x4{NAN, NAN, NAN, NAN} : acc[ni][j]);
+            for (int ni = 0; ni < NE; ni++) {
+                const int n = n0 + we + ni * 16 + kq * 4;
+                if (n < op.N) store4<T>(op, m, n, own == kForeign ? f32x4{NAN, NAN, NAN, NAN} : sum[ni][j]);
             }
         }
     };
@@ -863,16 +893,16 @@ void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int s
 template <typename T, int B, int WM, int WN>
 void launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
     const int nt = ((op.rows + B - 1) / B) * ((op.N + B - 1) / B);
-    const size_t es = sizeof(T), ring = kRing * tile_stage_bytes<B, B>(), tl = (size_t)B * (padded_rank(op.rank) + 4) * 4;
+    const size_t es = sizeof(T), ring = kTileGroups<B> * kRing * tile_stage_bytes<B, B>(), tl = (size_t)B * (padded_rank(op.rank) + 4) * 4;
     const bool dma = ((uintptr_t)op.x | (uintptr_t)op.w) % 16 == 0 && op.x_stride * es % 16 == 0 && op.w_stride * es % 16 == 0 &&
                      (long long)B * op.x_stride * (long long)es < (1ll << 31) && (long long)B * op.w_stride * (long long)es < (1ll << 31);
     const size_t lds = kOrderBytes<B> + (ring > tl ? ring : tl);
     if (dma) {
         lds_optin((const void*)k_tile<T, B, B, WM, WN, true>);
-        k_tile<T, B, B, WM, WN, true><<<dim3(nt), dim3(64 * WM * WN), lds, st>>>(op, part, splits);
+        k_tile<T, B, B, WM, WN, true><<<dim3(nt), dim3(64 * WM * WN * kTileGroups<B>), lds, st>>>(op, part, splits);
     } else {
         lds_optin((const void*)k_tile<T, B, B, WM, WN, false>);
-        k_tile<T, B, B, WM, WN, false><<<dim3(nt), dim3(64 * WM * WN), lds, st>>>(op, part, splits);
+        k_tile<T, B, B, WM, WN, false><<<dim3(nt), dim3(64 * WM * WN * kTileGroups<B>), lds, st>>>(op, part, splits);
     }
 }
 template <typename T, int BR>
