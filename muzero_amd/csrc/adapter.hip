@@ -1,10 +1,10 @@
 // mz_adapter_linear: y[m] = x[m] W^T + bias + s_i (x[m] A_i^T) B_i^T with i = index[m], the row's own adapter.
 //   k_shrink  t[m] = x[m] A_i^T in fp32, in parts over K, into the workspace.  The rows of a workgroup are ordered by adapter, so
 //             that up to 16 rows of one adapter share its A on the matrix cores.
-//   k_skinny  up to 64 rows (single tokens): bound by the bytes of W, which go straight from memory into the matrix
-//             instructions' registers, once; the waves of a workgroup split K.  With one or two rows of small rank t is computed
-//             by every workgroup for itself (A is read from L2), which saves the launch of k_shrink.
-//   k_tile    more rows: a tiled product, operands staged through LDS; the rows of a tile are ordered by adapter, so that
+//   k_skinny  up to 64 rows (single tokens), and more where there are few tiles: bound by the bytes of W, which go straight from
+//             memory into the matrix instructions' registers, once; the waves of a workgroup split K.  With one or two rows of
+//             small rank t is computed by every workgroup for itself (A is read from L2), which saves the launch of k_shrink.
+//   k_tile    else: a tiled product, operands staged through LDS; the rows of a tile are ordered by adapter, so that
 //             t B_i^T is one more step of the same matrix instructions on the accumulators, per adapter in 16 rows.
 // Both end with bias, the adapter's term and one rounding.  The adapter's term is computed apart from the accumulators and added
 // where the row uses that adapter: no row sees another row's adapter, whatever values it holds.
@@ -299,8 +299,9 @@ __device__ __forceinline__ void store4(const AdapterOp& op, int m, int n, f32x4 
     }
 }
 
-// ---- up to 64 rows -----------------------------------------------------------------------------------------------------------
-// Workgroup: 16 NT rows of W, all 16 MT rows of x; the waves split K by 128-byte steps; partial sums meet in LDS.
+// ---- few tiles -----------------------------------------------------------------------------------------------------------
+// Workgroup: 16 NT rows of W, 16 MT rows of x (up to 64 rows in all: all of them); the waves split K by 128-byte steps; partial sums
+// meet in LDS.
 // FJ > 0: t is computed here, FJ >= rows * rank tiles more tiles of 16 rows (of A).
 template <int MT>
 constexpr int kSkinnyWaves = MT == 1 ? 16 : 8;
@@ -320,6 +321,12 @@ __device__ __forceinline__ float dot_chunk(const float* t, u32x4 c) {
 template <typename T, int MT, int NT, int FJ>
 __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, const float* part, int splits) {
     constexpr int CE = kChunk<T>, NW = kSkinnyWaves<MT>, TILES = MT * NT, NTH = 64 * NW;
+    // the operation of this workgroup's rows
+    const int all_rows = op.rows, m0 = blockIdx.y * 16 * MT;
+    op.rows = min(16 * MT, all_rows - m0);
+    op.x = static_cast<const T*>(op.x) + m0 * op.x_stride;
+    op.y = static_cast<char*>(op.y) + m0 * op.y_stride * (op.out_type == kFp32 ? 4 : (int)sizeof(T));
+    op.index += m0;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     f32x4* red = reinterpret_cast<f32x4*>(smem);                              // [NW][TILES + FJ][64]
     int* adapter = reinterpret_cast<int*>(smem + skinny_lds<MT, NT, FJ>());   // [16 MT]
@@ -371,7 +378,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
     if (!FJ) {
         for (int q = tid; q < op.rows * (rp / 4); q += NTH) {
             const int m = q / (rp / 4), r = q % (rp / 4) * 4;
-            *reinterpret_cast<f32x4*>(tl + m * rp + r) = sum_parts(part, splits, op.rows, m, rp, r);
+            *reinterpret_cast<f32x4*>(tl + m * rp + r) = sum_parts(part, splits, all_rows, m0 + m, rp, r);
         }
     }
     while (more()) {
@@ -848,13 +855,32 @@ struct Plan {
     int splits, block;   // k_shrink: parts of K, rows per workgroup
 };
 constexpr int kCus = 256;
+// Tiles of 64 x 64 that leave half of the chip idle or more, each of which walks all of K alone: k_skinny's workgroups are smaller and
+// share K out over their waves.  Tiles against those, bf16 unless said: 720x939x98 (24 tiles) 33.1 and 22.8 us, 256x1024x1024 (64)
+// 15.8 and 13.3, 256x2048x1024 fp32 (64) 50.6 and 31.1, 512x4098x1024 (128) 45.4 and 39.3, 512x1024x1024 (128) 16.8 both,
+// 256x4096x2048 (128) 31.3 and 34.3, 256x4096x4096 (256) 33.5 and 60.9.
+constexpr int kFewTiles = 128;
 
 Plan make_plan(const AdapterOp& op) {
     Plan p{};
     const int rt = padded_rank(op.rank) / 16;
     const int pairs = (op.K * (op.type == kFp32 ? 4 : 2) + 127) / 128;
-    p.skinny = op.rows <= 64;
-    if (p.skinny) {
+    const auto tiles = [&](int m, int n) { return (long long)((op.rows + m - 1) / m) * ((op.N + n - 1) / n); };
+    p.skinny = op.rows <= 64 || tiles(64, 64) <= kFewTiles;
+    if (op.rows > 64 && p.skinny) {
+        // what a workgroup brings from L2, times the rounds of workgroups on the chip; among equals the fewest workgroups
+        long long least = 0;
+        for (int mt = 4; mt >= 1; mt--)
+            for (int nt = 3; nt >= 1; nt--) {
+                const long long cost = (tiles(16 * mt, 16 * nt) + kCus - 1) / kCus * (mt + nt);
+                if (!least || cost < least) {
+                    least = cost;
+                    p.mt = mt;
+                    p.nt = nt;
+                }
+            }
+        p.block = op.rows <= 1024 ? 16 : 128;
+    } else if (p.skinny) {
         p.mt = (op.rows + 15) / 16;
         // rows of W per workgroup: what leaves the fewest rounds of workgroups on the chip; among equals the most, as every
         // workgroup reads x
@@ -867,8 +893,7 @@ Plan make_plan(const AdapterOp& op) {
         p.block = 16;
     } else {
         p.block = op.rows <= 1024 ? 16 : 128;
-        auto tiles = [&](int b) { return (long long)((op.rows + b - 1) / b) * ((op.N + b - 1) / b); };
-        p.tile = tiles(256) >= kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
+        p.tile = tiles(256, 256) >= kCus ? 256 : tiles(128, 128) >= kCus ? 128 : 64;
     }
     const int blocks = (op.rows + p.block - 1) / p.block;
     int s = (2 * kCus + blocks - 1) / blocks;
@@ -880,9 +905,9 @@ Plan make_plan(const AdapterOp& op) {
 
 template <typename T, int MT, int NT, int FJ>
 void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
-    const size_t lds = skinny_lds<MT, NT, FJ>() + 16 * MT * 4 + (size_t)op.rows * padded_rank(op.rank) * 4;
+    const size_t lds = skinny_lds<MT, NT, FJ>() + 16 * MT * 4 + (size_t)std::min(op.rows, 16 * MT) * padded_rank(op.rank) * 4;
     lds_optin((const void*)k_skinny<T, MT, NT, FJ>);
-    k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT)), dim3(64 * kSkinnyWaves<MT>), lds, st>>>(op, part, splits);
+    k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT), (op.rows + 16 * MT - 1) / (16 * MT)), dim3(64 * kSkinnyWaves<MT>), lds, st>>>(op, part, splits);
 }
 template <typename T, int MT, int FJ>
 void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits, int nt) {
