@@ -176,11 +176,12 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
 
 // ---- t = x A^T -------------------------------------------------------------------------------------------------------------
 // Workgroup (block of BR rows, part of K): jobs of up to 16 rows of one adapter, a wave each.  part[s][row][padded rank].
-// 16 rows: a wave for every job there can be, in 4 workgroups; 128 rows: 8 waves, as many as 8 rank tiles leave registers for.
+// 16 rows: a wave for every job there can be, in 4 workgroups; 128 rows: 8 waves, as many as 8 rank tiles leave registers for, in 2
+// (2928 rows of 53 adapters, fp32: 15.7 us for the whole call with 2, 19.8 with one, 13.5 with 4; 16384 rows of 32: 29.2, 29.9, 31.2).
 template <int BR>
 constexpr int kShrinkWaves = BR == 16 ? 4 : 8;
 template <int BR>
-constexpr int kShrinkParts = BR == 16 ? 4 : 1;   // workgroups that share the jobs of a block
+constexpr int kShrinkParts = BR == 16 ? 4 : 2;   // workgroups that share the jobs of a block
 template <typename T, int RT, int BR>
 __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, float* part, int splits) {
     constexpr int CE = kChunk<T>;
@@ -213,10 +214,10 @@ __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, 
         f32x4 acc[RT] = {};
         int k = p0;
         constexpr int U = RT == 1 ? 4 : RT == 2 ? (BR == 16 ? 3 : 4) : RT == 8 && BR == 16 ? 1 : 2;   // what the registers hold
-        for (; k + U <= pf; k += U) {
-            u32x4 fx[U][2], fa[U][RT][2];
+        const auto whole = [&](auto U) __attribute__((always_inline)) {   // that many whole steps
+            u32x4 fx[U.value][2], fa[U.value][RT][2];
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int u = 0; u < U.value; u++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     fx[u][h] = load16(x + (k + u) * 8 * CE + h * 4 * CE);
@@ -225,12 +226,15 @@ __global__ __launch_bounds__(64 * kShrinkWaves<BR>) void k_shrink(AdapterOp op, 
                 }
             __builtin_amdgcn_sched_barrier(0);   // all loads in flight before the first use
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int u = 0; u < U.value; u++)
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int q = 0; q < RT; q++) acc[q] = mma<T>(fa[u][q][h], fx[u][h], acc[q]);
-        }
+            k += U.value;
+        };
+        while (k + U <= pf) whole(std::integral_constant<int, U>{});
+        while (U > 1 && k < pf) whole(std::integral_constant<int, 1>{});
         for (; k < p1; k++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -896,7 +900,9 @@ Plan make_plan(const AdapterOp& op) {
         p.tile = tiles(256, 256) >= kCus ? 256 : tiles(128, 128) >= kCus ? 128 : 64;
     }
     const int blocks = (op.rows + p.block - 1) / p.block;
-    int s = (2 * kCus + blocks - 1) / blocks;
+    // parts of K: a round of k_shrink's workgroups on the chip (8192x1024x1024 bf16: 4 parts 56.5 us, 2 59.8, 8 59.7; 16384x162x82 fp32:
+    // 2 parts 29.2 us, 3 31.6, 1 29.4)
+    const int s = (kCus * (p.block == 16 ? 2 : 1) + blocks - 1) / blocks;
     p.splits = s < 1 ? 1 : s > 16 ? 16 : s;
     if (p.splits > (pairs + 1) / 2) p.splits = (pairs + 1) / 2;
     if (p.fused) p.splits = 0;
