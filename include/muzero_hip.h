@@ -293,7 +293,8 @@ int mz_search_moves_injected_noalloc(mz_ctx* ctx, int B, const uint8_t* legal, c
  *    the call's work is done (NULL when that is 0): calls in flight at the same time, and graphs that may run at the same time,
  *    need one each.  Its contents before and after do not matter;
  *  - arguments are checked on the host before anything is queued: -1 and mz_last_error(NULL) (per thread) otherwise.  Calls
- *    from several threads are independent.  Strides are in elements; rows are contiguous; outputs must not overlap inputs;
+ *    from several threads are independent.  Strides are in elements; rows are contiguous; outputs that overlap inputs,
+ *    one another or the workspace are refused (columns of the same wider rows may lie side by side);
  *  - rows == 0 is a successful call that does nothing. */
 enum { MZ_DTYPE_FP32 = 0, MZ_DTYPE_BF16 = 1, MZ_DTYPE_F16 = 2 }; /* the numbers of MZ_PRECISION_* */
 
@@ -336,7 +337,7 @@ int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t worksp
  * 16 bits on 16-bit matrix instructions, fp32 on fp32 ones), rounded once to y's type.  Rows do not influence one another:
  * a row's inf or NaN, or an adapter's, stay with the rows that use them. */
 typedef struct mz_adapter_args {
-    int32_t rows, in_features, out_features; /* out_features <= 2^26, ceil(rows / 256) * ceil(out_features / 256) <= 2^22 */
+    int32_t rows, in_features, out_features; /* both features <= 2^26, ceil(rows / 256) * ceil(out_features / 256) <= 2^21 */
     int32_t rank, adapters;         /* rank: 1 .. 128; shorter adapters are padded with zeros */
     int32_t dtype;                  /* MZ_DTYPE_* of x, weight, bias, a, b */
     int32_t out_dtype;              /* of y: dtype, or MZ_DTYPE_FP32 */

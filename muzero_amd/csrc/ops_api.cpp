@@ -14,13 +14,29 @@ constexpr int kMaxRank = 128;
 constexpr int kMaxSampleRows = 1 << 21;     // a workgroup of up to 1024 threads each: below 2^32 threads
 constexpr int kMaxSampleActions = 262144;   // 2^18: sample.hip's histogram masses are sums of 2^46 in 64 bits
 
-// The device all operands live on: the first pointer names it, every other one must agree.
+// The device all operands live on: the first pointer names it, every other one must agree.  What a call writes must not overlap
+// anything else of it.
 struct Operands {
     int device = -1;
     const char* bad = nullptr;
     std::string why;
-    void add(const void* p, const char* name, size_t align) {
+    struct Block {   // rows of `width` bytes, `pitch` bytes apart
+        const char* name;
+        uintptr_t at;
+        unsigned __int128 end;
+        uintptr_t pitch, width;
+        bool written;
+    } block[16];
+    int blocks = 0;
+    void in(const void* p, const char* name, size_t elem, size_t rows, size_t stride, size_t width) { add(p, name, elem, rows, stride * elem, width * elem, false); }
+    void out(const void* p, const char* name, size_t elem, size_t rows, size_t stride, size_t width) { add(p, name, elem, rows, stride * elem, width * elem, true); }
+    void add(const void* p, const char* name, size_t align, size_t rows, size_t pitch, size_t width, bool written) {
         if (bad || !p) return;
+        const uintptr_t at0 = reinterpret_cast<uintptr_t>(p);
+        const Block b{name, at0, (unsigned __int128)(rows - 1) * pitch + width + at0, pitch, width, written};
+        for (int i = 0; i < blocks; i++)
+            if ((written || block[i].written) && overlap(block[i], b)) return fail(name, (std::string("overlaps ") + block[i].name).c_str());
+        block[blocks++] = b;
         hipPointerAttribute_t at;
         if (hipPointerGetAttributes(&at, p) != hipSuccess) {
             (void)hipGetLastError();
@@ -33,6 +49,12 @@ struct Operands {
             if (device < 0) device = at.device;
             else if (device != at.device) fail(name, "is memory of another device");
         }
+    }
+    static bool overlap(const Block& a, const Block& b) {
+        if (a.end <= b.at || b.end <= a.at) return false;
+        if (a.pitch != b.pitch || a.pitch == 0) return true;
+        const uintptr_t d = (b.at % a.pitch + a.pitch - a.at % a.pitch) % a.pitch;   // columns of the same wide rows
+        return !(d >= a.width && d + b.width <= a.pitch);
     }
     void fail(const char* name, const char* what) {
         bad = name;
@@ -62,7 +84,7 @@ int run_op(Operands& o, void* workspace, size_t have, size_t need, void* stream,
     if (need) {
         if (!workspace || have < need)
             return op_fail("workspace has " + std::to_string(workspace ? have : 0) + " bytes, needs " + std::to_string(need));
-        o.add(workspace, "workspace", 256);
+        o.add(workspace, "workspace", 256, 1, need, need, true);
     }
     if (o.bad) return op_fail(o.why);
     int dev = o.device;
@@ -125,8 +147,9 @@ SampleOp sample_op(const mz_sample_args& a) {
 const char* check_adapter(const mz_adapter_args* a) {
     if (!a) return "args is NULL";
     if (a->rows < 0) return "rows < 0";
-    if (((long long)a->rows + 255) / 256 * (((long long)a->out_features + 255) / 256) > (1 << 22) || a->out_features > (1 << 26)) return "too many outputs for one call";
     if (a->in_features < 1 || a->out_features < 1) return "in_features and out_features must be >= 1";
+    if (a->in_features > (1 << 26)) return "in_features must be at most 67108864";   // its bytes fit an int
+    if (((long long)a->rows + 255) / 256 * (((long long)a->out_features + 255) / 256) > (1 << 21) || a->out_features > (1 << 26)) return "too many outputs for one call";
     if (a->rank < 1 || a->rank > kMaxRank) return "rank must be 1 .. 128";
     if (a->adapters < 1) return "adapters must be >= 1";
     if (!known_type(a->dtype)) return "unknown dtype";
@@ -182,17 +205,18 @@ int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t worksp
         const SampleOp op = sample_op(*args);
         if (op.rows == 0) return 0;
         Operands o;
-        o.add(op.logits, "logits", type_bytes(op.type));
-        o.add(op.legal, "legal", 1);
-        o.add(op.u, "u", 8);
-        o.add(op.row_temperature, "row_temperature", 8);
-        o.add(op.row_top_k, "row_top_k", 4);
-        o.add(op.row_top_p, "row_top_p", 8);
-        o.add(op.row_min_p, "row_min_p", 8);
-        o.add(op.action, "action", 4);
-        o.add(op.logprob, "logprob", 4);
-        o.add(op.kept, "kept", 4);
-        o.add(op.probs, "probs", 4);
+        const size_t n = op.rows, A = op.actions;
+        o.in(op.logits, "logits", type_bytes(op.type), n, op.row_stride, A);
+        o.in(op.legal, "legal", 1, n, op.legal_stride, A);
+        o.in(op.u, "u", 8, n, 1, 1);
+        o.in(op.row_temperature, "row_temperature", 8, n, 1, 1);
+        o.in(op.row_top_k, "row_top_k", 4, n, 1, 1);
+        o.in(op.row_top_p, "row_top_p", 8, n, 1, 1);
+        o.in(op.row_min_p, "row_min_p", 8, n, 1, 1);
+        o.out(op.action, "action", 4, n, 1, 1);
+        o.out(op.logprob, "logprob", 4, n, 1, 1);
+        o.out(op.kept, "kept", 4, n, 1, 1);
+        o.out(op.probs, "probs", 4, n, op.probs_stride, A);
         return run_op(o, workspace, workspace_bytes, sample_workspace_bytes(op), stream, [&](hipStream_t st) { return launch_sample(st, op, workspace); });
     });
 }
@@ -206,14 +230,15 @@ int mz_adapter_linear(const mz_adapter_args* args, void* workspace, size_t works
         if (op.rows == 0) return 0;
         const size_t es = type_bytes(op.type);
         Operands o;
-        o.add(op.x, "x", es);
-        o.add(op.w, "weight", es);
-        o.add(op.bias, "bias", es);
-        o.add(op.a, "a", es);
-        o.add(op.b, "b", es);
-        o.add(op.scale, "scale", 4);
-        o.add(op.index, "index", 4);
-        o.add(op.y, "y", type_bytes(op.out_type));
+        const size_t M = op.rows, K = op.K, N = op.N, n = op.adapters;
+        o.in(op.x, "x", es, M, op.x_stride, K);
+        o.in(op.w, "weight", es, N, op.w_stride, K);
+        o.in(op.bias, "bias", es, 1, N, N);
+        o.in(op.a, "a", es, n * op.rank, K, K);
+        o.in(op.b, "b", es, n * N, op.rank, op.rank);
+        o.in(op.scale, "scale", 4, n, 1, 1);
+        o.in(op.index, "index", 4, M, 1, 1);
+        o.out(op.y, "y", type_bytes(op.out_type), M, op.y_stride, N);
         return run_op(o, workspace, workspace_bytes, adapter_workspace_bytes(op), stream, [&](hipStream_t st) { return launch_adapter(st, op, workspace); });
     });
 }

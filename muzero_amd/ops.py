@@ -121,7 +121,7 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     top_k, p_k = _setting(top_k, "top_k", torch.int32, rows, dev)
     top_p, p_p = _setting(top_p, "top_p", torch.float64, rows, dev)
     min_p, p_m = _setting(min_p, "min_p", torch.float64, rows, dev)
-    if top_k >= 2**31:
+    if type(top_k) is int and top_k >= 2**31:
         top_k = 2**31 - 1
     if out is None:
         on = logits.device
@@ -131,6 +131,8 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
             out["probs"] = torch.empty(B, A, dtype=torch.float32, device=on)
     get = out.get
     action, logprob, kept, pr = get("action"), get("logprob"), get("kept"), get("probs")
+    if logprob is not None and getattr(logprob, "requires_grad", False) or pr is not None and getattr(pr, "requires_grad", False):
+        _no_gradient()
     try:
         args = _SAMPLE.pack(
             B, A, DTYPES[t], top_k, temperature, top_p, min_p,
@@ -141,7 +143,7 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
             0 if kept is None else _tensor(kept, "out['kept']", torch.int32, rows, dev),
             0 if pr is None else _tensor(pr, "out['probs']", torch.float32, shape, dev, dense=False),
             0 if pr is None else _row_stride(pr))
-    except struct.error as e:
+    except (struct.error, OverflowError, TypeError) as e:
         raise capi.MuZeroError(f"temperature, top_k, top_p and min_p must be numbers in range ({e})") from None
     L = _lib()
     keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(args), workspace, dev)
@@ -161,7 +163,7 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
     if dev < 0 or t not in DTYPES:
         raise capi.MuZeroError(f"x: must be on a GPU and float32, bfloat16 or float16, not {t} on {x.device}")
     if (x.requires_grad or weight.requires_grad or a.requires_grad or getattr(b, "requires_grad", False)
-            or bias is not None and bias.requires_grad or scale is not None and scale.requires_grad):
+            or getattr(bias, "requires_grad", False) or getattr(scale, "requires_grad", False) or getattr(out, "requires_grad", False)):
         _no_gradient()
     M, K = x.shape
     n, r, _ = a.shape

@@ -99,3 +99,16 @@ def test_adapter_of_no_rows():
 
 def test_policy_struct_layouts():
     assert C.sizeof(capi.PolicySampling) == 32 and C.sizeof(capi.PolicyOutputs) == 48
+
+
+@pytest.mark.parametrize("change,text", [(dict(in_features=2**26 + 1, x_stride=2**26 + 1, weight_stride=2**26 + 1), "in_features"),
+                                         (dict(rows=2**30), "too many"), (dict(rows=2**20, out_features=2**20, y_stride=2**20), "too many"),
+                                         (dict(out_features=2**26 + 1, y_stride=2**26 + 1), "too many")])
+def test_adapter_refuses_sizes_beyond_its_limits(change, text):
+    a = capi.AdapterArgs(rows=2, in_features=64, out_features=32, rank=4, adapters=2, dtype=1, out_dtype=1, x=64, x_stride=64,
+                         weight=64, weight_stride=64, a=64, b=64, index=64, y=64, y_stride=32)
+    for k, v in change.items():
+        setattr(a, k, v)
+    assert capi.lib().mz_adapter_linear(C.byref(a), None, 0, None) == -1
+    assert text in last_error()
+    assert capi.lib().mz_adapter_workspace_bytes(C.byref(a)) == 0
