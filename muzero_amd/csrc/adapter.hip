@@ -1,7 +1,7 @@
 // mz_adapter_linear: y[m] = x[m] W^T + bias + s_i (x[m] A_i^T) B_i^T with i = index[m], the row's own adapter.
 //   k_shrink  t[m] = x[m] A_i^T in fp32, in parts over K, into the workspace.  The rows of a workgroup are ordered by adapter, so
 //             that up to 16 rows of one adapter share its A on the matrix cores.
-//   k_skinny  up to 64 rows (single tokens), and more where there are few tiles: bound by the bytes of W, which go straight from
+//   k_skinny  up to 48 rows (single tokens), and more where there are few tiles: bound by the bytes of W, which go straight from
 //             memory into the matrix instructions' registers, once; the waves of a workgroup split K.  With one or two rows of
 //             small rank t is computed by every workgroup for itself (A is read from L2), which saves the launch of k_shrink.
 //   k_tile    else: a tiled product, operands staged through LDS; the rows of a tile are ordered by adapter, so that
@@ -304,8 +304,9 @@ __device__ __forceinline__ void store4(const AdapterOp& op, int m, int n, f32x4 
 }
 
 // ---- few tiles -----------------------------------------------------------------------------------------------------------
-// Workgroup: 16 NT rows of W, 16 MT rows of x (up to 64 rows in all: all of them); the waves split K by 128-byte steps; partial sums
-// meet in LDS.
+// Workgroup: 16 NT rows of W, 16 MT rows of x; the waves split K by 128-byte steps; partial sums meet in LDS.
+// One row, 4096 to 4096 bf16: 13.3 us, 2.5 TB/s; 48 rows, 4096 to 11000 fp16 with 48 adapters of rank 32: 40 us, 3.3 TB/s (a large copy
+// moves 5.1): bound by how many loads of W are in flight, which the registers bound.
 // FJ > 0: t is computed here, FJ >= rows * rank tiles more tiles of 16 rows (of A).
 template <int MT>
 constexpr int kSkinnyWaves = MT == 1 ? 16 : 8;
@@ -500,8 +501,10 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------
 // LDS: a ring of stages, each 64 bytes of k (4 chunks) of BM rows of x and BN rows of W.  Chunk c of row r stands at slot
 // c ^ (r >> 1 & 3): the 8 lanes that an LDS read serves at a time then hit 8 different 16-byte columns.
-// DMA: rows of both operands are 16-byte aligned: global -> LDS without registers, three stages ahead.  Otherwise through
-// registers, one stage ahead.
+// DMA: rows of both operands are 16-byte aligned: global -> LDS without registers, three stages ahead.  Otherwise through registers.
+// With and without it, bf16: 8192x4096x4096 331 and 368 us, 2048x2048x2048 49.3 and 59.3, 1000x2048x2000 37.0 and 37.4.
+// Bound by LDS reads beside the matrix instructions where tiles are large (8192x4096x4096: 280 us, 0.98 PFLOP/s, the library's bare product
+// 1.33), by what each workgroup brings from L2 where they are small (1000x2050x1999: 37.5 us, 268 MB, 7 TB/s).
 template <int BM, int BN>
 constexpr size_t tile_stage_bytes() {
     return (size_t)(BM + BN) * 64;
@@ -746,7 +749,9 @@ __global__ __launch_bounds__(64 * WM * WN * kTileGroups<BM>, 2) void k_tile(Adap
     __syncthreads();
     // With few rows per adapter (by the numbers of both, not by the data: the two ways round differently, and a row's result must
     // not depend on its neighbours) every lane takes the B of its own row; else the matrix instructions take 16 rows at a time.
-    const bool per_row = op.rank <= 32 && BM < 8 * op.adapters;
+    // By rows and by matrix instructions, in mixed order: 2000x1024x1024 bf16 rank 16 (tiles of 64) 8 adapters 22.8 and 23.6 us,
+    // 12 22.8 and 25.5, 64 29.5 and 41.8; 4096x512x2304 (of 128) 16 adapters 62.3 and 66.1, 32 65.9 and 89.3.
+    const bool per_row = op.rank <= 32 && BM <= 8 * op.adapters;
     const auto add_term = [&](auto J) __attribute__((always_inline)) {
         constexpr int j = J.value;
         const int p = wm + j * 16 + lr, own = key[p];
@@ -864,14 +869,22 @@ constexpr int kCus = 256;
 // 15.8 and 13.3, 256x2048x1024 fp32 (64) 50.6 and 31.1, 512x4098x1024 (128) 45.4 and 39.3, 512x1024x1024 (128) 16.8 both,
 // 256x4096x2048 (128) 31.3 and 34.3, 256x4096x4096 (256) 33.5 and 60.9.
 constexpr int kFewTiles = 128;
+// Above it, W is streamed for few rows.  That against tiles, W from memory, bf16, 4096 to 11000: 16 rows 30.8 and 38.2 us, 32 rows 32.8
+// and 45.6, 48 rows 37.4 and 45.3, 64 rows 43.0 and 45.3; 4096 to 16384, where the last round of workgroups is not full: 32 rows 49.0
+// and 52.8, 48 rows 56.9 and 51.5, 64 rows 64.1 and 52.2.  fp32, 4096 to 11000: 32 rows 69.4 and 92.5, 48 rows 104 and 91.9.
+constexpr int kSkinnyRows16 = 48, kSkinnyRows32 = 32;
 
 Plan make_plan(const AdapterOp& op) {
     Plan p{};
     const int rt = padded_rank(op.rank) / 16;
     const int pairs = (op.K * (op.type == kFp32 ? 4 : 2) + 127) / 128;
     const auto tiles = [&](int m, int n) { return (long long)((op.rows + m - 1) / m) * ((op.N + n - 1) / n); };
-    p.skinny = op.rows <= 64 || tiles(64, 64) <= kFewTiles;
-    if (op.rows > 64 && p.skinny) {
+    const int few_rows = op.type == kFp32 ? kSkinnyRows32 : kSkinnyRows16;
+    p.skinny = op.rows <= few_rows || tiles(64, 64) <= kFewTiles;
+    // few rows per adapter, whatever their number: smaller blocks order faster and spread further.  Blocks of 16 and of 128 rows:
+    // 100x4096x1024 bf16 21.5 and 27.5 us, 720x939x98 fp16 23.6 and 26.8, 1000x2050x1999 43.9 and 43.1, 1024x1024x2048 25.1 and 22.5
+    p.block = op.rows < 1024 ? 16 : 128;
+    if (p.skinny && op.rows > few_rows) {
         // what a workgroup brings from L2, times the rounds of workgroups on the chip; among equals the fewest workgroups
         long long least = 0;
         for (int mt = 4; mt >= 1; mt--)
@@ -883,7 +896,6 @@ Plan make_plan(const AdapterOp& op) {
                     p.nt = nt;
                 }
             }
-        p.block = op.rows <= 1024 ? 16 : 128;
     } else if (p.skinny) {
         p.mt = (op.rows + 15) / 16;
         // rows of W per workgroup: what leaves the fewest rounds of workgroups on the chip; among equals the most, as every
@@ -892,12 +904,16 @@ Plan make_plan(const AdapterOp& op) {
         p.nt = 3;
         for (int nt = 2; nt >= 1; nt--)
             if (rounds(nt) < rounds(p.nt)) p.nt = nt;
-        // every workgroup reads the A of all rows: only while that is little
-        p.fused = op.rows * rt <= 2;
-        p.block = 16;
+        // Every workgroup reads the A of all rows: only while that is little.  Fused and not, one row of rank 16 unless said, bf16:
+        // 4096 to 11000 21.7 and 22.7 us, 8192 to 8192 31.1 and 40.5; 2048 to 2048, rank 32 10.3 and 10.5; two rows, 1024 to 1024
+        // 7.8 and 9.0, 4096 to 4096 16.5 and 13.6; fp32: 162 to 82 5.5 and 8.6, 4096 to 4096 27.3 and 22.4
+        const int es = op.type == kFp32 ? 4 : 2, t_tiles = op.rows * rt;
+        p.fused = t_tiles <= 2 && ((long long)t_tiles * op.K * es <= 8192 || (t_tiles == 1 && es == 2));
     } else {
-        p.block = op.rows <= 1024 ? 16 : 128;
-        p.tile = tiles(256, 256) >= kCus ? 256 : tiles(128, 128) >= kCus ? 128 : 64;
+        // The larger tile reads less, the smaller one fills the chip: the largest that still does.  Sides 64, 128, 256, bf16:
+        // 4096x4096x4096 320, 207, 170 us; 2048x4096x4096 168, 111, 146; 512x4096x4096 59, 74, 149; 16384x2048x128 63, 73, 127.
+        // fp32, whose matrix instructions are slow enough for 128: 16384x512x512 118, 95, 168; 2048x2048x2048 161, 164, 523.
+        p.tile = op.type != kFp32 && tiles(256, 256) >= kCus ? 256 : tiles(128, 128) >= kCus ? 128 : 64;
     }
     const int blocks = (op.rows + p.block - 1) / p.block;
     // parts of K: a round of k_shrink's workgroups on the chip (8192x1024x1024 bf16: 4 parts 56.5 us, 2 59.8, 8 59.7; 16384x162x82 fp32:
@@ -963,8 +979,8 @@ hipError_t launch_typed(hipStream_t st, const AdapterOp& op, void* workspace) {
         else if (p.mt == 2) launch_skinny<T, 2, 0>(st, op, part, p.splits, p.nt);
         else if (p.mt == 3) launch_skinny<T, 3, 0>(st, op, part, p.splits, p.nt);
         else launch_skinny<T, 4, 0>(st, op, part, p.splits, p.nt);
-    } else if (p.tile == 256) {
-        launch_tile<T, 256, 4, 2>(st, op, part, p.splits);
+    } else if (sizeof(T) == 2 && p.tile == 256) {
+        if constexpr (sizeof(T) == 2) launch_tile<T, 256, 4, 2>(st, op, part, p.splits);
     } else if (p.tile == 128) {
         launch_tile<T, 128, 2, 2>(st, op, part, p.splits);
     } else {

@@ -10,12 +10,17 @@
 // (histograms, whose LDS atomics arrive in any order) in exact integers, so a row's answer is a function of the row alone.
 //
 //   A <= 256   k_sample_wave: a wavefront per row, the row in registers (<= 4 entries a lane); ranking = bitonic sort of
-//              (key, index) pairs over the lanes.
+//              the keys over the lanes.  Bound by the issue of vector instructions, 64-bit exponentials first: 16384 rows of 82 with
+//              top-k, top-p and min-p of their own and probabilities written: 22 us, 0.55 TB/s.  (By a workgroup per row, as
+//              below, 4096 rows of 256 take 58 us instead of 13.)
 //   A >  256   k_sample_block: a workgroup per row, passes over the row (its re-reads hit L2 / the memory-side cache):
 //              maximum -> candidates.  With top-k <= 128 the k-th largest of 256 partial maxima bounds the k-th entry from
 //              below, so about k entries pass and one wave finishes as above.  A nucleus without top-k needs the mass of the
 //              whole row: a histogram of count and mass over log2-spaced bins gives it, and the bin the border falls in;
-//              small nuclei are finished by one wave, large ones narrow the border's bin to one (value, index).
+//              small nuclei are finished by one wave, large ones narrow the border's bin to one (value, index).  256 rows of 131072
+//              bf16 entries: with top-k 50 30 us (2.2 TB/s), with top-p 0.9 131 us, bound by vector and LDS atomic work per entry.
+//   few long rows   k_sample_maxima + k_sample_split: 2 to 16 workgroups per row, the last to finish ranks the candidates of
+//              all; 64 rows of 50257 fp32 entries, top-k 40 and top-p 0.95: 16 us, bound by latency (two launches, one wave's end).
 #include "ops.h"
 
 #include <float.h>
@@ -29,7 +34,7 @@ constexpr int kWaveRows = 4;       // rows (waves) per workgroup of k_sample_wav
 constexpr int kList = 256;         // candidates one wave ranks in registers
 constexpr int kFastK = 128;        // top-k up to which the bound by partial maxima is tried
 constexpr int kBins = 2048;
-constexpr int kFix = 45;           // fraction bits of a histogram mass: 2^46 per entry * 2^17 entries < 2^63
+constexpr int kFix = 45;           // fraction bits of a histogram mass: 2^45.51 per entry * 2^18 entries < 2^64
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
@@ -1282,9 +1287,10 @@ __global__ __launch_bounds__(kSplitThreads) void k_sample_split(SampleOp op, Spl
 }
 
 // 0: a workgroup per row.  Splitting pays while workgroups of one row each leave most of the chip idle, and a row is long enough
-// to be worth a second launch.
+// to be worth a second launch: one row of 131072 bf16 entries (top-k 50) 20.8 us whole, 12.2 by 16 workgroups; 64 rows 22.0, by 4 16.4;
+// 64 rows of 50000 14.9 and 13.8, of 32768 12.8 and 13.0, of 24000 12.1 and 13.6; 100 rows of 131072 22.2, by 2 19.4, of 50000 15.4 and 15.5.
 inline int log_splits(const SampleOp& op) {
-    if (op.actions < 16384 || op.rows > 128) return 0;
+    if (op.rows > 128 || op.actions < (op.rows <= 64 ? 49152 : 98304)) return 0;
     return op.rows <= 16 ? 4 : op.rows <= 32 ? 3 : op.rows <= 64 ? 2 : 1;
 }
 
@@ -1295,7 +1301,10 @@ hipError_t launch_typed(hipStream_t st, const SampleOp& op, void* workspace) {
         if (op.actions <= W) k_sample_wave<T, 1><<<grid, block, 0, st>>>(op);
         else if (op.actions <= 2 * W) k_sample_wave<T, 2><<<grid, block, 0, st>>>(op);
         else k_sample_wave<T, 4><<<grid, block, 0, st>>>(op);
-    } else if (op.actions <= 8192) {
+    } else if (op.actions <= 8192 || (op.rows > 256 && op.actions <= 64ll * op.rows)) {
+        // Several workgroups to a CU hide one another's serial parts; a CU with one row needs all its waves.  256 and 1024 threads, top-p
+        // 0.9 of bf16: 64 rows of 8192 10.9 and 13.2 us, 256 of 16384 39.2 and 33.9, 512 of 16384 47.4 and 63.6, 512 of 65536 156 and 148,
+        // 1024 of 32768 139 and 171, 2048 of 16384 141 and 246, 256 of 131072 240 and 131
         k_sample_block<T, 256><<<dim3(op.rows), dim3(256), 0, st>>>(op);
     } else if (const int ls = log_splits(op)) {
         SplitRow* rows = static_cast<SplitRow*>(workspace);
