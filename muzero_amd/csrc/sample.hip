@@ -130,6 +130,9 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k ^ ((int)k < 0 ? 0x80000000u : 0xffffffffu)); }
 constexpr uint32_t kNoKey = 0x007fffffu;   // key of -inf: an entry that takes no part
+// The upper end of a range of keys as the largest key that an entry can have: entries are keyed as z + 0, so none has the key of -0.
+// As a float that end is equal to +0, whose key lies above it: a comparison of floats would take the zeros into the range.
+__device__ __forceinline__ uint32_t upper_end(uint32_t k) { return k == 0x7fffffffu ? k - 1 : k; }
 // ranking as an unsigned 64-bit order: larger z first, then smaller index; 0 = no entry
 __device__ __forceinline__ u64 rank_of(float z, int i) { return z > -INFINITY ? ((u64)key_of(z + 0.0f) << 32) | (uint32_t)~i : 0ull; }
 __device__ __forceinline__ int index_of_rank(u64 r) { return (int)~(uint32_t)r; }
@@ -914,7 +917,7 @@ struct Row {
                 const Scale s = sc;
                 const uint32_t top = khi;
                 if (!open) klo = first_key(klo, top, (float)za, lane, [=](float z) { double f; return bin_of(z, s, &f) <= bin; });
-                khi = first_key(klo, top + 1, (float)zb, lane, [=](float z) { double f; return bin_of(z, s, &f) < bin; }) - 1;
+                khi = upper_end(first_key(klo, top + 1, (float)zb, lane, [=](float z) { double f; return bin_of(z, s, &f) < bin; }) - 1);
                 if (above + cnt <= kList) {
                     *list_n = gather(of_key(klo), INFINITY, b0);
                     *small = true;
@@ -924,9 +927,9 @@ struct Row {
                 const int a0 = above;
                 const double m0 = above_mass;
                 const int rb = pick_bin(want, frac, false, mass, a0, m0, power, open ? 0 : kBins, &above, &above_mass, &cnt);
-                khi = khi - ((uint32_t)rb << shift);
-                const uint32_t width = (1u << shift) - 1;
-                klo = khi - klo > width ? khi - width : klo;
+                const uint32_t end = khi - ((uint32_t)rb << shift), width = (1u << shift) - 1;
+                klo = end - klo > width ? end - width : klo;
+                khi = upper_end(end);   // (a picked bin has entries, so it does not become empty)
             }
             if (cnt <= kList || (khi >> LowBits<T>::N) == (klo >> LowBits<T>::N)) break;
             shift = max(0, 32 - __clz((int)(khi - klo)) - 11);
