@@ -171,12 +171,13 @@ class MuZeroError(RuntimeError):
 
 
 def _ptr(a):
-    """numpy array -> host address; torch tensor -> data_ptr(); int -> as is; None -> NULL."""
+    """numpy array -> host address, which keeps the array (it may be a converted copy that nothing else holds); torch tensor ->
+    data_ptr(); int -> as is; None -> NULL."""
     if a is None:
         return None
     if isinstance(a, np.ndarray):
         assert a.flags["C_CONTIGUOUS"]
-        return a.ctypes.data
+        return a.ctypes.data_as(C.c_void_p)
     if isinstance(a, int):
         return a
     if hasattr(a, "data_ptr"):
