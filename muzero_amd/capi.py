@@ -6,6 +6,7 @@ Arrays may be numpy arrays (host memory) or torch CUDA tensors / raw integer dev
 (device memory); the library detects which.
 """
 import ctypes as C
+import operator
 import os
 
 import numpy as np
@@ -192,6 +193,33 @@ def _np(a, dtype):
     return np.ascontiguousarray(a, dtype=dtype)
 
 
+def _sized(a, name, dtypes, n, written=False):
+    """An argument of at least n elements for the C ABI, which gets no sizes or types: None and addresses as they are; lists and
+    numpy arrays converted to dtypes[0] (not those to write to); torch tensors of one of `dtypes`."""
+    if a is None or isinstance(a, int):
+        return a
+    want = np.dtype(dtypes[0])
+    if isinstance(a, (np.ndarray, list, tuple)) and not written:
+        try:
+            given, a = a, _np(a, want)
+            kept = want.kind == "f" or np.array_equal(a, given)
+        except (TypeError, ValueError, OverflowError) as e:
+            raise MuZeroError(f"{name}: {e}") from None
+        if not kept:
+            raise MuZeroError(f"{name}: holds values that are no {want.name}")
+    if isinstance(a, np.ndarray):
+        ok, size = a.dtype == want and a.flags["C_CONTIGUOUS"] and (a.flags["WRITEABLE"] or not written), a.size
+    elif hasattr(a, "data_ptr"):
+        ok, size = str(a.dtype).split(".")[-1] in dtypes and a.is_contiguous(), a.numel()
+    else:
+        raise MuZeroError(f"{name}: a numpy array or a torch tensor is needed")
+    if not ok:
+        raise MuZeroError(f"{name}: must be contiguous and {' or '.join(dtypes)}, not {a.dtype}")
+    if size < n:
+        raise MuZeroError(f"{name}: has {size} elements, needs {n}")
+    return a
+
+
 def make_config(spec, num_simulations, initial_gumbel_m, c_visit, c_scale=1.0, discount=1.0, known_bounds=None,
                 root_exploration_fraction=0.0, hybrid=False, gumbel_action_selection=True, temperature_root=1.0,
                 max_games=1, max_simulations=None, precision=PRECISION_FP32, pool_slots=0, gumbel_seed=None):
@@ -320,14 +348,22 @@ class Context:
     def play_policy(self, B, obs, legal, u, adapter=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, outputs=None):
         """One raw-policy move per game.  outputs: dict of preallocated numpy arrays / torch CUDA tensors (any subset of
         action, logprob, kept, playout_policy, logits, value), or None for numpy arrays of everything."""
-        A = self.A
+        A, net = self.A, self.cfg.net
         o = dict(action=np.empty(B, np.int32), logprob=np.empty(B, np.float32), kept=np.empty(B, np.int32),
                  playout_policy=np.empty((B, A), np.float32), logits=np.empty((B, A), np.float32),
                  value=np.empty(B, np.float64)) if outputs is None else outputs
-        po = PolicyOutputs(*[_ptr(o.get(name)) for name, _ in PolicyOutputs._fields_])
-        s = PolicySampling(temperature, top_p, min_p, top_k, 0)
-        self._check(lib().mz_play_policy(self._h, B, _ptr(_np(obs, np.float32)), _ptr(_np(legal, np.uint8)),
-                                         _ptr(_np(adapter, np.int32)), C.byref(s), _ptr(_np(u, np.float64)), C.byref(po)))
+        types = dict(action="int32", logprob="float32", kept="int32", playout_policy="float32", logits="float32", value="float64")
+        po = PolicyOutputs(*[_ptr(_sized(o.get(name), name, (types[name],), B * A if name in ("playout_policy", "logits") else B, written=True))
+                             for name, _ in PolicyOutputs._fields_])
+        try:   # (a ctypes field would cut an int to its low bits)
+            top_k = min(operator.index(top_k), 2**31 - 1)
+            s = PolicySampling(temperature, top_p, min_p, max(top_k, -1), 0)
+        except TypeError as e:
+            raise MuZeroError(f"temperature, top_k, top_p and min_p must be numbers ({e})") from None
+        self._check(lib().mz_play_policy(
+            self._h, B, _ptr(_sized(obs, "obs", ("float32",), B * net.obs_planes * net.height * net.width)),
+            _ptr(_sized(legal, "legal", ("uint8", "bool"), B * A)), _ptr(_sized(adapter, "adapter", ("int32",), B)), C.byref(s),
+            _ptr(_sized(u, "u", ("float64",), B)), C.byref(po)))
         return o
 
     # --- move level (PlanAction.planAction for B games) -------------------------------------------

@@ -3,6 +3,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 from muzero_amd import capi, netspec
 
@@ -80,3 +81,39 @@ def test_converted_arguments_of_search_moves(context):
                      gumbel=rng.uniform(size=(B, spec.action_space)).astype(np.float32))
         ctx.search_moves(B, **given)
         same(library.got, given)
+
+
+def test_play_policy_keeps_top_k_whole(context):
+    """A number beyond the field's 32 bits keeps all actions; it is not cut to its low bits (0: off, or 3 of them)."""
+    ctx, library, spec, B = context
+    given = converted(np.random.default_rng(2), spec, B)
+    for k, arrives in ((5, 5), (2**32, 2**31 - 1), (2**32 + 3, 2**31 - 1), (2**40, 2**31 - 1), (-(2**32) + 3, -1), (np.int64(7), 7)):
+        ctx.play_policy(B, **given, top_k=k)
+        assert library.sampling.top_k == arrives
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(u=np.zeros(5)), "u: has 5 elements, needs 6"), (dict(u=torch.zeros(6)), "u: must be .* float64"),
+    (dict(u=torch.zeros(12, dtype=torch.float64)[::2]), "u: must be contiguous"), (dict(legal=np.ones((5, 9), np.uint8)), "legal: has 45"),
+    (dict(legal=torch.ones(6, 9)), "legal"), (dict(legal=np.full((6, 9), 256)), "legal: holds values"), (dict(obs=np.zeros((6, 3, 3))), "obs: has 54"),
+    (dict(obs=torch.zeros(6, 300, dtype=torch.float16)), "obs"), (dict(adapter=np.full(6, 2**32)), "adapter: holds values"),
+    (dict(adapter=np.full(6, 0.5)), "adapter: holds values"), (dict(adapter=torch.zeros(6, dtype=torch.int64)), "adapter"),
+    (dict(adapter=[[0, 1], [2]]), "adapter"), (dict(u="0.5"), "u: a numpy array"), (dict(top_k=2.5), "must be numbers"),
+    (dict(top_k=None), "must be numbers"), (dict(temperature=None), "must be numbers"), (dict(min_p="0"), "must be numbers"),
+    (dict(outputs=dict(action=np.zeros(6, np.int64))), "action"), (dict(outputs=dict(logits=np.zeros((6, 8), np.float32))), "logits: has 48"),
+    (dict(outputs=dict(value=torch.zeros(6))), "value"), (dict(outputs=dict(kept=[0] * 6)), "kept")])
+def test_play_policy_refuses(context, change, text):
+    ctx, library, spec, B = context
+    with pytest.raises(capi.MuZeroError, match=text):
+        ctx.play_policy(B, **{**converted(np.random.default_rng(3), spec, B), **change})
+
+
+def test_play_policy_takes_more_than_it_needs_and_addresses(context):
+    ctx, library, spec, B = context
+    given = converted(np.random.default_rng(4), spec, B)
+    u = torch.rand(9, dtype=torch.float64)
+    given.update(u=u, legal=torch.ones(6, 9, dtype=torch.bool), adapter=torch.zeros(6, dtype=torch.int32))
+    ctx.play_policy(B, **given)
+    np.testing.assert_array_equal(library.got["u"], u[:6].numpy())
+    ctx.play_policy(B, **{**given, "u": u.data_ptr()})
+    np.testing.assert_array_equal(library.got["u"], u[:6].numpy())
