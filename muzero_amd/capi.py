@@ -334,15 +334,13 @@ class Context:
         if a is None:
             self._check(lib().mz_load_policy_adapters(self._h, 0, 0, None, None, None))
             return
-        a, b, scale = _np(a, np.float32), _np(b, np.float32), _np(scale, np.float32)
-        n, rank, hw = a.shape
-        if hw != 2 * self.cfg.net.height * self.cfg.net.width or tuple(b.shape) != (n, self.A, rank):
+        a, b, scale = (_sized(v, name, ("float32",), 0) for v, name in ((a, "a"), (b, "b"), (scale, "scale")))
+        sa, sb, ss = (tuple(getattr(v, "shape", ())) for v in (a, b, scale))
+        n, rank = sa[:2] if len(sa) == 3 else (0, 0)
+        if sa != (n, rank, 2 * self.cfg.net.height * self.cfg.net.width) or sb != (n, self.A, rank):
             raise MuZeroError("a must be [n, rank, 2 * height * width] and b [n, action_space, rank]")
-        if scale is not None and tuple(scale.shape) != (n,):
+        if scale is not None and ss != (n,):
             raise MuZeroError("scale must be [n]")
-        for v in (a, b, scale):
-            if v is not None and not isinstance(v, np.ndarray) and "float32" not in str(v.dtype):
-                raise MuZeroError("adapters must be float32")
         self._check(lib().mz_load_policy_adapters(self._h, n, rank, _ptr(a), _ptr(b), _ptr(scale)))
 
     def play_policy(self, B, obs, legal, u, adapter=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, outputs=None):

@@ -117,3 +117,12 @@ def test_play_policy_takes_more_than_it_needs_and_addresses(context):
     np.testing.assert_array_equal(library.got["u"], u[:6].numpy())
     ctx.play_policy(B, **{**given, "u": u.data_ptr()})
     np.testing.assert_array_equal(library.got["u"], u[:6].numpy())
+
+
+@pytest.mark.parametrize("change", [dict(a=np.zeros((3, 18))), dict(b=None), dict(b=1.0), dict(a=[[1.0], [2.0, 3.0]]), dict(a=np.zeros((0, 2, 18))),
+                                    dict(a=torch.zeros(3, 2, 18, dtype=torch.float64)), dict(a=torch.zeros(3, 18, 2).transpose(1, 2)),
+                                    dict(scale=np.ones(2)), dict(scale=2.0), dict(scale="2")])
+def test_load_policy_adapters_refuses(context, change):
+    ctx = context[0]
+    with pytest.raises(capi.MuZeroError):
+        ctx.load_policy_adapters(**{**dict(a=np.zeros((3, 2, 18)), b=np.zeros((3, 9, 2))), **change})
