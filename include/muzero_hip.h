@@ -334,7 +334,8 @@ int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t worksp
 /* A projection that all rows share, with a low-rank adapter of each row's own beside it:
  *   y[m] = x[m] W^T + bias + scale[i] * (x[m] A[i]^T) B[i]^T,   i = index[m]
  * index -1: the shared projection alone; any other index outside [0, adapters) makes the row NaN.  Sums are fp32 (inputs of
- * 16 bits on 16-bit matrix instructions, fp32 on fp32 ones), rounded once to y's type.  Rows do not influence one another:
+ * 16 bits on 16-bit matrix instructions, fp32 on fp32 ones), x A^T keeps the precision of fp32 between its two products, and y is
+ * rounded once to its type.  Rows do not influence one another:
  * a row's inf or NaN, or an adapter's, stay with the rows that use them. */
 typedef struct mz_adapter_args {
     int32_t rows, in_features, out_features; /* both features <= 2^26, ceil(rows / 256) * ceil(out_features / 256) <= 2^21 */

@@ -174,6 +174,20 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
     return v;
 }
 
+// The bf16 in front of each of 8 floats (truncated: none becomes inf), and what is left.  A float is the sum of three such parts
+// exactly.
+__device__ __forceinline__ u32x4 take_bf16(float (&v)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]) & 0xffff0000u;
+        r[i] = a >> 16 | b;
+        v[2 * i] -= __uint_as_float(a & 0xffff0000u);
+        v[2 * i + 1] -= __uint_as_float(b);
+    }
+    return r;
+}
+
 // ---- t = x A^T -------------------------------------------------------------------------------------------------------------
 // Workgroup (block of BR rows, part of K): jobs of up to 16 rows of one adapter, a wave each.  part[s][row][padded rank].
 // 16 rows: a wave for every job there can be, in 4 workgroups; 128 rows: 8 waves, as many as 8 rank tiles leave registers for, in 2
@@ -749,13 +763,43 @@ __global__ __launch_bounds__(64 * WM * WN * kTileGroups<BM>, 2) void k_tile(Adap
     __syncthreads();
     // With few rows per adapter (by the numbers of both, not by the data: the two ways round differently, and a row's result must
     // not depend on its neighbours) every lane takes the B of its own row; else the matrix instructions take 16 rows at a time.
-    // By rows and by matrix instructions, in mixed order: 2000x1024x1024 bf16 rank 16 (tiles of 64) 8 adapters 22.8 and 23.6 us,
-    // 12 22.8 and 25.5, 64 29.5 and 41.8; 4096x512x2304 (of 128) 16 adapters 62.3 and 66.1, 32 65.9 and 89.3.
+    // By rows and by matrix instructions, in mixed order: 2000x1024x1024 bf16 rank 16 (tiles of 64) 8 adapters 24.6 and 26.3 us,
+    // 12 24.4 and 27.3, 64 30.0 and 42.6; 4096x512x2304 (of 128) 16 adapters 62.4 and 67.2, 32 66.0 and 90.7.
     const bool per_row = op.rank <= 32 && BM <= 8 * op.adapters;
     const auto add_term = [&](auto J) __attribute__((always_inline)) {
         constexpr int j = J.value;
         const int p = wm + j * 16 + lr, own = key[p];
-        if (per_row && own >= 0) {
+        // bf16: t as the sum of three bf16 numbers, exactly.  fp16: t scaled by a power of two to a maximum in [2^14, 2^15), as the sum of two fp16 numbers: within 2^-24 of its value down to
+        // 2^-15 of the maximum, where their subnormal step, 2^-24, begins to tell.  Below that a third number, 2^24 times larger, takes what
+        // they leave (`wide`), down to 2^-38 of the maximum, where the first is not 0 yet.  Rows whose ranks are still further apart, and
+        // rows of both types with an inf or a NaN, are summed by themselves.  All of this goes by the row's own t alone.
+        bool by_itself = per_row, wide = false;
+        float back = 1.f, to = 1.f;
+        if (sizeof(T) == 2 && !per_row) {
+            float mx = 0, mn = INFINITY;
+            for (int r = kq * 4; r < rp; r += 16)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float v = fabsf(tl[p * ts + r + e]);
+                    mx = v < INFINITY ? fmaxf(mx, v) : INFINITY;
+                    mn = v > 0 ? fminf(mn, v) : mn;
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            by_itself = !(mx < INFINITY);
+            if constexpr (__is_same(T, _Float16)) {
+                mn = fminf(mn, __shfl_xor(mn, 16));
+                mn = fminf(mn, __shfl_xor(mn, 32));
+                if (mx > 0) {
+                    by_itself = mx > 0x1p100f || mx < 0x1p-80f || mn < mx * 0x1p-38f;
+                    wide = mn < mx * 0x1p-15f;
+                    const int em = by_itself ? 0 : ilogbf(mx) - 14;
+                    back = ldexpf(1.f, em);
+                    to = ldexpf(1.f, -em);
+                }
+            }
+        }
+        if (by_itself && own >= 0) {
             const float sc = op.scale ? op.scale[own] : 1.f;
             f32x4 d[NE] = {};
             for (int r = 0; r < op.rank; r += CE) {
@@ -779,64 +823,72 @@ __global__ __launch_bounds__(64 * WM * WN * kTileGroups<BM>, 2) void k_tile(Adap
 #pragma unroll
                 for (int e = 0; e < 4; e++) sum[ni][j][e] = fmaf(sc, d[ni][e], sum[ni][j][e]);
         }
-        float back = 1.f, to = 1.f;
-        if constexpr (__is_same(T, _Float16)) {
-            float mx = 0;
-            for (int r = kq * 4; r < rp; r += 16)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(tl[p * ts + r + e]));
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            // scaled into [0.5, 1) by a power of two
-            const int em = mx > 0 && mx < INFINITY ? max(-100, min(100, ilogbf(mx) + 1)) : 0;
-            back = ldexpf(1.f, em);
-            to = ldexpf(1.f, -em);
-        }
         // per adapter among the 16 rows
-        unsigned long long todo = __ballot(own >= 0 && !per_row);
+        unsigned long long todo = __ballot(own >= 0 && !by_itself);
         while (todo) {
             const int i = __shfl(own, __ffsll(todo) - 1);
-            const bool use = own == i;
+            const bool use = own == i && !by_itself;
             todo &= ~__ballot(use);
-            const float sc = (op.scale ? op.scale[i] : 1.f) * back;
-            f32x4 d[NE] = {};
-            for (int r0 = 0; r0 < rp; r0 += 16) {
-                u32x4 ft;   // 16 bits: k = 16 ranks of the leading part of t, then the same 16 of what it leaves; fp32: the 16 ranks
-                int rb;
-                if constexpr (sizeof(T) == 4) {
-                    rb = r0 + kq * 4;
-                    ft = *reinterpret_cast<const u32x4*>(tl + p * ts + rb);
-                } else {
-                    rb = r0 + (kq & 1) * 8;
-                    T h[8];
+            const float sc = op.scale ? op.scale[i] : 1.f;
+            const auto product = [&](auto Part) __attribute__((always_inline)) {
+                constexpr bool kThird = Part.value == 1;
+                f32x4 d[NE] = {};
+                for (int r0 = 0; r0 < rp; r0 += 16) {
+                    // fp32: 16 ranks as they are.  16 bits: a product of 16 ranks of one part of t, then of the same 16 of another: of the
+                    // first and second part (t0), and in bf16, which needs three to hold a float, of the third and nothing (t1).
+                    const int rb = r0 + (sizeof(T) == 4 ? kq * 4 : (kq & 1) * 8);
+                    const bool other = kq >= 2;
+                    u32x4 t0, t1;
+                    if constexpr (sizeof(T) == 4) {
+                        t0 = *reinterpret_cast<const u32x4*>(tl + p * ts + rb);
+                    } else {
+                        float v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float v = tl[p * ts + rb + e] * to;
-                        h[e] = from_float<T>(v);
-                        if (kq >= 2) {
-                            const float rest = v - to_float(h[e]);
-                            h[e] = from_float<T>(rest == rest ? rest : 0.f);   // inf - inf: the leading part says it
+                        for (int e = 0; e < 8; e++) v[e] = tl[p * ts + rb + e] * (__is_same(T, bf16_t) ? 1.f : to);
+                        if constexpr (__is_same(T, bf16_t)) {
+                            const u32x4 a = take_bf16(v), b = take_bf16(v), c = take_bf16(v);
+                            t0 = other ? b : a;
+                            t1 = other ? u32x4{0, 0, 0, 0} : c;
+                        } else {
+                            T h[8];
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                h[e] = from_float<T>(v[e]);
+                                if (kThird || other) {
+                                    const float rest = v[e] - to_float(h[e]);
+                                    h[e] = from_float<T>(rest);
+                                    if (kThird) h[e] = from_float<T>(other ? 0.f : (rest - to_float(h[e])) * 0x1p24f);
+                                }
+                            }
+                            __builtin_memcpy(&t0, h, 16);
                         }
                     }
-                    __builtin_memcpy(&ft, h, 16);
-                }
 #pragma unroll
-                for (int ni = 0; ni < NE; ni++) {
-                    const int n = min(n0 + we + ni * 16 + lr, op.N - 1);
-                    u32x4 v = load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + n) * op.rank, rb, op.rank);
-                    if constexpr (sizeof(T) == 2) {
-                        // an inf of B times the rest of t, which may have the other sign, is not wanted beside inf times its leading part
-                        if (kq >= 2) v = finite_only<T>(v);
+                    for (int ni = 0; ni < NE; ni++) {
+                        const int n = min(n0 + we + ni * 16 + lr, op.N - 1);
+                        u32x4 v = load_chunk(static_cast<const T*>(op.b) + ((long long)i * op.N + n) * op.rank, rb, op.rank);
+                        // an inf of B meets the first part of t alone: the others may be 0 or have the other sign
+                        if constexpr (__is_same(T, bf16_t)) {
+                            const u32x4 f = finite_only<T>(v);
+                            d[ni] = mma<T>(f, t1, d[ni]);
+                            v = other ? f : v;
+                        } else if constexpr (sizeof(T) == 2) {
+                            if (kThird || other) v = finite_only<T>(v);
+                        }
+                        d[ni] = mma<T>(v, t0, d[ni]);
                     }
-                    d[ni] = mma<T>(v, ft, d[ni]);
                 }
-            }
-            if (use) {
+                if (use && (!kThird || wide)) {
+                    const float unit = kThird ? back * 0x1p-24f : back;
 #pragma unroll
-                for (int ni = 0; ni < NE; ni++)
+                    for (int ni = 0; ni < NE; ni++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sum[ni][j][e] = fmaf(sc, d[ni][e], sum[ni][j][e]);
-            }
+                        for (int e = 0; e < 4; e++) sum[ni][j][e] = fmaf(sc, d[ni][e] * unit, sum[ni][j][e]);
+                }
+            };
+            product(std::integral_constant<int, 0>{});
+            if constexpr (__is_same(T, _Float16))
+                if (__ballot(use && wide)) product(std::integral_constant<int, 1>{});
         }
     };
     static_for(add_term, std::make_integer_sequence<int, MI>{});

@@ -1,0 +1,160 @@
+"""-m gpu: the adapters' term of ops.adapter_linear in the precision of fp32 sums, where the tiles' matrix instructions form it from
+16-bit parts of t = x A^T.  t is the sum of such parts to 2^-24 of its value, so an entry is a sum of K products and then of up to 3
+products a rank, each exact: off by at most 2 (K + 6 rank + 2) 2^-24 of the sum of the absolute values (2: as in test_gpu_adapter.py; K
+for the sum and the parts of t, 6 for three products and their sums) and by the rounding to its type.  Short sums and fp32 results
+leave no room for a t of 16 bits."""
+import numpy as np
+import pytest
+import torch
+
+from muzero_amd import ops
+from tests import op_refs
+from tests.test_gpu_adapter import TYPES, make
+
+pytestmark = pytest.mark.gpu
+TILES = {64: (1100, 520), 128: (2100, 2100), 256: (4200, 4200)}
+
+
+def check(s, out_dtype=torch.float32):
+    y = ops.adapter_linear(**s, out_dtype=out_dtype)
+    with np.errstate(invalid="ignore"):
+        want, size = op_refs.adapter(**s)
+    got = y.double().cpu().numpy()
+    K, r = s["x"].shape[1], s["a"].shape[1]
+    tol = 2 * (K + 6 * r + 2) * 2.0**-24 * size
+    tol = tol + (torch.finfo(out_dtype).eps / 2) * (np.abs(want) + tol) + torch.finfo(out_dtype).smallest_normal
+    # beyond the type's largest number by half a step and more, rounding gives inf
+    f = torch.finfo(out_dtype)
+    beyond = f.max + f.eps / 2 * 2.0 ** np.floor(np.log2(f.max))
+    over = np.isinf(got) & np.isfinite(want) & (np.abs(want) + 2 * (K + 6 * r + 2) * 2.0**-24 * size >= beyond)
+    want = np.where(over, np.copysign(np.inf, want), want)
+    fine = np.isfinite(want)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    np.testing.assert_array_equal(got[~fine], want[~fine])
+    off = np.abs(got[fine] - want[fine])
+    assert (off <= tol[fine]).all(), ((off > tol[fine]).sum(), (off / tol[fine]).max())
+
+
+def alone(rng, M, K, N, r, n, dtype):
+    """The term alone: no shared projection, no bias; x and A positive, so that t has the size of its terms."""
+    s = make(rng, M, K, N, r, n, dtype, bias=False, scale=False)
+    s["weight"].zero_()
+    s["x"].abs_()
+    s["a"].abs_()
+    return s
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("side", list(TILES))
+def test_all_bits_of_t(side, dtype):
+    rng = np.random.default_rng(side)
+    M, N = TILES[side]
+    for K, r, n in ((4, 1, 3), (5, 2, 3), (4, 40, 24)):
+        check(alone(rng, M, K, N, r, n, dtype))
+    check(make(rng, M, 8, N, 3, 3, dtype))
+
+
+@pytest.mark.parametrize("side", [64, 128])
+def test_ranks_of_very_different_size(side):
+    """fp16: t of the ranks far apart in size, B making up for it: both kinds of ranks matter alike."""
+    rng = np.random.default_rng(side + 1)
+    M, N = TILES[side]
+    for K, r, up, down in ((64, 8, 1e3, 1e-4), (64, 20, 2e2, 1e-3), (8, 2, 6e3, 2e-5)):
+        s = make(rng, M, K, N, r, 3, "fp16")
+        s["a"][:, ::2] *= up
+        s["b"][:, :, ::2] *= down
+        s["a"][:, 1::2] *= 1e-3
+        s["b"][:, :, 1::2] *= 1e2
+        check(s)
+        check(s, torch.float16)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("side", [64, 128])
+def test_large_and_small_t(side, dtype):
+    """fp16: as far as its numbers reach; bf16: while the least part of t is a normal number."""
+    rng = np.random.default_rng(side + 2)
+    for up, down in ((2e4, 1e-6), (1e-5, 3e3)) if dtype == "fp16" else ((1e30, 1e-28), (1e-29, 1e28)):
+        s = make(rng, *TILES[side][:1], 16, TILES[side][1], 5, 3, dtype)
+        s["a"] *= up
+        s["b"] *= down
+        check(s)
+
+
+def test_t_between_the_largest_bf16_and_the_largest_fp32():
+    M, N = TILES[64]
+    s = make(np.random.default_rng(0), M, 4, N, 1, 3, "bf16", bias=False, scale=False)
+    s["weight"].zero_()
+    s["x"][:] = torch.tensor([2.0**64, 2.0**60, 2.0**60, 0.0])
+    s["a"][:] = torch.tensor([255 / 128 * 2.0**63, 2.0**59, 2.0**58, 0.0])      # t = (2 - 2^-7) 2^127 + 2^119 + 2^118
+    s["b"][:] = 2.0**-100
+    check(s)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("side", [64, 128])
+def test_inf_and_nan_of_t_and_of_b(side, dtype):
+    """Values of few bits, whose lower parts are 0: an inf must not meet them."""
+    rng = np.random.default_rng(side + 3)
+    M, N = TILES[side]
+    for r in (1, 3, 20):
+        s = make(rng, M, 4, N, r, 3, dtype, bias=False)
+        s["x"] = torch.from_numpy(2.0 ** rng.integers(-2, 3, (M, 4))).to(TYPES[dtype]).cuda()
+        s["a"] = torch.from_numpy(2.0 ** rng.integers(-2, 3, (3, r, 4))).to(TYPES[dtype]).cuda()
+        s["b"] = torch.from_numpy(2.0 ** rng.integers(-2, 3, (3, N, r))).to(TYPES[dtype]).cuda()
+        s["x"][3, 1], s["x"][5, 2], s["x"][7, 0] = float("inf"), float("-inf"), float("nan")
+        s["weight"].abs_()
+        s["b"][1, 7, 0], s["b"][1, 9, r - 1], s["b"][2, 11, 0] = float("inf"), float("-inf"), float("nan")
+        s["x"][40:50] = 0
+        check(s)
+        check(s, TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_an_inf_beside_large_t(dtype):
+    """One rank of t is inf, another beyond the largest fp16 and of the other sign: the sum is inf."""
+    s = make(np.random.default_rng(1), TILES[64][0], 16, TILES[64][1], 2, 3, dtype, scale=False)
+    s["x"].abs_()
+    s["a"].abs_()
+    s["b"].abs_()
+    s["a"][:, 1] = 3e4
+    s["b"][:, :, 1] *= -1
+    s["a"][1, 0, 3] = float("inf")
+    check(s)
+    check(s, TYPES[dtype])
+
+
+def test_rows_of_both_kinds_side_by_side():
+    """fp16: rows whose ranks lie far apart among rows whose do not, of the same adapters; the latter bit for bit as without the former."""
+    rng = np.random.default_rng(2)
+    M, N = TILES[64]
+    s = make(rng, M, 8, N, 4, 3, "fp16")
+    s["a"][:, 0, 4:] = 0
+    s["a"][:, 1:, :4] *= 1e-3
+    s["x"][:, :4] *= 1e-2
+    y = ops.adapter_linear(**s, out_dtype=torch.float32)
+    s["x"][::5, :4] *= 6e4
+    check(s)
+    z = ops.adapter_linear(**s, out_dtype=torch.float32)
+    rest = torch.arange(M, device="cuda") % 5 != 0
+    assert torch.equal(y[rest], z[rest])
+
+
+def test_ranks_as_far_apart_as_fp16_goes():
+    """t of one rank 2^35 to 2^60 times that of the other, B the other way round; an inf of B in some columns."""
+    rng = np.random.default_rng(3)
+    M, N = TILES[64]
+    for large, small in ((2.0**10, 2.0**-10), (2.0**15, 2.0**-12), (2.0**15, 2.0**-20)):
+        s = make(rng, M, 8, N, 4, 3, "fp16")
+        s["x"].abs_()
+        s["x"][:, 4:] *= 2.0**-6
+        s["a"][:] = 0
+        s["b"][:] = torch.from_numpy(rng.uniform(1, 2, (3, N, 4)).astype(np.float16)).cuda()
+        s["a"][:, ::2, :4] = large
+        s["b"][:, :, ::2] *= 2.0**-14
+        s["a"][:, 1::2, 4:] = small
+        s["b"][:, :, 1::2] *= 2.0**14
+        check(s)
+        s["b"][1, ::7, 1] = float("inf")
+        s["b"][2, ::9, 0] = float("-inf")
+        check(s)
