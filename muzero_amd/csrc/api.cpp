@@ -132,10 +132,11 @@ struct mz_ctx {
     size_t comm_buf_count = 0;
     // device outputs
     DeviceMoveOutputs dout{};
-    // raw-policy moves (mz_play_policy): adapters of the policy head, its features and adapted logits, operator workspaces
+    // raw-policy moves (mz_play_policy): the policy head's last linear ([A][2 HW], bias [A]; as packed, w_master may be ahead of it),
+    // its adapters, features and adapted logits, operator workspaces
     int ad_n = 0, ad_rank = 0;
     bool ad_scaled = false;
-    DevBuf ad_a, ad_b, ad_scale, pol_feat, pol_logits, pol_ws;
+    DevBuf pol_fc, ad_a, ad_b, ad_scale, pol_feat, pol_logits, pol_ws;
     // timing
     bool timing = false;
     std::vector<EventPair> events;
@@ -499,7 +500,8 @@ int pack_and_upload(mz_ctx* ctx, const std::vector<float>& blob) {
     pack_conv(dst, h.pconv, bw.take((size_t)2 * C), 2, C, 1);
     pack_copy(dst, h.plng, bw.take((size_t)2 * HW), (size_t)2 * HW);
     pack_copy(dst, h.plnb, bw.take((size_t)2 * HW), (size_t)2 * HW);
-    pack_transpose(dst, h.pfcw, bw.take((size_t)A * 2 * HW), A, 2 * HW);  // [A][2HW] -> [2HW][A]
+    const float* pfc = bw.take((size_t)A * 2 * HW);
+    pack_transpose(dst, h.pfcw, pfc, A, 2 * HW);  // [A][2HW] -> [2HW][A]
     pack_copy(dst, h.pfcb, bw.take((size_t)A), (size_t)A);
     while (dst.size() % 4) dst.push_back(0.f);
     pack_conv(dst, h.vconv, bw.take((size_t)C), 1, C, 1);
@@ -520,6 +522,9 @@ int pack_and_upload(mz_ctx* ctx, const std::vector<float>& blob) {
     }
     HIP_TRY(hipMemcpy(ctx->w_f32, dst.data(), dst.size() * sizeof(float), hipMemcpyHostToDevice));
     HIP_TRY(hipMemcpy(ctx->prog_dev, &pr, sizeof(pr), hipMemcpyHostToDevice));
+    const size_t pfc_bytes = ((size_t)A * 2 * HW + A) * sizeof(float);
+    if (grow(ctx, ctx->pol_fc, pfc_bytes)) return -1;
+    HIP_TRY(hipMemcpy(ctx->pol_fc.p, pfc, pfc_bytes, hipMemcpyHostToDevice));
     if (ctx->cfg.precision != MZ_PRECISION_FP32) {
         std::string err;
         if (mfma_pack_weights(ctx->mfma, ctx->nd, blob.data(), blob.size(), &err) != 0) return ctx_fail(ctx, err);
@@ -973,7 +978,7 @@ void mz_destroy(mz_ctx* ctx) {
     if (ctx->mfma) mfma_destroy(ctx->mfma);
     if (ctx->comm) (void)rccl()->CommDestroy((ncclComm_t)ctx->comm);
     if (ctx->comm_buf) (void)hipFree(ctx->comm_buf);
-    for (DevBuf* b : {&ctx->ad_a, &ctx->ad_b, &ctx->ad_scale, &ctx->pol_feat, &ctx->pol_logits, &ctx->pol_ws})
+    for (DevBuf* b : {&ctx->pol_fc, &ctx->ad_a, &ctx->ad_b, &ctx->ad_scale, &ctx->pol_feat, &ctx->pol_logits, &ctx->pol_ws})
         if (b->p) (void)hipFree(b->p);
     for (auto& e : ctx->events) {
         (void)hipEventDestroy(e.a);
@@ -1305,9 +1310,7 @@ int mz_play_policy(mz_ctx* ctx, int B, const float* obs, const uint8_t* legal, c
     float* logits = ctx->net_logits;
     if (adapter) {
         logits = (float*)ctx->pol_logits.p;
-        // the end of the blob: fc [A][2 HW], bias [A], then the value head
-        const size_t value_head = d.C + 2 * (size_t)d.HW + (size_t)d.C * d.HW + 2 * (size_t)d.C + 1;
-        const float* fc = ctx->w_master + ctx->n_params - value_head - A - A * K;
+        const float* fc = (const float*)ctx->pol_fc.p;
         mz_adapter_args a{};
         a.rows = B;
         a.in_features = (int)K;
