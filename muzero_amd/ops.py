@@ -43,7 +43,8 @@ def _need(ok, text):
 def _tensor(t, name, dtype, shape, device, dense=True):
     """Address of t, a tensor of that dtype and shape on GPU `device` whose rows are contiguous (dense: all of it)."""
     try:   # one test for the usual case; which one failed is found out below
-        if t.dtype is dtype and t.shape == shape and t.get_device() == device and (t.is_contiguous() or not dense and t.stride(-1) == 1):
+        if (t.dtype is dtype and t.shape == shape and t.get_device() == device and not t.requires_grad
+                and (t.is_contiguous() or not dense and t.stride(-1) == 1)):
             return t.data_ptr()
     except AttributeError:
         pass
@@ -51,8 +52,10 @@ def _tensor(t, name, dtype, shape, device, dense=True):
     _need(t.dtype == dtype, f"{name}: {t.dtype}, needs {dtype}")
     _need(tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, needs {tuple(shape)}")
     _need(t.get_device() == device, f"{name}: on {t.device}, the other operands on cuda:{device}")
-    _need(not dense, f"{name}: must be contiguous")
+    _need(t.is_contiguous() or not dense, f"{name}: must be contiguous")
     _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: the last dimension must be contiguous")
+    _need(not (t.requires_grad and torch.is_grad_enabled()),
+          f"{name}: requires a gradient and this operator has none: call it under torch.no_grad()")
     return t.data_ptr()
 
 
@@ -63,11 +66,6 @@ def _row_stride(t):
 def _stream(device):
     """torch's current stream of GPU `device`, as a hipStream_t."""
     return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
-
-
-def _no_gradient():
-    if torch.is_grad_enabled():
-        raise capi.MuZeroError("an input requires a gradient and this operator has none: call it under torch.no_grad()")
 
 
 def _fail():
@@ -106,8 +104,6 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     t, dev = logits.dtype, logits.get_device()
     if dev < 0 or t not in DTYPES:
         raise capi.MuZeroError(f"logits: must be on a GPU and float32, bfloat16 or float16, not {t} on {logits.device}")
-    if logits.requires_grad:
-        _no_gradient()
     shape = logits.shape
     B, A = shape
     rows = (B,)
@@ -131,8 +127,6 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
             out["probs"] = torch.empty(B, A, dtype=torch.float32, device=on)
     get = out.get
     action, logprob, kept, pr = get("action"), get("logprob"), get("kept"), get("probs")
-    if logprob is not None and getattr(logprob, "requires_grad", False) or pr is not None and getattr(pr, "requires_grad", False):
-        _no_gradient()
     try:
         args = _SAMPLE.pack(
             B, A, DTYPES[t], top_k, temperature, top_p, min_p,
@@ -162,9 +156,6 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
     t, dev = x.dtype, x.get_device()
     if dev < 0 or t not in DTYPES:
         raise capi.MuZeroError(f"x: must be on a GPU and float32, bfloat16 or float16, not {t} on {x.device}")
-    if (x.requires_grad or weight.requires_grad or a.requires_grad or getattr(b, "requires_grad", False)
-            or getattr(bias, "requires_grad", False) or getattr(scale, "requires_grad", False) or getattr(out, "requires_grad", False)):
-        _no_gradient()
     M, K = x.shape
     n, r, _ = a.shape
     N = weight.shape[0]

@@ -1,0 +1,52 @@
+"""-m gpu: the operators of muzero_amd.ops have no gradients, and say so for every tensor that could ask for one."""
+import numpy as np
+import pytest
+import torch
+
+from muzero_amd import capi, ops
+from tests.test_gpu_adapter import check as check_adapter
+from tests.test_gpu_adapter import make
+from tests.test_gpu_sample import check as check_sample
+from tests.test_gpu_sample import inputs
+
+pytestmark = pytest.mark.gpu
+SETTINGS = ("temperature", "top_p", "min_p")
+
+
+def sample_arguments(rows=5, actions=20):
+    z, u, _ = inputs(np.random.default_rng(0), rows, actions, torch.float32)
+    per_row = {k: torch.full((rows,), v, dtype=torch.float64, device="cuda") for k, v in zip(SETTINGS, (0.9, 0.8, 0.01))}
+    out = dict(action=torch.empty(rows, dtype=torch.int32, device="cuda"), logprob=torch.empty(rows, device="cuda"),
+               probs=torch.empty(rows, actions, device="cuda"), kept=torch.empty(rows, dtype=torch.int32, device="cuda"))
+    return dict(logits=z, u=u, **per_row), out
+
+
+@pytest.mark.parametrize("name", ["logits", "u", *SETTINGS, "logprob", "probs"])
+def test_sampling_refuses(name):
+    given, out = sample_arguments()
+    where = given if name in given else out
+    where[name] = where[name].clone().requires_grad_()
+    with pytest.raises(capi.MuZeroError, match="gradient"):
+        ops.sample_actions(**given, out=out)
+    with torch.no_grad():
+        check_sample(given.pop("logits"), given.pop("u"), out=out, **given)
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "a", "b", "bias", "scale"])
+def test_projection_refuses(name):
+    s = make(np.random.default_rng(1), 6, 40, 24, 3, 2, "fp32")
+    s[name] = s[name].clone().requires_grad_()
+    with pytest.raises(capi.MuZeroError, match="gradient"):
+        ops.adapter_linear(**s)
+    with torch.no_grad():
+        check_adapter({k: v.detach() for k, v in s.items()}, "fp32")
+        ops.adapter_linear(**s)
+
+
+def test_what_was_refused_with_a_gradient_is_refused_without():
+    """Under no_grad a tensor that requires one still has to have the right layout."""
+    given, _ = sample_arguments()
+    with torch.no_grad():
+        given["u"] = torch.rand(10, dtype=torch.float64, device="cuda", requires_grad=True)[::2]
+        with pytest.raises(capi.MuZeroError, match="u: must be contiguous"):
+            ops.sample_actions(**given)
