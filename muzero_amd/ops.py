@@ -1,11 +1,12 @@
 """The library's operators on torch tensors (mz_sample_actions, mz_adapter_linear of include/muzero_hip.h): checks of types, shapes and
 devices, then one call of the C ABI on torch's current stream of the tensors' device.  Nothing is copied, converted or
 synchronised; a call can be captured into a torch.cuda.graph.  There are no gradients: inputs that ask for them are refused
-while torch's grad mode is on.  Errors are capi.MuZeroError."""
+while torch's grad mode is on, forward-mode tangents always.  Errors are capi.MuZeroError."""
 import ctypes as C
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import capi
 
@@ -68,6 +69,12 @@ def _stream(device):
     return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
+def _no_tangent(*values):
+    for v in values:
+        if isinstance(v, torch.Tensor) and v.is_floating_point() and forward_ad.unpack_dual(v).tangent is not None:
+            raise capi.MuZeroError("an argument carries a forward-mode tangent and this operator has no derivative")
+
+
 def _fail():
     raise capi.MuZeroError(capi.lib().mz_last_error(None).decode())
 
@@ -113,6 +120,7 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
         if lt is not torch.uint8 and lt is not torch.bool:
             raise capi.MuZeroError("legal: a uint8 or bool tensor is needed")
         p_legal, s_legal = _tensor(legal, "legal", lt, shape, dev, dense=False), _row_stride(legal)
+    given_t, given_p, given_m = temperature, top_p, min_p
     temperature, p_t = _setting(temperature, "temperature", torch.float64, rows, dev)
     top_k, p_k = _setting(top_k, "top_k", torch.int32, rows, dev)
     top_p, p_p = _setting(top_p, "top_p", torch.float64, rows, dev)
@@ -127,6 +135,8 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
             out["probs"] = torch.empty(B, A, dtype=torch.float32, device=on)
     get = out.get
     action, logprob, kept, pr = get("action"), get("logprob"), get("kept"), get("probs")
+    if forward_ad._current_level >= 0:   # inside a dual_level
+        _no_tangent(logits, u, given_t, given_p, given_m, logprob, pr)
     try:
         args = _SAMPLE.pack(
             B, A, DTYPES[t], top_k, temperature, top_p, min_p,
@@ -167,6 +177,8 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
         out_dtype = t
     if out_dtype not in DTYPES:
         raise capi.MuZeroError(f"out: {out_dtype} is not supported")
+    if forward_ad._current_level >= 0:   # inside a dual_level
+        _no_tangent(x, weight, a, b, bias, scale, out)
     args = _ADAPTER.pack(
         M, K, N, r, n, DTYPES[t], DTYPES[out_dtype], 0,
         _tensor(x, "x", t, (M, K), dev, dense=False), _row_stride(x),

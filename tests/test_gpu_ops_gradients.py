@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from muzero_amd import capi, ops
 from tests.test_gpu_adapter import check as check_adapter
@@ -50,3 +51,39 @@ def test_what_was_refused_with_a_gradient_is_refused_without():
         given["u"] = torch.rand(10, dtype=torch.float64, device="cuda", requires_grad=True)[::2]
         with pytest.raises(capi.MuZeroError, match="u: must be contiguous"):
             ops.sample_actions(**given)
+
+
+@pytest.mark.parametrize("name", ["logits", "u", *SETTINGS, "logprob", "probs"])
+def test_sampling_refuses_tangents(name):
+    given, out = sample_arguments()
+    where = given if name in given else out
+    with forward_ad.dual_level():
+        check_sample(given["logits"], given["u"], out=out, **{k: given[k] for k in SETTINGS})
+        where[name] = forward_ad.make_dual(where[name], torch.ones_like(where[name]))
+        for context in (torch.enable_grad, torch.no_grad):
+            with context(), pytest.raises(capi.MuZeroError, match="tangent"):
+                ops.sample_actions(**given, out=out)
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "a", "b", "bias", "scale"])
+def test_projection_refuses_tangents(name):
+    s = make(np.random.default_rng(2), 6, 40, 24, 3, 2, "fp32")
+    with forward_ad.dual_level():
+        check_adapter(s, "fp32")
+        s[name] = forward_ad.make_dual(s[name], torch.ones_like(s[name]))
+        with pytest.raises(capi.MuZeroError, match="tangent"):
+            ops.adapter_linear(**s)
+
+
+def test_derivatives_by_functions_end_in_an_error():
+    given, _ = sample_arguments()
+    s = make(np.random.default_rng(3), 6, 40, 24, 3, 2, "fp32")
+    sample = lambda z: ops.sample_actions(**{**given, "logits": z})["logprob"]  # noqa: E731
+    project = lambda x: ops.adapter_linear(**{**s, "x": x})  # noqa: E731
+    for f, v in ((sample, given["logits"]), (project, s["x"])):
+        with pytest.raises((capi.MuZeroError, RuntimeError)):
+            torch.func.jvp(f, (v,), (torch.ones_like(v),))
+        with pytest.raises((capi.MuZeroError, RuntimeError)):
+            torch.func.grad(lambda t: f(t).sum())(v)
+        with pytest.raises((capi.MuZeroError, RuntimeError)):
+            torch.func.vmap(f)(v[None])
