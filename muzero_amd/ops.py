@@ -10,14 +10,16 @@ from torch.autograd import forward_ad
 
 from . import capi
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the same number without a Stream object around it
+# of a list of tensors, without the tests around it
+_increment_version = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+# torch's current stream of a GPU, as a hipStream_t: the same number without a Stream object around it, where torch has that
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 # the argument structs of the C ABI as bytes (capi.SampleArgs, capi.AdapterArgs have the fields): packing costs a quarter of
 # filling a ctypes Structure, and these calls are short
 _SAMPLE = struct.Struct("=4i3d14q")
 _ADAPTER = struct.Struct("=8i11q")
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MZ_DTYPE_*
-
-
+_NUMBERS = (float, int)   # (a test for Tensor goes through its metaclass and is slow)
 _entries = None
 
 
@@ -64,11 +66,6 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _stream(device):
-    """torch's current stream of GPU `device`, as a hipStream_t."""
-    return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
-
-
 def _no_tangent(*values):
     for v in values:
         if isinstance(v, torch.Tensor) and v.is_floating_point() and forward_ad.unpack_dual(v).tangent is not None:
@@ -79,21 +76,14 @@ def _fail():
     raise capi.MuZeroError(capi.lib().mz_last_error(None).decode())
 
 
-def _setting(v, name, dtype, shape, device):
-    """A number, or a tensor with one per row: (scalar, address)."""
-    if type(v) is not float and type(v) is not int and isinstance(v, torch.Tensor):
-        return 0, _tensor(v, name, dtype, shape, device)
-    return v, 0
-
-
 def _workspace(need, given, device):
     """(tensor to keep alive, address, bytes).  torch's allocator hands the memory out per stream (and per graph)."""
+    if given is None and need == 0:
+        return None, None, 0
     if given is not None:
         _need(isinstance(given, torch.Tensor) and given.dtype == torch.uint8 and given.is_contiguous() and given.get_device() == device,
               f"workspace: a contiguous uint8 tensor on cuda:{device} is needed")
         return given, given.data_ptr(), given.numel()
-    if need == 0:
-        return None, None, 0
     w = torch.empty(need, dtype=torch.uint8, device=f"cuda:{device}")
     return w, w.data_ptr(), need
 
@@ -111,6 +101,8 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
     t, dev = logits.dtype, logits.get_device()
     if dev < 0 or t not in DTYPES:
         raise capi.MuZeroError(f"logits: must be on a GPU and float32, bfloat16 or float16, not {t} on {logits.device}")
+    if forward_ad._current_level >= 0:   # inside a dual_level
+        _no_tangent(logits, u, temperature, top_p, min_p, *(out or {}).values())
     shape = logits.shape
     B, A = shape
     rows = (B,)
@@ -120,39 +112,48 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
         if lt is not torch.uint8 and lt is not torch.bool:
             raise capi.MuZeroError("legal: a uint8 or bool tensor is needed")
         p_legal, s_legal = _tensor(legal, "legal", lt, shape, dev, dense=False), _row_stride(legal)
-    given_t, given_p, given_m = temperature, top_p, min_p
-    temperature, p_t = _setting(temperature, "temperature", torch.float64, rows, dev)
-    top_k, p_k = _setting(top_k, "top_k", torch.int32, rows, dev)
-    top_p, p_p = _setting(top_p, "top_p", torch.float64, rows, dev)
-    min_p, p_m = _setting(min_p, "min_p", torch.float64, rows, dev)
+    p_t = p_k = p_p = p_m = 0   # a number, or a tensor with one per row
+    if type(temperature) not in _NUMBERS and isinstance(temperature, torch.Tensor):
+        p_t, temperature = _tensor(temperature, "temperature", torch.float64, rows, dev), 0
+    if type(top_k) not in _NUMBERS and isinstance(top_k, torch.Tensor):
+        p_k, top_k = _tensor(top_k, "top_k", torch.int32, rows, dev), 0
+    if type(top_p) not in _NUMBERS and isinstance(top_p, torch.Tensor):
+        p_p, top_p = _tensor(top_p, "top_p", torch.float64, rows, dev), 0
+    if type(min_p) not in _NUMBERS and isinstance(min_p, torch.Tensor):
+        p_m, min_p = _tensor(min_p, "min_p", torch.float64, rows, dev), 0
     if type(top_k) is int and top_k >= 2**31:
         top_k = 2**31 - 1
-    if out is None:
+    given = out is not None
+    if not given:
         on = logits.device
         out = dict(action=torch.empty(B, dtype=torch.int32, device=on), logprob=torch.empty(B, dtype=torch.float32, device=on),
                    kept=torch.empty(B, dtype=torch.int32, device=on))
         if probs:
             out["probs"] = torch.empty(B, A, dtype=torch.float32, device=on)
-    get = out.get
-    action, logprob, kept, pr = get("action"), get("logprob"), get("kept"), get("probs")
-    if forward_ad._current_level >= 0:   # inside a dual_level
-        _no_tangent(logits, u, given_t, given_p, given_m, logprob, pr)
+    action, logprob, kept, probs = out.get("action"), out.get("logprob"), out.get("kept"), out.get("probs")
+    p_action, p_logprob, p_kept, p_probs, s_probs = _tensor(action, "out['action']", torch.int32, rows, dev), 0, 0, 0, 0
+    written = [action]
+    if logprob is not None:
+        p_logprob = _tensor(logprob, "out['logprob']", torch.float32, rows, dev)
+        written.append(logprob)
+    if kept is not None:
+        p_kept = _tensor(kept, "out['kept']", torch.int32, rows, dev)
+        written.append(kept)
+    if probs is not None:
+        p_probs, s_probs = _tensor(probs, "out['probs']", torch.float32, shape, dev, dense=False), _row_stride(probs)
+        written.append(probs)
+    p_logits, p_u = _tensor(logits, "logits", t, shape, dev, dense=False), _tensor(u, "u", torch.float64, rows, dev)
     try:
-        args = _SAMPLE.pack(
-            B, A, DTYPES[t], top_k, temperature, top_p, min_p,
-            _tensor(logits, "logits", t, shape, dev, dense=False), _row_stride(logits), p_legal, s_legal,
-            _tensor(u, "u", torch.float64, rows, dev), p_t, p_k, p_p, p_m,
-            _tensor(action, "out['action']", torch.int32, rows, dev),
-            0 if logprob is None else _tensor(logprob, "out['logprob']", torch.float32, rows, dev),
-            0 if kept is None else _tensor(kept, "out['kept']", torch.int32, rows, dev),
-            0 if pr is None else _tensor(pr, "out['probs']", torch.float32, shape, dev, dense=False),
-            0 if pr is None else _row_stride(pr))
+        args = _SAMPLE.pack(B, A, DTYPES[t], top_k, temperature, top_p, min_p, p_logits, _row_stride(logits), p_legal, s_legal, p_u,
+                            p_t, p_k, p_p, p_m, p_action, p_logprob, p_kept, p_probs, s_probs)
     except (struct.error, OverflowError, TypeError) as e:
         raise capi.MuZeroError(f"temperature, top_k, top_p and min_p must be numbers in range ({e})") from None
-    L = _lib()
+    L = _entries or _lib()
     keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(args), workspace, dev)
     if L.mz_sample_actions(args, ws, nbytes, _stream(dev)) != 0:
         _fail()
+    if given:   # a graph that saved one of them must notice
+        _increment_version(written)
     return out
 
 
@@ -169,7 +170,8 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
     M, K = x.shape
     n, r, _ = a.shape
     N = weight.shape[0]
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(M, N, dtype=t if out_dtype is None else out_dtype, device=x.device)
     elif out_dtype is None:
         out_dtype = getattr(out, "dtype", None)
@@ -188,8 +190,10 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
         0 if scale is None else _tensor(scale, "scale", torch.float32, (n,), dev),
         _tensor(index, "index", torch.int32, (M,), dev), _tensor(out, "out", out_dtype, (M, N), dev, dense=False),
         _row_stride(out))
-    L = _lib()
+    L = _entries or _lib()
     keep, ws, nbytes = _workspace(L.mz_adapter_workspace_bytes(args), workspace, dev)
     if L.mz_adapter_linear(args, ws, nbytes, _stream(dev)) != 0:
         _fail()
+    if given:   # a graph that saved it must notice
+        _increment_version([out])
     return out

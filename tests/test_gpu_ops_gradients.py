@@ -87,3 +87,41 @@ def test_derivatives_by_functions_end_in_an_error():
             torch.func.grad(lambda t: f(t).sum())(v)
         with pytest.raises((capi.MuZeroError, RuntimeError)):
             torch.func.vmap(f)(v[None])
+
+
+@pytest.mark.parametrize("name", ["logprob", "probs"])
+def test_a_graph_notices_that_its_saved_sample_was_overwritten(name):
+    given, out = sample_arguments()
+    ops.sample_actions(**given, out=out)
+    w = torch.ones_like(out[name], requires_grad=True)
+    y = (w * out[name]).sum()
+    ops.sample_actions(**given, out={k: v for k, v in out.items() if k != name})
+    y.backward(retain_graph=True)
+    ops.sample_actions(**given, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_a_graph_notices_that_its_saved_projection_was_overwritten():
+    s = make(np.random.default_rng(4), 6, 40, 24, 3, 2, "fp32")
+    out = ops.adapter_linear(**s)
+    w = torch.ones_like(out, requires_grad=True)
+    y = (w * out).sum()
+    ops.adapter_linear(**s)
+    y.backward(retain_graph=True)
+    ops.adapter_linear(**s, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_outputs_made_in_inference_mode():
+    s = make(np.random.default_rng(5), 6, 40, 24, 3, 2, "fp32")
+    given, _ = sample_arguments()
+    with torch.inference_mode():
+        _, out = sample_arguments()
+        ops.sample_actions(**given, out=out)
+        y = torch.empty(6, 24, device="cuda")
+        check_adapter(s, "fp32", out=y)
+    with torch.no_grad():
+        ops.sample_actions(**given, out=out)
+        check_adapter(s, "fp32", out=y)
