@@ -147,7 +147,7 @@ def sample_actions(logits, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, m
         args = _SAMPLE.pack(B, A, DTYPES[t], top_k, temperature, top_p, min_p, p_logits, _row_stride(logits), p_legal, s_legal, p_u,
                             p_t, p_k, p_p, p_m, p_action, p_logprob, p_kept, p_probs, s_probs)
     except (struct.error, OverflowError, TypeError) as e:
-        raise capi.MuZeroError(f"temperature, top_k, top_p and min_p must be numbers in range ({e})") from None
+        raise capi.MuZeroError(f"sizes, temperature, top_k, top_p and min_p must be numbers in range ({e})") from None
     L = _entries or _lib()
     keep, ws, nbytes = _workspace(L.mz_sample_workspace_bytes(args), workspace, dev)
     if L.mz_sample_actions(args, ws, nbytes, _stream(dev)) != 0:
@@ -181,15 +181,18 @@ def adapter_linear(x, weight, a, b, index, bias=None, scale=None, out_dtype=None
         raise capi.MuZeroError(f"out: {out_dtype} is not supported")
     if forward_ad._current_level >= 0:   # inside a dual_level
         _no_tangent(x, weight, a, b, bias, scale, out)
-    args = _ADAPTER.pack(
-        M, K, N, r, n, DTYPES[t], DTYPES[out_dtype], 0,
-        _tensor(x, "x", t, (M, K), dev, dense=False), _row_stride(x),
-        _tensor(weight, "weight", t, (N, K), dev, dense=False), _row_stride(weight),
-        0 if bias is None else _tensor(bias, "bias", t, (N,), dev),
-        _tensor(a, "a", t, (n, r, K), dev), _tensor(b, "b", t, (n, N, r), dev),
-        0 if scale is None else _tensor(scale, "scale", torch.float32, (n,), dev),
-        _tensor(index, "index", torch.int32, (M,), dev), _tensor(out, "out", out_dtype, (M, N), dev, dense=False),
-        _row_stride(out))
+    try:
+        args = _ADAPTER.pack(
+            M, K, N, r, n, DTYPES[t], DTYPES[out_dtype], 0,
+            _tensor(x, "x", t, (M, K), dev, dense=False), _row_stride(x),
+            _tensor(weight, "weight", t, (N, K), dev, dense=False), _row_stride(weight),
+            0 if bias is None else _tensor(bias, "bias", t, (N,), dev),
+            _tensor(a, "a", t, (n, r, K), dev), _tensor(b, "b", t, (n, N, r), dev),
+            0 if scale is None else _tensor(scale, "scale", torch.float32, (n,), dev),
+            _tensor(index, "index", torch.int32, (M,), dev), _tensor(out, "out", out_dtype, (M, N), dev, dense=False),
+            _row_stride(out))
+    except struct.error as e:
+        raise capi.MuZeroError(f"sizes must be below 2^31 ({e})") from None
     L = _entries or _lib()
     keep, ws, nbytes = _workspace(L.mz_adapter_workspace_bytes(args), workspace, dev)
     if L.mz_adapter_linear(args, ws, nbytes, _stream(dev)) != 0:
