@@ -978,41 +978,35 @@ Plan make_plan(const AdapterOp& op) {
 }
 
 template <typename T, int MT, int NT, int FJ>
-void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
+hipError_t launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
     const size_t lds = skinny_lds<MT, NT, FJ>() + 16 * MT * 4 + (size_t)std::min(op.rows, 16 * MT) * padded_rank(op.rank) * 4;
     lds_optin((const void*)k_skinny<T, MT, NT, FJ>);
-    k_skinny<T, MT, NT, FJ><<<dim3((op.N + 16 * NT - 1) / (16 * NT), (op.rows + 16 * MT - 1) / (16 * MT)), dim3(64 * kSkinnyWaves<MT>), lds, st>>>(op, part, splits);
+    const dim3 grid((op.N + 16 * NT - 1) / (16 * NT), (op.rows + 16 * MT - 1) / (16 * MT));
+    return launch_kernel(st, grid, dim3(64 * kSkinnyWaves<MT>), lds, k_skinny<T, MT, NT, FJ>, op, part, splits);
 }
 template <typename T, int MT, int FJ>
-void launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits, int nt) {
-    if (nt == 1) launch_skinny<T, MT, 1, FJ>(st, op, part, splits);
-    else if (nt == 2) launch_skinny<T, MT, 2, FJ>(st, op, part, splits);
-    else launch_skinny<T, MT, 3, FJ>(st, op, part, splits);
+hipError_t launch_skinny(hipStream_t st, const AdapterOp& op, const float* part, int splits, int nt) {
+    if (nt == 1) return launch_skinny<T, MT, 1, FJ>(st, op, part, splits);
+    if (nt == 2) return launch_skinny<T, MT, 2, FJ>(st, op, part, splits);
+    return launch_skinny<T, MT, 3, FJ>(st, op, part, splits);
 }
 template <typename T, int B, int WM, int WN>
-void launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
+hipError_t launch_tile(hipStream_t st, const AdapterOp& op, const float* part, int splits) {
     const int nt = ((op.rows + B - 1) / B) * ((op.N + B - 1) / B);
     const size_t es = sizeof(T), ring = kTileGroups<B> * kRing * tile_stage_bytes<B, B>(), tl = (size_t)B * (padded_rank(op.rank) + 4) * 4;
     const bool dma = ((uintptr_t)op.x | (uintptr_t)op.w) % 16 == 0 && op.x_stride * es % 16 == 0 && op.w_stride * es % 16 == 0 &&
                      (long long)B * op.x_stride * (long long)es < (1ll << 31) && (long long)B * op.w_stride * (long long)es < (1ll << 31);
     const size_t lds = kOrderBytes<B> + (ring > tl ? ring : tl);
-    if (dma) {
-        lds_optin((const void*)k_tile<T, B, B, WM, WN, true>);
-        k_tile<T, B, B, WM, WN, true><<<dim3(nt), dim3(64 * WM * WN * kTileGroups<B>), lds, st>>>(op, part, splits);
-    } else {
-        lds_optin((const void*)k_tile<T, B, B, WM, WN, false>);
-        k_tile<T, B, B, WM, WN, false><<<dim3(nt), dim3(64 * WM * WN * kTileGroups<B>), lds, st>>>(op, part, splits);
-    }
+    const auto kernel = dma ? k_tile<T, B, B, WM, WN, true> : k_tile<T, B, B, WM, WN, false>;
+    lds_optin((const void*)kernel);
+    return launch_kernel(st, dim3(nt), dim3(64 * WM * WN * kTileGroups<B>), lds, kernel, op, part, splits);
 }
 template <typename T, int BR>
-void launch_shrink(hipStream_t st, const AdapterOp& op, float* part, int splits) {
+hipError_t launch_shrink(hipStream_t st, const AdapterOp& op, float* part, int splits) {
     constexpr int NTH = 64 * kShrinkWaves<BR>;
     const dim3 grid((op.rows + BR - 1) / BR, splits, kShrinkParts<BR>);
     const int rt = padded_rank(op.rank) / 16;
-    if (rt == 1) k_shrink<T, 1, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
-    else if (rt == 2) k_shrink<T, 2, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
-    else if (rt <= 4) k_shrink<T, 4, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
-    else k_shrink<T, 8, BR><<<grid, dim3(NTH), 0, st>>>(op, part, splits);
+    return launch_kernel(st, grid, dim3(NTH), 0, rt == 1 ? k_shrink<T, 1, BR> : rt == 2 ? k_shrink<T, 2, BR> : rt <= 4 ? k_shrink<T, 4, BR> : k_shrink<T, 8, BR>, op, part, splits);
 }
 
 template <typename T>
@@ -1020,26 +1014,25 @@ hipError_t launch_typed(hipStream_t st, const AdapterOp& op, void* workspace) {
     const Plan p = make_plan(op);
     float* part = static_cast<float*>(workspace);
     if (!p.fused) {
-        if (p.block == 16) launch_shrink<T, 16>(st, op, part, p.splits);
-        else launch_shrink<T, 128>(st, op, part, p.splits);
-        if (hipError_t e = hipGetLastError()) return e;
+        if (hipError_t e = p.block == 16 ? launch_shrink<T, 16>(st, op, part, p.splits) : launch_shrink<T, 128>(st, op, part, p.splits)) return e;
     }
+    hipError_t e = hipErrorInvalidConfiguration;
     if (p.skinny) {
-        if (p.fused && op.rows * padded_rank(op.rank) == 16) launch_skinny<T, 1, 1>(st, op, part, p.splits, p.nt);
-        else if (p.fused) launch_skinny<T, 1, 2>(st, op, part, p.splits, p.nt);
-        else if (p.mt == 1) launch_skinny<T, 1, 0>(st, op, part, p.splits, p.nt);
-        else if (p.mt == 2) launch_skinny<T, 2, 0>(st, op, part, p.splits, p.nt);
-        else if (p.mt == 3) launch_skinny<T, 3, 0>(st, op, part, p.splits, p.nt);
-        else launch_skinny<T, 4, 0>(st, op, part, p.splits, p.nt);
+        if (p.fused && op.rows * padded_rank(op.rank) == 16) e = launch_skinny<T, 1, 1>(st, op, part, p.splits, p.nt);
+        else if (p.fused) e = launch_skinny<T, 1, 2>(st, op, part, p.splits, p.nt);
+        else if (p.mt == 1) e = launch_skinny<T, 1, 0>(st, op, part, p.splits, p.nt);
+        else if (p.mt == 2) e = launch_skinny<T, 2, 0>(st, op, part, p.splits, p.nt);
+        else if (p.mt == 3) e = launch_skinny<T, 3, 0>(st, op, part, p.splits, p.nt);
+        else e = launch_skinny<T, 4, 0>(st, op, part, p.splits, p.nt);
     } else if (sizeof(T) == 2 && p.tile == 256) {
-        if constexpr (sizeof(T) == 2) launch_tile<T, 256, 4, 2>(st, op, part, p.splits);
+        if constexpr (sizeof(T) == 2) e = launch_tile<T, 256, 4, 2>(st, op, part, p.splits);
     } else if (p.tile == 128) {
-        launch_tile<T, 128, 2, 2>(st, op, part, p.splits);
+        e = launch_tile<T, 128, 2, 2>(st, op, part, p.splits);
     } else {
-        launch_tile<T, 64, 2, 2>(st, op, part, p.splits);
+        e = launch_tile<T, 64, 2, 2>(st, op, part, p.splits);
     }
-    if (hipError_t e = take_optin_error()) return e;
-    return hipGetLastError();
+    if (hipError_t o = take_optin_error()) return o;
+    return e;
 }
 
 }  // namespace

@@ -6,10 +6,24 @@
 #include <stdint.h>
 
 #include <string>
+#include <tuple>
 
 namespace mz {
 
 int op_fail(const std::string& msg);   // text for mz_last_error(NULL); returns -1
+
+// Queues a kernel; the status is this launch's own.  (hipGetLastError after <<<>>> also gives what an earlier call of the thread, of
+// whatever library, has left behind.)
+template <typename... P, typename... A>
+hipError_t launch_kernel(hipStream_t st, dim3 grid, dim3 block, size_t lds, void (*kernel)(P...), A... a) {
+    std::tuple<P...> held(a...);
+    return std::apply(
+        [&](P&... p) {
+            void* args[] = {&p...};
+            return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, args, lds, st);
+        },
+        held);
+}
 
 enum OpType { kFp32 = 0, kBf16 = 1, kF16 = 2 };   // MZ_DTYPE_*
 

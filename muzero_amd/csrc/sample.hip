@@ -1301,23 +1301,19 @@ template <typename T>
 hipError_t launch_typed(hipStream_t st, const SampleOp& op, void* workspace) {
     if (op.actions <= 4 * W) {
         const dim3 grid((op.rows + kWaveRows - 1) / kWaveRows), block(W * kWaveRows);
-        if (op.actions <= W) k_sample_wave<T, 1><<<grid, block, 0, st>>>(op);
-        else if (op.actions <= 2 * W) k_sample_wave<T, 2><<<grid, block, 0, st>>>(op);
-        else k_sample_wave<T, 4><<<grid, block, 0, st>>>(op);
+        return launch_kernel(st, grid, block, 0, op.actions <= W ? k_sample_wave<T, 1> : op.actions <= 2 * W ? k_sample_wave<T, 2> : k_sample_wave<T, 4>, op);
     } else if (op.actions <= 8192 || (op.rows > 256 && op.actions <= 64ll * op.rows)) {
         // Several workgroups to a CU hide one another's serial parts; a CU with one row needs all its waves.  256 and 1024 threads, top-p
         // 0.9 of bf16: 64 rows of 8192 10.9 and 13.2 us, 256 of 16384 39.2 and 33.9, 512 of 16384 47.4 and 63.6, 512 of 65536 156 and 148,
         // 1024 of 32768 139 and 171, 2048 of 16384 141 and 246, 256 of 131072 240 and 131
-        k_sample_block<T, 256><<<dim3(op.rows), dim3(256), 0, st>>>(op);
+        return launch_kernel(st, dim3(op.rows), dim3(256), 0, k_sample_block<T, 256>, op);
     } else if (const int ls = log_splits(op)) {
         SplitRow* rows = static_cast<SplitRow*>(workspace);
-        k_sample_maxima<T><<<dim3(op.rows << ls), dim3(kSplitThreads), 0, st>>>(op, rows, ls);
-        if (hipError_t e = hipGetLastError()) return e;
-        k_sample_split<T><<<dim3(op.rows << ls), dim3(kSplitThreads), 0, st>>>(op, rows, ls);
-    } else {
-        k_sample_block<T, 1024><<<dim3(op.rows), dim3(1024), 0, st>>>(op);
+        const dim3 grid(op.rows << ls), block(kSplitThreads);
+        if (hipError_t e = launch_kernel(st, grid, block, 0, k_sample_maxima<T>, op, rows, ls)) return e;
+        return launch_kernel(st, grid, block, 0, k_sample_split<T>, op, rows, ls);
     }
-    return hipGetLastError();
+    return launch_kernel(st, dim3(op.rows), dim3(1024), 0, k_sample_block<T, 1024>, op);
 }
 
 }  // namespace
