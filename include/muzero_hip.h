@@ -307,7 +307,10 @@ enum { MZ_DTYPE_FP32 = 0, MZ_DTYPE_BF16 = 1, MZ_DTYPE_F16 = 2 }; /* the numbers 
  *   action = the first kept entry in INDEX order at which the running sum of w exceeds u * (sum of the kept), u in [0, 1].
  *   temperature == 0: the first of the ranking, whatever u.  +inf entries share all the weight.
  * A row with no such entry, and a row whose u or per-row parameter is out of range or NaN, gets action -1, kept 0, logprob 0
- * and probs 0.  Weights and sums are 64-bit; a row's result does not depend on the other rows. */
+ * and probs 0.  Weights are 64-bit; their sums are 64-bit, or (top_p over long rows) exact sums of the weights rounded to 45 bits, those
+ * below 2^-63 of the largest left out.  A row's result does not depend on what other rows hold.  Their number chooses among kernels, and
+ * with it the order of the sums: a row alone and in a batch agree but for the last bits of logprob and probs, and for an action or
+ * count where u or top_p lies within that rounding of a border.  The same call gives the same bits. */
 typedef struct mz_sample_args {
     int32_t rows, actions;          /* rows: 0 .. 2097152, actions: 1 .. 262144 */
     int32_t dtype;                  /* MZ_DTYPE_* of logits */
@@ -335,8 +338,8 @@ int mz_sample_actions(const mz_sample_args* args, void* workspace, size_t worksp
  *   y[m] = x[m] W^T + bias + scale[i] * (x[m] A[i]^T) B[i]^T,   i = index[m]
  * index -1: the shared projection alone; any other index outside [0, adapters) makes the row NaN.  Sums are fp32 (inputs of
  * 16 bits on 16-bit matrix instructions, fp32 on fp32 ones), x A^T keeps the precision of fp32 between its two products, and y is
- * rounded once to its type.  Rows do not influence one another:
- * a row's inf or NaN, or an adapter's, stay with the rows that use them. */
+ * rounded once to its type.  Rows do not influence one another: a row's inf or NaN, or an adapter's, stay with the rows that use them.
+ * The numbers of rows and adapters choose among kernels, and with it the order of the sums; the same call gives the same bits. */
 typedef struct mz_adapter_args {
     int32_t rows, in_features, out_features; /* both features <= 2^26, ceil(rows / 256) * ceil(out_features / 256) <= 2^21 */
     int32_t rank, adapters;         /* rank: 1 .. 128; shorter adapters are padded with zeros */

@@ -7,7 +7,8 @@
 //     draw: the first kept i in INDEX order with sum_{j <= i, kept} w_j > u * S,  S = the kept mass.
 // Whether an entry is kept and which is drawn are decided by sums next to a border, so weights and sums are 64-bit: an entry of
 // relative weight 1e-7 next to the border of a nucleus must not depend on the order of a sum.  Sums run in a fixed order, or
-// (histograms, whose LDS atomics arrive in any order) in exact integers, so a row's answer is a function of the row alone.
+// (histograms, whose LDS atomics arrive in any order) in exact integers, so a row's answer is a function of the row and of the kernel,
+// which goes by the numbers of rows and actions; between kernels the order of the sums differs.
 //
 //   A <= 256   k_sample_wave: a wavefront per row, the row in registers (<= 4 entries a lane); ranking = bitonic sort of
 //              the keys over the lanes.  Bound by the issue of vector instructions, 64-bit exponentials first: 16384 rows of 82 with
