@@ -20,7 +20,7 @@ struct Operands {
     int device = -1;
     const char* bad = nullptr;
     std::string why;
-    struct Block {   // rows of `width` bytes, `pitch` bytes apart
+    struct Block {   // rows of `width` bytes, `pitch` bytes apart (0: one row)
         const char* name;
         uintptr_t at;
         unsigned __int128 end;
@@ -33,7 +33,7 @@ struct Operands {
     void add(const void* p, const char* name, size_t align, size_t rows, size_t pitch, size_t width, bool written) {
         if (bad || !p) return;
         const uintptr_t at0 = reinterpret_cast<uintptr_t>(p);
-        const Block b{name, at0, (unsigned __int128)(rows - 1) * pitch + width + at0, pitch, width, written};
+        const Block b{name, at0, (unsigned __int128)(rows - 1) * pitch + width + at0, rows > 1 ? pitch : 0, width, written};
         for (int i = 0; i < blocks; i++)
             if ((written || block[i].written) && overlap(block[i], b)) return fail(name, (std::string("overlaps ") + block[i].name).c_str());
         block[blocks++] = b;
@@ -52,9 +52,10 @@ struct Operands {
     }
     static bool overlap(const Block& a, const Block& b) {
         if (a.end <= b.at || b.end <= a.at) return false;
-        if (a.pitch != b.pitch || a.pitch == 0) return true;
-        const uintptr_t d = (b.at % a.pitch + a.pitch - a.at % a.pitch) % a.pitch;   // columns of the same wide rows
-        return !(d >= a.width && d + b.width <= a.pitch);
+        const uintptr_t pitch = a.pitch ? a.pitch : b.pitch;   // one row may stand in any wide row
+        if (pitch == 0 || (a.pitch && b.pitch && a.pitch != b.pitch)) return true;
+        const uintptr_t d = (b.at % pitch + pitch - a.at % pitch) % pitch;   // columns of the same wide rows
+        return !(d >= a.width && d + b.width <= pitch);
     }
     void fail(const char* name, const char* what) {
         bad = name;
