@@ -516,9 +516,10 @@ __global__ __launch_bounds__(64 * kSkinnyWaves<MT>) void k_skinny(AdapterOp op, 
 // LDS: a ring of stages, each 64 bytes of k (4 chunks) of BM rows of x and BN rows of W.  Chunk c of row r stands at slot
 // c ^ (r >> 1 & 3): the 8 lanes that an LDS read serves at a time then hit 8 different 16-byte columns.
 // DMA: rows of both operands are 16-byte aligned: global -> LDS without registers, three stages ahead.  Otherwise through registers.
-// With and without it, bf16: 8192x4096x4096 331 and 368 us, 2048x2048x2048 49.3 and 59.3, 1000x2048x2000 37.0 and 37.4.
-// Bound by LDS reads beside the matrix instructions where tiles are large (8192x4096x4096: 280 us, 0.98 PFLOP/s, the library's bare product
-// 1.33), by what each workgroup brings from L2 where they are small (1000x2050x1999: 37.5 us, 268 MB, 7 TB/s).
+// With and without it, bf16, whole calls: 8192x4096x4096 273 and 310 us, 2048x2048x2048 43.4 and 52.9, 1000x2048x2000 32.2 and 33.7.
+// Bound by LDS reads, barriers and their waits beside the matrix instructions where tiles are large (8192x4096x4096: 293 us in a trace,
+// 0.94 PFLOP/s, matrix pipes busy 49 % of the time; the library's bare product 1.33), by what each workgroup brings from L2 where they are
+// small (1000x2050x1999: 38.4 us, 268 MB, 7 TB/s).
 template <int BM, int BN>
 constexpr size_t tile_stage_bytes() {
     return (size_t)(BM + BN) * 64;
@@ -919,11 +920,13 @@ constexpr int kCus = 256;
 // Tiles of 64 x 64 that leave half of the chip idle or more, each of which walks all of K alone: k_skinny's workgroups are smaller and
 // share K out over their waves.  Tiles against those, bf16 unless said: 720x939x98 (24 tiles) 33.1 and 22.8 us, 256x1024x1024 (64)
 // 15.8 and 13.3, 256x2048x1024 fp32 (64) 50.6 and 31.1, 512x4098x1024 (128) 45.4 and 39.3, 512x1024x1024 (128) 16.8 both,
-// 256x4096x2048 (128) 31.3 and 34.3, 256x4096x4096 (256) 33.5 and 60.9.
+// 256x4096x2048 (128) 31.3 and 34.3, 256x4096x4096 (256) 33.5 and 60.9.  (At 128 tiles the faster one goes by the shape, which the rule
+// does not: up to a tenth lost.)
 constexpr int kFewTiles = 128;
 // Above it, W is streamed for few rows.  That against tiles, W from memory, bf16, 4096 to 11000: 16 rows 30.8 and 38.2 us, 32 rows 32.8
 // and 45.6, 48 rows 37.4 and 45.3, 64 rows 43.0 and 45.3; 4096 to 16384, where the last round of workgroups is not full: 32 rows 49.0
-// and 52.8, 48 rows 56.9 and 51.5, 64 rows 64.1 and 52.2.  fp32, 4096 to 11000: 32 rows 69.4 and 92.5, 48 rows 104 and 91.9.
+// and 52.8, 48 rows 56.9 and 51.5, 64 rows 64.1 and 52.2.  fp32, 4096 to 11000: 32 rows 69.4 and 92.5, 48 rows 104 and 91.9.  (Between 33
+// and 64 rows the faster one also goes by the number of outputs, which the rule does not: up to a tenth lost.)
 constexpr int kSkinnyRows16 = 48, kSkinnyRows32 = 32;
 
 Plan make_plan(const AdapterOp& op) {

@@ -22,6 +22,8 @@
 //              bf16 entries: with top-k 50 30 us (2.2 TB/s), with top-p 0.9 131 us, bound by vector and LDS atomic work per entry.
 //   few long rows   k_sample_maxima + k_sample_split: 2 to 16 workgroups per row, the last to finish ranks the candidates of
 //              all; 64 rows of 50257 fp32 entries, top-k 40 and top-p 0.95: 16 us, bound by latency (two launches, one wave's end).
+//              Rows that no short cut serves are left to one workgroup each: one row of 131072 bf16, top-p 0.9 100 us, no filter
+//              46, top-k 1000 79.
 #include "ops.h"
 
 #include <float.h>
@@ -1292,7 +1294,8 @@ __global__ __launch_bounds__(kSplitThreads) void k_sample_split(SampleOp op, Spl
 
 // 0: a workgroup per row.  Splitting pays while workgroups of one row each leave most of the chip idle, and a row is long enough
 // to be worth a second launch: one row of 131072 bf16 entries (top-k 50) 20.8 us whole, 12.2 by 16 workgroups; 64 rows 22.0, by 4 16.4;
-// 64 rows of 50000 14.9 and 13.8, of 32768 12.8 and 13.0, of 24000 12.1 and 13.6; 100 rows of 131072 22.2, by 2 19.4, of 50000 15.4 and 15.5.
+// 64 rows of 50000 14.9 and 13.8, of 32768 12.8 and 13.0, of 24000 12.1 and 13.6; one row of 32768 11.3 and 12.6, of 24000 10.4 and 22.9;
+// 100 rows of 131072 22.2, by 2 19.4, of 50000 15.4 and 15.5.
 inline int log_splits(const SampleOp& op) {
     if (op.rows > 128 || op.actions < (op.rows <= 64 ? 49152 : 98304)) return 0;
     return op.rows <= 16 ? 4 : op.rows <= 32 ? 3 : op.rows <= 64 ? 2 : 1;
