@@ -770,10 +770,10 @@ __global__ __launch_bounds__(64 * WM * WN * kTileGroups<BM>, 2) void k_tile(Adap
     const auto add_term = [&](auto J) __attribute__((always_inline)) {
         constexpr int j = J.value;
         const int p = wm + j * 16 + lr, own = key[p];
-        // bf16: t as the sum of three bf16 numbers, exactly.  fp16: t scaled by a power of two to a maximum in [2^14, 2^15), as the sum of two fp16 numbers: within 2^-24 of its value down to
+        // bf16: t as the sum of three bf16 numbers, exactly (from 2^-100 on, so that the third is a normal one).  fp16: t scaled by a power of two to a maximum in [2^14, 2^15), as the sum of two fp16 numbers: within 2^-24 of its value down to
         // 2^-15 of the maximum, where their subnormal step, 2^-24, begins to tell.  Below that a third number, 2^24 times larger, takes what
-        // they leave (`wide`), down to 2^-38 of the maximum, where the first is not 0 yet.  Rows whose ranks are still further apart, and
-        // rows of both types with an inf or a NaN, are summed by themselves.  All of this goes by the row's own t alone.
+        // they leave (`wide`), down to 2^-38 of the maximum, where the first is not 0 yet.  Rows whose ranks are still further apart (bf16:
+        // below 2^-100), and rows with an inf or a NaN, are summed by themselves.  All of this goes by the row's own t alone.
         bool by_itself = per_row, wide = false;
         float back = 1.f, to = 1.f;
         if (sizeof(T) == 2 && !per_row) {
@@ -787,10 +787,11 @@ __global__ __launch_bounds__(64 * WM * WN * kTileGroups<BM>, 2) void k_tile(Adap
                 }
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            by_itself = !(mx < INFINITY);
-            if constexpr (__is_same(T, _Float16)) {
-                mn = fminf(mn, __shfl_xor(mn, 16));
-                mn = fminf(mn, __shfl_xor(mn, 32));
+            mn = fminf(mn, __shfl_xor(mn, 16));
+            mn = fminf(mn, __shfl_xor(mn, 32));
+            if constexpr (__is_same(T, bf16_t)) {
+                by_itself = !(mx < INFINITY) || mn < 0x1p-100f;
+            } else {
                 if (mx > 0) {
                     by_itself = mx > 0x1p100f || mx < 0x1p-80f || mn < mx * 0x1p-38f;
                     wide = mn < mx * 0x1p-15f;

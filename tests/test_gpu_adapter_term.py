@@ -158,3 +158,16 @@ def test_ranks_as_far_apart_as_fp16_goes():
         s["b"][1, ::7, 1] = float("inf")
         s["b"][2, ::9, 0] = float("-inf")
         check(s)
+
+
+@pytest.mark.parametrize("n", [3, 24])
+def test_t_near_the_smallest_numbers(n):
+    """bf16: t down to subnormal fp32 numbers, B making up for it; and beside ranks of ordinary size."""
+    for small in (1e-31, 1e-34, 1e-36, 1e-37):
+        s = make(np.random.default_rng(5), TILES[64][0], 16, TILES[64][1], 5, n, "bf16")
+        s["a"] *= small
+        s["b"] *= 1 / small
+        check(s)
+        s["a"][:, 0] *= 1 / small
+        s["b"][:, :, 0] = 0
+        check(s)
